@@ -590,6 +590,8 @@ std::vector<Tensor> bipartite_attn_bwd(Tensor q, Tensor k, Tensor v,
 
 }  // namespace
 
+void bind_rows(pybind11::module& m);  // ext_rows.hip
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "gansformer_amd gfx950 HIP kernels";
   m.def("fba", &fba, "fused bias+act (grad=0) / grad variant (grad=1)");
@@ -614,4 +616,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "fused attention backward -> (dq, dk, dv)");
   m.def("gemm_skinny", &gemm_skinny,
         "tall-skinny C = A @ op(B) MFMA GEMM");
+  bind_rows(m);
 }

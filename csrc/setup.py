@@ -24,7 +24,7 @@ sources = [os.path.join(CSRC, f) for f in (
     "conv2d_wgrad_slab.hip", "conv2d_up2.hip", "conv2d_s2.hip",
     "upfirdn2d_sep.hip", "modnorm.hip",
     "mbstd.hip", "attn.hip", "attn_bwd.hip", "gemm_skinny.hip",
-    "pack.hip")]
+    "pack.hip", "layer_norm.hip", "linear_act.hip", "ext_rows.hip")]
 
 setup(
     name="gansformer_amd_ext",

@@ -22,3 +22,5 @@ from .mbstd import minibatch_stddev  # noqa: F401
 from .modnorm import modnorm  # noqa: F401
 from .linear import linear_nobias, linear_transposed  # noqa: F401
 from .bipartite import bipartite_attention  # noqa: F401
+from .layer_norm import layer_norm  # noqa: F401
+from .linear_act import linear_act, linear_activations  # noqa: F401

@@ -1,0 +1,141 @@
+"""Matrix product with bias, activation and residual in its epilogue.
+
+    z = weight_gain * x @ weight^T + bias_gain * bias
+    y = clamp(act(z) * gain) + residual
+
+One kernel where `linear_nobias` and `bias_act` take a scaled copy of the
+weight, a library product, a bias/activation pass and an addition. Backward:
+
+    dz = dy * gain * act'(z), zero where the clamp holds
+    dx = weight_gain * dz @ weight      dweight = weight_gain * dz^T @ x
+    dbias = bias_gain * sum_rows dz     dresidual = dy
+
+z is kept for the backward in x's dtype where the activation (or a clamp)
+needs it. All four products run on the kernels of csrc/linear_act.hip; a
+create_graph backward goes through the differentiable composition.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import native
+from .fused_act import _eager_act, activation_defs
+from .layer_norm import _GPU_DTYPES, _check_param, _eager_grads
+
+# bias_act's activations and the two smooth ones of feed-forward layers:
+# gelu(z) = z * Phi(z) (exact, by erf) and silu(z) = z * sigmoid(z)
+linear_activations = {
+    **activation_defs,
+    "gelu": (5, 0.0, 1.0, True),
+    "silu": (6, 0.0, 1.0, True),
+}
+
+
+def _act(z, act, alpha):
+    if act == "gelu":
+        return z * 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5)))
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    return _eager_act(z, act, alpha)
+
+
+def _eager_linear_act(x, weight, bias, residual, act, alpha, gain, clamp,
+                      weight_gain, bias_gain):
+    ft = torch.float64 if x.dtype == torch.float64 else torch.float32
+    z = x.to(ft).matmul(weight.to(ft).t()) * weight_gain
+    if bias is not None:
+        z = z + bias.to(ft) * bias_gain
+    y = _act(z, act, alpha) * gain
+    if clamp is not None:
+        y = y.clamp(-clamp, clamp)
+    if residual is not None:
+        y = y + residual.to(ft)
+    return y.to(x.dtype)
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, alpha, gain, clamp,
+                weight_gain, bias_gain):
+        code = linear_activations[act][0]
+        # a linear layer's slope is the gain everywhere
+        keep = act != "linear" or clamp is not None
+        y, z = native.require_ext().linear_act_fwd(
+            x, weight, bias, residual, code, alpha, gain,
+            math.inf if clamp is None else clamp, weight_gain, bias_gain,
+            keep)
+        ctx.save_for_backward(x, weight, bias, residual, z)
+        ctx.params = (act, alpha, gain, clamp, weight_gain, bias_gain)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, bias, residual, z = ctx.saved_tensors
+        act, alpha, gain, clamp, weight_gain, bias_gain = ctx.params
+        need = ctx.needs_input_grad
+        if torch.is_grad_enabled():
+            return _eager_grads(
+                lambda *t: _eager_linear_act(*t, *ctx.params),
+                (x, weight, bias, residual), need, dy) + (None,) * 6
+        dx, dw, db = native.require_ext().linear_act_bwd(
+            dy, z, x, weight, bias, linear_activations[act][0], alpha, gain,
+            math.inf if clamp is None else clamp, weight_gain, bias_gain,
+            need[0], need[1], need[2])
+        return (dx, dw, db, dy if need[3] else None) + (None,) * 6
+
+
+def linear_act(x, weight, bias=None, act="linear", residual=None, alpha=None,
+               gain=None, clamp=None, weight_gain=1.0, bias_gain=1.0):
+    """clamp(act(weight_gain * x @ weight^T + bias_gain * bias) * gain)
+    + residual.
+
+    x: [..., K]; weight: [N, K] in x's dtype; bias: [N] in x's dtype or
+    float32; residual: [..., N] in x's dtype, added after the clamp. act is
+    one of `linear_activations`, with `bias_act`'s default alpha and gain.
+    clamp: None or negative for none. Returns [..., N] in x's dtype, rounded
+    once from 32 bits. On the GPU x is float32 or bfloat16; x, weight and
+    residual may have strided rows.
+    """
+    if act not in linear_activations:
+        raise ValueError(f"linear_act: unknown activation {act!r}")
+    if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"linear_act: x {tuple(x.shape)} and weight "
+                         f"{tuple(weight.shape)} do not fit")
+    n, k = weight.shape
+    if n < 1 or k < 1:
+        raise ValueError(f"linear_act: empty weight {tuple(weight.shape)}")
+    if weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f"linear_act: weight is {weight.dtype} on "
+                         f"{weight.device}, x {x.dtype} on {x.device}")
+    _check_param("linear_act: bias", bias, x, (n,))
+    if residual is not None:
+        if residual.shape != x.shape[:-1] + (n,):
+            raise ValueError(f"linear_act: residual {tuple(residual.shape)} "
+                             f"does not fit the output "
+                             f"{tuple(x.shape[:-1]) + (n,)}")
+        if residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError(f"linear_act: residual is {residual.dtype} on "
+                             f"{residual.device}, x {x.dtype} on {x.device}")
+    _, def_alpha, def_gain, _ = linear_activations[act]
+    alpha = float(def_alpha if alpha is None else alpha)
+    gain = float(def_gain if gain is None else gain)
+    clamp = None if clamp is None or clamp < 0 else float(clamp)
+    if not native.use_native(x):
+        return _eager_linear_act(x, weight, bias, residual, act, alpha, gain,
+                                 clamp, weight_gain, bias_gain)
+    if x.dtype not in _GPU_DTYPES:
+        raise ValueError(f"linear_act: expected float32 or bfloat16 on the "
+                         f"GPU, got {x.dtype}")
+    if torch.is_grad_enabled() and (
+            x.requires_grad or weight.requires_grad
+            or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad)):
+        return _LinearAct.apply(x, weight, bias, residual, act, alpha, gain,
+                                clamp, float(weight_gain), float(bias_gain))
+    return native.require_ext().linear_act_fwd(
+        x, weight, bias, residual, linear_activations[act][0], alpha, gain,
+        math.inf if clamp is None else clamp, weight_gain, bias_gain,
+        False)[0]

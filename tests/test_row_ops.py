@@ -1,0 +1,735 @@
+"""layer_norm and linear_act against their definitions in 64 bits.
+
+Tolerances are bounds, derived here from the arithmetic and not from runs.
+u = 2^-24 is a float rounding. A sum of k products in float in any order is
+off by at most k u sum|a b| (to first order), whatever the order. A value
+stored as bf16 is off by at most half a step, 2^-8 of it; HALF[t] is that
+half step of a type. Errors pass through an activation times the largest
+slope, SLOPE, and through a slope times its largest derivative, CURVE.
+"""
+
+import math
+
+import pytest
+import torch
+from torch.autograd import gradcheck, gradgradcheck
+
+from gansformer_amd.ops import (bias_act, layer_norm, linear_act,
+                                linear_activations)
+
+U = 2.0 ** -24
+HALF = {t: torch.finfo(t).eps / 2
+        for t in (torch.float32, torch.bfloat16, torch.float64)}
+# largest |act'| and |act''| over the reals (rounded up), before the gain
+SLOPE = {"linear": 1.0, "relu": 1.0, "lrelu": 1.0, "tanh": 1.0,
+         "sigmoid": 0.25, "gelu": 1.13, "silu": 1.1}
+CURVE = {"linear": 0.0, "relu": 0.0, "lrelu": 0.0, "tanh": 0.77,
+         "sigmoid": 0.1, "gelu": 0.8, "silu": 0.5}
+ACTS = list(linear_activations)
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def within(got, want, tol, what=""):
+    got = got.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    off = (got - want).abs() - tol
+    assert torch.isfinite(got).all(), what
+    worst = off.max().item() if off.numel() else -1.0
+    assert worst <= 0, (what, worst, ((got - want).abs() / tol).max().item())
+
+
+# ---------------- the definitions, in 64 bits ----------------
+def ln_parts(x, w, eps=1e-5):
+    x = x.double()
+    mean = x.mean(-1, keepdim=True)
+    rstd = ((x - mean) ** 2).mean(-1, keepdim=True).add(eps).rsqrt()
+    w = torch.ones((), dtype=torch.float64, device=x.device) \
+        if w is None else w.double()
+    return x, mean, rstd, (x - mean) * rstd, w
+
+
+def check_ln(x, w, b, dy=None, got=None):
+    """got: (y,) or (y, dx, dw, db), None where not asked for."""
+    t = x.dtype
+    xd, mean, rstd, xn, wd = ln_parts(x, w)
+    n = x.shape[-1]
+    bd = 0.0 if b is None else b.double()
+    y = xn * wd + bd
+    # The mean is off by a sum's error: a thread adds at most n/64 + 8
+    # values (a wave or a block shares a row) and a tree adds 10 more
+    # levels. That shift, the roundings of x - mean, of rstd and of the two
+    # last operations all act on xn in units of (|x| + mean|x|) rstd.
+    steps = n / 64 + 24
+    scale = (xd.abs() + xd.abs().mean(-1, keepdim=True)) * rstd
+    e_xn = steps * U * scale + steps * U * xn.abs()
+    within(got[0], y, HALF[t] * y.abs() + 1e-30 + e_xn * wd.abs()
+           + 4 * U * ((xn * wd).abs() + abs(bd)), "y")
+    if dy is None:
+        return
+    d = dy.double()
+    g = d * wd
+    m1, m2 = g.mean(-1, keepdim=True), (g * xn).mean(-1, keepdim=True)
+    dx = rstd * (g - m1 - xn * m2)
+    e_m1 = steps * U * g.abs().mean(-1, keepdim=True)
+    e_m2 = steps * U * (g * xn).abs().mean(-1, keepdim=True) \
+        + (g.abs() * e_xn).mean(-1, keepdim=True)
+    big = g.abs() + g.abs().mean(-1, keepdim=True) \
+        + xn.abs() * (g * xn).abs().mean(-1, keepdim=True)
+    if got[1] is not None:
+        within(got[1], dx, HALF[t] * dx.abs() + 1e-30 + rstd * (
+            8 * U * big + steps * U * big + e_m1 + xn.abs() * e_m2
+            + e_xn * m2.abs()), "dx")
+    lead = tuple(range(x.ndim - 1))
+    rows = x.numel() // n
+    for k, (terms, e) in {2: (d * xn, d.abs() * e_xn),
+                          3: (d, torch.zeros_like(d))}.items():
+        if got[k] is None:
+            continue
+        want = terms.sum(lead)
+        tol = rows * U * terms.abs().sum(lead) + e.sum(lead)
+        within(got[k], want, HALF[got[k].dtype] * want.abs() + tol + 1e-30,
+               ("", "", "dw", "db")[k])
+
+
+def act_parts(z, act):
+    """activation and slope of z in 64 bits, before the gain"""
+    if act == "relu":
+        return z.clamp_min(0), (z > 0).double()
+    if act == "lrelu":
+        return torch.where(z > 0, z, 0.2 * z), torch.where(z > 0, 1.0, 0.2).to(z)
+    if act == "tanh":
+        return z.tanh(), 1 - z.tanh() ** 2
+    if act == "sigmoid":
+        s = torch.sigmoid(z)
+        return s, s * (1 - s)
+    if act == "gelu":
+        p = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * p, p + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    return z, torch.ones_like(z)
+
+
+class Linear:
+    """A linear_act call, its values in 64 bits and their tolerances."""
+
+    def __init__(self, x, w, b, res, act="linear", clamp=None, gain=None,
+                 wg=1.0, bg=1.0):
+        self.x, self.w, self.b, self.res = x, w, b, res
+        self.act, self.clamp, self.wg, self.bg = act, clamp, wg, bg
+        self.gain = linear_activations[act][2] if gain is None else gain
+        self.kw = dict(act=act, clamp=clamp, gain=gain, weight_gain=wg,
+                       bias_gain=bg)
+        t = x.dtype
+        x2, wd = x.double().reshape(-1, x.shape[-1]), w.double()
+        k = x2.shape[1]
+        bd = torch.zeros((), dtype=torch.float64, device=x.device) \
+            if b is None else b.double() * bg
+        z = wg * (x2 @ wd.t()) + bd
+        self.e_z = (k + 4) * U * (abs(wg) * (x2.abs() @ wd.abs().t())
+                                  + bd.abs()) + 1e-30
+        self.z = z
+        a, s = act_parts(z, act)
+        y = a * self.gain
+        self.slope = s * self.gain
+        # 8 U: the activation's own arithmetic, a few roundings of values no
+        # larger than max(1, |z|)
+        e_y = abs(self.gain) * (SLOPE[act] * self.e_z
+                                + 8 * U * (1 + z.abs()))
+        # where a rounding of z may pick the other branch (sign or clamp)
+        self.border = torch.zeros_like(z, dtype=torch.bool)
+        if act in ("relu", "lrelu"):
+            self.border |= z.abs() <= 2 * self.e_z
+        if clamp is not None:
+            edge = (y.abs() - clamp).abs()
+            self.border |= edge <= 2 * e_y + 4 * HALF[t] * clamp * (1 + clamp)
+            self.slope = torch.where(y.abs() < clamp, self.slope, 0.0)
+            y = y.clamp(-clamp, clamp)
+        if res is not None:
+            r = res.double().reshape(y.shape)
+            e_y = e_y + U * (y.abs() + r.abs())
+            y = y + r
+        self.y = y.reshape(x.shape[:-1] + (w.shape[0],))
+        self.e_y = (e_y + HALF[t] * y.abs()).reshape(self.y.shape)
+
+    def check_forward(self, y):
+        within(y, self.y, self.e_y, "y")
+
+    def dy(self, gen):
+        """an incoming gradient, zero where a rounding decides the slope"""
+        d = torch.randn(self.z.shape, generator=gen, device=self.z.device)
+        return torch.where(self.border, 0.0, d).to(self.x.dtype).reshape(
+            self.y.shape)
+
+    def check_backward(self, dy, dx=None, dw=None, db=None):
+        t, h = self.x.dtype, HALF[self.x.dtype]
+        x2, wd = self.x.double().reshape(-1, self.x.shape[-1]), self.w.double()
+        d = dy.double().reshape(self.z.shape)
+        dz = d * self.slope
+        # the slope is taken at z as it was kept (half a step off) and has
+        # a few roundings of its own
+        e_s = abs(self.gain) * (
+            CURVE[self.act] * (self.e_z + h * self.z.abs()) + 12 * U
+            * (1 + self.z.abs()))
+        if self.act == "linear":
+            e_s = 0 * e_s
+        e_sum = d.abs() * e_s + 2 * U * dz.abs()
+        # the products read dz in x's dtype
+        e_dz = e_sum + h * dz.abs()
+        m, n, k = dz.shape[0], dz.shape[1], x2.shape[1]
+        wg = abs(self.wg)
+        if dx is not None:
+            want = self.wg * (dz @ wd)
+            tol = wg * (e_dz @ wd.abs()
+                        + (n + 4) * U * ((dz.abs() + e_dz) @ wd.abs()))
+            within(dx.reshape(want.shape), want,
+                   tol + h * (want.abs() + tol) + 1e-30, "dx")
+        if dw is not None:
+            want = self.wg * (dz.t() @ x2)
+            tol = wg * (e_dz.t() @ x2.abs()
+                        + (m + 4) * U * ((dz.abs() + e_dz).t() @ x2.abs()))
+            within(dw, want, tol + h * (want.abs() + tol) + 1e-30, "dw")
+        if db is not None:
+            want = self.bg * dz.sum(0)
+            tol = abs(self.bg) * (e_sum.sum(0) + (m + 4) * U
+                                  * (dz.abs() + e_sum).sum(0))
+            within(db, want, tol + HALF[db.dtype] * (want.abs() + tol)
+                   + 1e-30, "db")
+
+
+# ---------------- CPU: the composition ----------------
+def randn(*shape, dtype=F32, device="cpu", seed=0, grad=False):
+    g = torch.Generator(device=device).manual_seed(seed)
+    t = torch.randn(*shape, generator=g, device=device).to(dtype)
+    return t.requires_grad_() if grad else t
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, torch.float64])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (2, 5, 64)])
+def test_layer_norm_cpu(dtype, shape):
+    x = randn(*shape, dtype=dtype)
+    w, b = randn(shape[-1], seed=1), randn(shape[-1], seed=2)
+    if dtype == torch.float64:
+        w, b = w.double(), b.double()
+    check_ln(x, w, b, got=[layer_norm(x, w, b)])
+    check_ln(x, None, None, got=[layer_norm(x)])
+
+
+def test_layer_norm_gradcheck():
+    x = randn(3, 5, dtype=torch.float64, grad=True)
+    w = randn(5, dtype=torch.float64, seed=1, grad=True)
+    b = randn(5, dtype=torch.float64, seed=2, grad=True)
+    assert gradcheck(layer_norm, (x, w, b))
+    assert gradgradcheck(layer_norm, (x, w, b))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_act_cpu(act, dtype):
+    c = Linear(randn(2, 3, 7, dtype=dtype), randn(5, 7, dtype=dtype, seed=1),
+               randn(5, seed=2), randn(2, 3, 5, dtype=dtype, seed=3), act,
+               clamp=0.7, wg=0.5, bg=2.0)
+    c.check_forward(linear_act(c.x, c.w, c.b, residual=c.res, **c.kw))
+
+
+@pytest.mark.parametrize("act", ["linear", "relu", "lrelu"])
+def test_linear_act_is_bias_act_of_the_product(act):
+    x, w, b = randn(4, 7), randn(5, 7, seed=1), randn(5, seed=2)
+    ref = bias_act((x @ w.t()).unsqueeze(-1), b, act=act).squeeze(-1)
+    assert torch.allclose(linear_act(x, w, b, act=act), ref, atol=1e-5)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_linear_act_gradcheck(act):
+    # |z| >= 0.5 away from the kink of relu and lrelu: x and w positive,
+    # bias of either sign and larger than x w can undo
+    x = randn(3, 4, dtype=torch.float64).abs().requires_grad_()
+    w = (randn(2, 4, dtype=torch.float64, seed=1).abs() * 0.01)
+    w.requires_grad_()
+    b = torch.tensor([1.0, -1.0], dtype=torch.float64, requires_grad=True)
+    r = randn(3, 2, dtype=torch.float64, seed=3, grad=True)
+
+    def f(x, w, b, r):
+        return linear_act(x, w, b, act=act, residual=r, weight_gain=0.7,
+                          bias_gain=1.3)
+    assert gradcheck(f, (x, w, b, r))
+    assert gradgradcheck(f, (x, w, b, r))
+
+
+def refusals(dev):
+    x, w = randn(4, 8, device=dev), randn(6, 8, device=dev)
+    v = randn(8, device=dev)
+    yield "shape", lambda: layer_norm(x, v[:7])
+    yield "shape", lambda: layer_norm(x, v, v.reshape(1, 8))
+    yield "weight is", lambda: layer_norm(x.bfloat16(), v, v.bfloat16())
+    yield "expected", lambda: layer_norm(x, v.bfloat16())
+    yield "at least 1", lambda: layer_norm(x[:, :0])
+    yield "at least 1", lambda: layer_norm(x[0, 0])
+    yield "unknown", lambda: linear_act(x, w, act="swish")
+    yield "do not fit", lambda: linear_act(x, w.t())
+    yield "do not fit", lambda: linear_act(x[0, 0], w)
+    yield "empty", lambda: linear_act(x, w[:0])
+    yield "empty", lambda: linear_act(x[:, :0], w[:, :0])
+    yield "weight is", lambda: linear_act(x, w.bfloat16())
+    yield "shape", lambda: linear_act(x, w, v)
+    yield "expected", lambda: linear_act(x, w, v[:6].bfloat16())
+    yield "fit the output", lambda: linear_act(x, w, residual=x)
+    yield "residual is", lambda: linear_act(
+        x, w, residual=x[:, :6].bfloat16())
+
+
+def test_refusals_cpu():
+    for message, call in refusals("cpu"):
+        with pytest.raises(ValueError, match=message):
+            call()
+
+
+# ---------------- GPU ----------------
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    from gansformer_amd.ops import native
+    native.require_ext()  # fail loudly, never silently eager
+    return torch.device("cuda:0")
+
+
+@pytest.mark.gpu
+def test_refusals_gpu(dev):
+    for message, call in refusals(dev):
+        with pytest.raises(ValueError, match=message):
+            call()
+    x, w = randn(4, 8, device=dev), randn(6, 8, device=dev)
+    for f in (lambda t: layer_norm(x.to(t)),
+              lambda t: linear_act(x.to(t), w.to(t))):
+        for t in (torch.float64, torch.float16):
+            with pytest.raises(ValueError, match="float32 or bfloat16"):
+                f(t)
+    for f in (lambda: layer_norm(x, w[0].cpu()),
+              lambda: linear_act(x, w.cpu()),
+              lambda: linear_act(x, w, w[:, 0].cpu()),
+              lambda: linear_act(x, w, residual=x[:, :6].cpu())):
+        with pytest.raises(ValueError, match="cpu"):
+            f()
+
+
+def ln_inputs(dev, rows, n, dtype, ptype=F32):
+    """rows of different size, with means of their own"""
+    x = (randn(rows, n, device=dev) * (0.5 + randn(rows, 1, device=dev,
+                                                   seed=1).abs())
+         + 2 * randn(rows, 1, device=dev, seed=2)).to(dtype)
+    return (x.requires_grad_(),
+            (1 + 0.2 * randn(n, device=dev, seed=3)).to(ptype)
+            .requires_grad_(),
+            randn(n, device=dev, seed=4, dtype=ptype).requires_grad_(),
+            randn(rows, n, device=dev, seed=5, dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 64, 65, 128, 255, 512, 771, 1024,
+                               1021, 2048, 2056, 4099, 8192, 20011, 32768])
+@pytest.mark.parametrize("rows", [1, 3, 17, 300])
+def test_layer_norm(dev, dtype, n, rows):
+    x, w, b, dy = ln_inputs(dev, rows, n, dtype)
+    with torch.no_grad():
+        check_ln(x, w, b, got=[layer_norm(x, w, b)])
+    y = layer_norm(x, w, b)
+    check_ln(x, w, b, dy, (y.detach(), *torch.autograd.grad(y, (x, w, b), dy)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(5000, 64), (3001, 96), (2500, 512),
+                                    (40000, 24), (1, 100000)])
+def test_layer_norm_many_rows(dev, dtype, rows, n):
+    x, w, b, dy = ln_inputs(dev, rows, n, dtype)
+    y = layer_norm(x, w, b)
+    check_ln(x, w, b, dy, (y.detach(), *torch.autograd.grad(y, (x, w, b), dy)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [40, 513, 5000])
+def test_layer_norm_parameters(dev, n):
+    """Every combination of parameters and of the gradients asked for."""
+    x, w, b, dy = ln_inputs(dev, 33, n, BF16, BF16)
+    for ww, bb in ((w, b), (w, None), (None, b), (None, None)):
+        y = layer_norm(x, ww, bb)
+        got = torch.autograd.grad(
+            y, [t for t in (x, ww, bb) if t is not None], dy)
+        it = iter(got[1:])
+        check_ln(x, ww, bb, dy,
+                 (y.detach(), got[0], next(it) if ww is not None else None,
+                  next(it) if bb is not None else None))
+    for keep in range(3):
+        leaves = [t.detach() for t in (x, w, b)]
+        leaves[keep].requires_grad_()
+        y = layer_norm(*leaves)
+        got = [None, None, None]
+        (got[keep],) = torch.autograd.grad(y, leaves[keep], dy)
+        check_ln(x, w, b, dy, (y.detach(), *got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layer_norm_strides(dev, dtype):
+    """Slices (odd offsets, wide rows), repeated rows, broadcast dy."""
+    n = 120
+    wide = randn(6, 9, 3 * n + 5, device=dev, dtype=dtype)
+    w, b = randn(2 * n, device=dev, seed=1)[::2], randn(n, device=dev, seed=2)
+    for x in (wide[..., 7:7 + n], wide[:, 2:8, n:2 * n], wide[:, 0, :n],
+              wide[0, :, 1:n + 1], wide[..., :3 * n:3],
+              wide.transpose(0, 1)[..., 8:8 + n],
+              wide[:1, 0, :n].expand(50, n)):
+        x = x.detach().requires_grad_()
+        y = layer_norm(x, w, b)
+        assert y.is_contiguous()
+        dy = randn(*x.shape, device=dev, seed=3, dtype=dtype)
+        check_ln(x, w, b, dy, (y.detach(), *torch.autograd.grad(
+            y, x, dy, retain_graph=True), None, None))
+        (dx,) = torch.autograd.grad(y.sum(), x)  # dy of stride 0
+        check_ln(x, w, b, torch.ones_like(dy), (y.detach(), dx, None, None))
+
+
+@pytest.mark.gpu
+def test_layer_norm_empty(dev):
+    x = randn(0, 33, device=dev, grad=True)
+    w, b = randn(33, device=dev, grad=True), randn(33, device=dev, grad=True)
+    y = layer_norm(x, w, b)
+    assert y.shape == (0, 33)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert dx.shape == (0, 33) and not dw.any() and not db.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [64, 70, 512, 3000, 40000])
+def test_layer_norm_bad_rows_stay_alone(dev, dtype, n):
+    """Rows of infinities and NaN do not reach others; constant rows give
+    the bias."""
+    x, w, b, dy = (t.detach() for t in ln_inputs(dev, 40, n, dtype))
+    bad = x.clone()
+    bad[3, 0], bad[17, n - 1], bad[18] = math.inf, math.nan, -math.inf
+    bad[20] = 4.0
+    y = layer_norm(bad, w, b)
+    good = [i for i in range(40) if i not in (3, 17, 18, 20)]
+    assert torch.equal(y[good], layer_norm(x, w, b)[good])
+    assert torch.isnan(y[[3, 17, 18]]).all()
+    assert torch.equal(y[20], b.to(dtype))
+
+
+@pytest.mark.gpu
+def test_layer_norm_far_mean(dev):
+    """The variance comes from centred values: a mean 1000 times the
+    deviation keeps its digits (the tolerance scales with |x| rstd)."""
+    x = randn(64, 768, device=dev) + 1000.0
+    check_ln(x, None, None, got=[layer_norm(x)])
+
+
+@pytest.mark.gpu
+def test_layer_norm_far_rows(dev):
+    """Offsets past 32 bits: over 2^31 elements."""
+    n, rows = 512, (1 << 22) + 70
+    x = torch.zeros(rows, n, device=dev, dtype=BF16)
+    tail = randn(100, n, device=dev, dtype=BF16)
+    x[-100:] = tail
+    x.requires_grad_()
+    w = randn(n, device=dev, seed=1, grad=True)
+    y = layer_norm(x, w)
+    dy = torch.zeros_like(y)
+    dy[-100:] = tail.flip(0)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert not y[:-100].any()  # rows of zeros
+    check_ln(tail, w, None, tail.flip(0), (y[-100:].detach(), dx[-100:], dw,
+                                           None))
+
+
+LINEAR_SIZES = [
+    (1, 1, 1), (1, 512, 512), (2, 7, 3), (3, 8, 1), (5, 1, 9),
+    (16, 64, 32), (17, 512, 512), (31, 100, 33), (33, 512, 40),
+    (64, 64, 64), (65, 129, 127), (100, 24, 200), (128, 128, 128),
+    (129, 256, 136), (257, 515, 259), (300, 72, 520), (544, 512, 512),
+    (32, 8192, 64), (1, 4099, 130), (17, 1024, 1), (1000, 16, 24),
+]
+
+
+def linear_inputs(dev, m, k, n, dtype, btype=F32):
+    return (randn(m, k, device=dev, dtype=dtype),
+            randn(n, k, device=dev, dtype=dtype, seed=1),
+            randn(n, device=dev, dtype=btype, seed=2),
+            randn(m, n, device=dev, dtype=dtype, seed=3))
+
+
+def linear_grads(c, dev, dy=None):
+    leaves = [t.detach().requires_grad_() for t in (c.x, c.w, c.b, c.res)
+              if t is not None]
+    it = iter(leaves)
+    args = [next(it) if t is not None else None
+            for t in (c.x, c.w, c.b, c.res)]
+    y = linear_act(args[0], args[1], args[2], residual=args[3], **c.kw)
+    c.check_forward(y.detach())
+    dy = c.dy(torch.Generator(device=dev).manual_seed(9)) if dy is None else dy
+    got = iter(torch.autograd.grad(y, leaves, dy))
+    dx, dw = next(got), next(got)
+    db = next(got) if c.b is not None else None
+    c.check_backward(dy, dx, dw, db)
+    if c.res is not None:
+        assert torch.equal(next(got), dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", LINEAR_SIZES)
+def test_linear_act_sizes(dev, dtype, m, k, n):
+    x, w, b, res = linear_inputs(dev, m, k, n, dtype)
+    c = Linear(x, w, b, res, "gelu", wg=1 / math.sqrt(k))
+    with torch.no_grad():
+        c.check_forward(linear_act(x, w, b, residual=res, **c.kw))
+    linear_grads(c, dev)
+    c = Linear(x, w, None, None, "linear")
+    with torch.no_grad():
+        c.check_forward(linear_act(x, w))
+    linear_grads(c, dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("clamp", [None, 0.6])
+@pytest.mark.parametrize("m", [3, 150])
+def test_linear_act_activations(dev, dtype, act, clamp, m):
+    x, w, b, res = linear_inputs(dev, m, 40, 56, dtype, btype=dtype)
+    for bias, residual in ((b, res), (b, None), (None, res)):
+        linear_grads(Linear(x, w, bias, residual, act, clamp, gain=1.7,
+                            wg=0.2, bg=0.5), dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(5000, 256, 264), (2048, 1024, 512),
+                                   (70001, 64, 48), (4100, 515, 130),
+                                   (600, 2048, 1030)])
+def test_linear_act_large(dev, dtype, m, k, n):
+    x, w, b, res = linear_inputs(dev, m, k, n, dtype)
+    linear_grads(Linear(x, w, b, res, "silu", wg=1 / math.sqrt(k)), dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [4, 90])
+def test_linear_act_strides(dev, dtype, m):
+    """Slices with odd offsets and strides, transposed, repeated rows."""
+    k, n = 72, 40
+    wide = randn(m, 3, 2 * k + 3, device=dev, dtype=dtype)
+    deep = randn(2 * k + 3, m, device=dev, dtype=dtype)
+    ww = randn(n, 2 * k + 1, device=dev, dtype=dtype, seed=1)
+    wt = randn(k, n, device=dev, dtype=dtype, seed=1).t()
+    rr = randn(m, 2 * n + 1, device=dev, dtype=dtype, seed=3)
+    for x in (wide[:, 1, 3:3 + k], wide[:, 0, :k], wide[:, 2, 8:8 + k],
+              deep[:k].t(), deep[0:2 * k:2].t(), wide[:1, 0, :k].expand(m, k)):
+        for w in (ww[:, :k], ww[:, 1:1 + k], wt):
+            for res in (rr[:, 1:n + 1], rr[:, ::2][:, :n],
+                        rr[:1, :n].expand(m, n)):
+                linear_grads(Linear(x, w, None, res, "silu", wg=0.1), dev)
+    x3 = wide[..., :k]  # three-dimensional, rows that do not collapse
+    linear_grads(Linear(x3, ww[:, :k], None, None, "gelu", wg=0.1), dev)
+    linear_grads(Linear(wide[0, 0, :k], ww[:, :k], None, None, "gelu",
+                        wg=0.1), dev)  # one vector
+    c = Linear(wide[:, 0, :k], ww[:, :k], None, None, "linear")
+    linear_grads(c, dev, dy=torch.ones(1, 1, device=dev, dtype=dtype)
+                 .expand(m, n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [2, 80])
+def test_linear_act_single_gradients(dev, m):
+    """Only what is asked for is computed, and it is the same."""
+    x, w, b, res = linear_inputs(dev, m, 48, 64, BF16)
+    full = [t.clone().requires_grad_() for t in (x, w, b, res)]
+    dy = randn(m, 64, device=dev, dtype=BF16, seed=6)
+    want = torch.autograd.grad(
+        linear_act(full[0], full[1], full[2], "gelu", full[3]), full, dy)
+    for i in range(4):
+        one = [t.detach() for t in (x, w, b, res)]
+        one[i].requires_grad_()
+        (got,) = torch.autograd.grad(
+            linear_act(one[0], one[1], one[2], "gelu", one[3]), one[i], dy)
+        assert torch.equal(got, want[i])
+        one[i].requires_grad_(False)
+
+
+@pytest.mark.gpu
+def test_linear_act_empty(dev):
+    x = randn(0, 3, 8, device=dev, grad=True)
+    w, b = randn(5, 8, device=dev, grad=True), randn(5, device=dev, grad=True)
+    y = linear_act(x, w, b, act="gelu")
+    assert y.shape == (0, 3, 5)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert dx.shape == x.shape and not dw.any() and not db.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(9, 64, 64), (200, 128, 96),
+                                   (700, 264, 520)])
+def test_linear_act_bad_values_stay_alone(dev, dtype, m, k, n):
+    """A NaN or infinity in a row of x stays in that row of y, one in the
+    weight in that column; nothing beyond the edges is read."""
+    x, w, b, res = linear_inputs(dev, m, k, n, dtype)
+    y = linear_act(x, w, b, "lrelu", res)
+    x2, w2 = x.clone(), w.clone()
+    x2[2, 5], x2[m - 1, k - 1], w2[n - 2, 0] = math.nan, math.inf, math.nan
+    y2 = linear_act(x2, w2, b, "lrelu", res)
+    rows = [i for i in range(m) if i not in (2, m - 1)]
+    cols = [i for i in range(n) if i != n - 2]
+    assert torch.equal(y2[rows][:, cols], y[rows][:, cols])
+    assert torch.isnan(y2[2]).all() and torch.isnan(y2[:, n - 2]).all()
+    assert not torch.isfinite(y2[m - 1]).any()
+    # the rows around a slice of x, and the columns, are not part of it
+    frame = torch.full((m + 2, k + 16), math.nan, device=dev, dtype=dtype)
+    frame[1:m + 1, 8:k + 8] = x
+    assert torch.equal(linear_act(frame[1:m + 1, 8:k + 8], w, b, "lrelu",
+                                  res), y)
+
+
+@pytest.mark.gpu
+def test_linear_act_far_rows(dev):
+    """Offsets past 32 bits: over 2^31 elements of x."""
+    k, n, rows = 512, 16, (1 << 22) + 70
+    x = torch.zeros(rows, k, device=dev, dtype=BF16)
+    tail = randn(100, k, device=dev, dtype=BF16)
+    x[-100:] = tail
+    x.requires_grad_()
+    w = randn(n, k, device=dev, dtype=BF16, seed=1, grad=True)
+    y = linear_act(x, w, act="silu", weight_gain=0.05)
+    assert not y[:-100].any()
+    c = Linear(tail, w.detach(), None, None, "silu", wg=0.05)
+    c.check_forward(y[-100:].detach())
+    dy = torch.zeros_like(y)
+    dy[-100:] = randn(100, n, device=dev, seed=4).bfloat16()
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert not dx[:-100].any()
+    c.check_backward(dy[-100:], dx[-100:], dw)
+
+
+# ---------------- together ----------------
+def block(x, p):
+    """pre-norm residual layer, then a widening and a narrowing one"""
+    x = linear_act(layer_norm(x, p[0], p[1]), p[2], p[3], "lrelu", x,
+                   weight_gain=0.1)
+    h = linear_act(layer_norm(x, p[0], p[1]), p[4], act="gelu",
+                   weight_gain=0.1)
+    return linear_act(h, p[5], residual=x, weight_gain=0.1)
+
+
+def block_inputs(dev, m, c, dtype):
+    p = [1 + 0.1 * randn(c, device=dev, seed=1), randn(c, device=dev, seed=2),
+         randn(c, c, device=dev, seed=3, dtype=dtype),
+         randn(c, device=dev, seed=4),
+         randn(4 * c, c, device=dev, seed=5, dtype=dtype),
+         randn(c, 4 * c, device=dev, seed=6, dtype=dtype)]
+    return [randn(m, c, device=dev, dtype=dtype)] + p
+
+
+def grads_of_block(leaves, dy):
+    leaves = [t.detach().requires_grad_() for t in leaves]
+    y = block(leaves[0], leaves[1:])
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,c", [(17, 128), (513, 96)])
+def test_block_matches_the_cpu(dev, m, c):
+    """float32 throughout, against the composition in 64 bits. The norms
+    of the differences: each of the six operators adds a relative error of
+    at most about (terms) u to values of order one and hands on those it
+    gets, so 6 * 4c u bounds the forward pass, and the backward pass runs
+    through the same six and their 6 transposes, m terms for a weight."""
+    leaves = block_inputs(dev, m, c, F32)
+    dy = randn(m, c, device=dev, seed=9)
+    got = grads_of_block(leaves, dy)
+    want = grads_of_block([t.double().cpu() for t in leaves],
+                          dy.double().cpu())
+    tol = 12 * max(4 * c, m) * U
+    for g, r in zip(got, want):
+        assert (g.double().cpu() - r).norm() <= tol * r.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_block_double_backward(dev, dtype):
+    """create_graph runs through the composition on the GPU as on the CPU:
+    the same float operations in another order (bf16: the same roundings
+    of every operator's outputs, half a step each of a handful)."""
+    leaves = block_inputs(dev, 11, 32, dtype)
+
+    def penalty(ts):
+        ts = [t.detach().requires_grad_() for t in ts]
+        y = block(ts[0], ts[1:])
+        (g,) = torch.autograd.grad(y.float().square().sum(), ts[0],
+                                   create_graph=True)
+        return torch.autograd.grad(g.float().square().sum(), ts)
+    got, want = penalty(leaves), penalty([t.cpu() for t in leaves])
+    for g, r in zip(got, want):
+        r = r.float()
+        # some 24 operations deep; 32 roundings that all point one way
+        assert (g.float().cpu() - r).norm() <= 32 * 2 * HALF[dtype] * r.norm() \
+            + 32 * 128 * U * r.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [1, 17, 2000])
+def test_same_results_every_time(dev, dtype, m):
+    leaves = block_inputs(dev, m, 256, dtype)
+    dy = randn(m, 256, device=dev, seed=9, dtype=dtype)
+    first = grads_of_block(leaves, dy)
+    for _ in range(3):
+        for a, b in zip(first, grads_of_block(leaves, dy)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_on_another_stream(dev):
+    leaves = block_inputs(dev, 600, 128, BF16)
+    dy = randn(600, 128, device=dev, seed=9, dtype=BF16)
+    want = grads_of_block(leaves, dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = grads_of_block(leaves, dy)
+        again = grads_of_block(leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b, c in zip(want, got, again):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [17, 600])
+def test_captured_and_replayed(dev, m):
+    """Two graphs captured from the same calls, replayed in turn with new
+    inputs and eager work between them."""
+    leaves = [t.requires_grad_() for t in block_inputs(dev, m, 64, BF16)]
+    dy = randn(m, 64, device=dev, seed=9, dtype=BF16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(block(leaves[0], leaves[1:]), leaves, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = block(leaves[0], leaves[1:])
+            outs.append([y, *torch.autograd.grad(y, leaves, dy)])
+        graphs.append(g)
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(randn(m, 64, device=dev, seed=20 + i))
+        want = grads_of_block(leaves, dy)
+        for k in ((0, 1), (1, 0), (0, 0), (1, 1))[i]:
+            graphs[k].replay()
+            torch.cuda.synchronize()
+            for a, b in zip(outs[k], want):
+                assert torch.equal(a, b)
