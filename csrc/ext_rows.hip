@@ -180,7 +180,10 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
   if (need_dw) dw = torch::empty({n}, popt);
   if (need_db) db = torch::empty({n}, popt);
   if (need_dw || need_db)
-    partial = torch::empty({2, gfa::layer_norm_bwd_groups(xr.count, n), n},
+    partial = torch::empty({2, gfa::layer_norm_bwd_groups(
+                                   xr.count, n,
+                                   x.scalar_type() == torch::kFloat32),
+                            n},
                            f32);
   DISPATCH_TP(x, p32, {
     gfa::launch_layer_norm_bwd<T, P>(

@@ -65,10 +65,10 @@ void linear_gemm_kernel(T* __restrict__ c, const T* __restrict__ a,
           z += e.bias_gain * (e.bias_f32
                                   ? static_cast<const float*>(e.bias)[n]
                                   : to_f32(static_cast<const T*>(e.bias)[n]));
-        if (e.z) e.z[m * g.N + n] = from_f32<T>(z);
+        if (e.z) put(e.z + m * g.N + n, z);
         float y = act_value(z, e.act);
         if (e.residual) y += to_f32(e.residual[m * e.res_stride + n]);
-        c[m * g.N + n] = from_f32<T>(y);
+        put(c + m * g.N + n, y);
       }
 }
 
@@ -97,7 +97,7 @@ void linear_dz_kernel(T* __restrict__ dz, float* __restrict__ partial,
     float d = to_f32(dy[r * dy_stride + i]);
     if (z) {
       d *= act_slope(to_f32(z[r * n + i]), act);
-      dz[r * n + i] = from_f32<T>(d);
+      put(dz + r * n + i, d);
     }
     sum += d;  // before its rounding
   }

@@ -6,6 +6,16 @@
 
 namespace gfa {
 
+// rounding to T in hardware, to nearest even, NaN kept
+template <typename T> GFA_DEV typename Raw<T>::type round_raw(float v);
+template <> GFA_DEV float round_raw<float>(float v) { return v; }
+template <> GFA_DEV u16 round_raw<bf16>(float v) {
+  return __builtin_bit_cast(u16, static_cast<__bf16>(v));
+}
+template <typename T> GFA_DEV void put(T* p, float v) {
+  *reinterpret_cast<typename Raw<T>::type*>(p) = round_raw<T>(v);
+}
+
 // activation codes of gansformer_amd/ops/linear_act.py
 enum Act { kLinear = 0, kRelu, kLrelu, kTanh, kSigmoid, kGelu, kSilu };
 
@@ -71,7 +81,7 @@ void launch_layer_norm_fwd(T* y, float* mean, float* rstd, const T* x,
                            long x_stride, const P* w, const P* b, long rows,
                            int n, float eps, hipStream_t);
 // partial: [2][groups][n] floats; dx, dw, db null if not wanted
-int layer_norm_bwd_groups(long rows, int n);
+int layer_norm_bwd_groups(long rows, int n, bool f32);
 template <typename T, typename P>
 void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
                            long dy_stride, const T* x, long x_stride,
