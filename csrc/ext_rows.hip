@@ -312,11 +312,11 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     if (need_db) {
       const float scale = (float)(bias_gain * slope);
       if (bias->scalar_type() == torch::kFloat32)
-        gfa::launch_sum_groups<float>(mptr<float>(db),
+        gfa::launch_sum_groups<float>(mptr<float>(db), nullptr,
                                       partial->data_ptr<float>(), groups,
                                       (int)n, scale, cur_stream());
       else
-        gfa::launch_sum_groups<gfa::bf16>(mptr<gfa::bf16>(db),
+        gfa::launch_sum_groups<gfa::bf16>(mptr<gfa::bf16>(db), nullptr,
                                           partial->data_ptr<float>(), groups,
                                           (int)n, scale, cur_stream());
     }

@@ -68,12 +68,18 @@ GFA_DEV void row_sum2(float& a, float& b, int lanes, float* red, int& turn) {
 }
 
 // ---- rows in registers ----
-// A row is held by L lanes, E elements each, as chunks of 16 bytes that
-// neighbouring lanes read side by side: L is a power of two up to 64 within
-// a wave (several rows a wave where a row is short), or 256 or 1024 threads.
-// x is read once and y written once; the loads need only the alignment of
-// an element, so strides and widths of any size take the same path, with
-// the last, partial chunk read element by element.
+// A row is held by L lanes, E elements each, as chunks of V elements (16
+// bytes) that neighbouring lanes read side by side: L is a power of two up
+// to 64 within a wave (several rows a wave where a row is short), or 256 or
+// 1024 threads. x is read once and y written once. The loads need only the
+// alignment of an element, so strides of any size take the same path.
+//
+// Widths that are no multiple of L * E (TAIL): a chunk that would end past
+// the row is moved back to end with it. Its first elements then belong to
+// the chunk before; they are computed and stored twice, alike, and left out
+// of the sums. So no load or store is behind a branch, which would make the
+// next row's loads wait (at 524288x96 bf16 the backward took 142 us with
+// chunks read element by element at the end, 72 us this way).
 template <typename T> struct Chunk;
 template <> struct Chunk<float> {
   static constexpr int V = 4;
@@ -84,89 +90,102 @@ template <> struct Chunk<bf16> {
   typedef u16 Vec __attribute__((ext_vector_type(8), aligned(2)));
 };
 
-// v[0..V) = p[i..i+V), zero from n on
-template <typename T>
-GFA_DEV void load_chunk(float* v, const T* p, int i, int n) {
-  using C = Chunk<T>;
-  if (i + C::V <= n) {
-    const auto c = *reinterpret_cast<const typename C::Vec*>(p + i);
+// A lane's part of a row: where its chunks begin, and which elements count.
+// V is Chunk<T>::V, or 1 for rows shorter than a chunk.
+template <typename T, int V, int E, bool TAIL>
+struct Lane {
+  using R = typename Raw<T>::type;
+  int at[E / V], skip[E / V];  // skip: elements left out of the sums
+
+  GFA_DEV Lane(int li, int L, int n) {
 #pragma unroll
-    for (int j = 0; j < C::V; ++j) v[j] = raw_to_f32(c[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < C::V; ++j) v[j] = i + j < n ? to_f32(p[i + j]) : 0.f;
+    for (int k = 0; k < E / V; ++k) {
+      const int i = (k * L + li) * V;
+      at[k] = TAIL ? min(i, n - V) : i;
+      skip[k] = TAIL ? i - at[k] : 0;
+    }
   }
-}
+  GFA_DEV bool counts(int e) const { return !TAIL || e % V >= skip[e / V]; }
+  GFA_DEV int index(int e) const { return at[e / V] + e % V; }
 
-template <typename T>
-GFA_DEV void store_chunk(T* p, const float* v, int i, int n) {
-  using C = Chunk<T>;
-  if (i + C::V <= n) {
-    typename C::Vec c;
+  GFA_DEV void load(R* v, const T* row) const {
 #pragma unroll
-    for (int j = 0; j < C::V; ++j)
-      c[j] = round_raw<T>(v[j]);
-    *reinterpret_cast<typename C::Vec*>(p + i) = c;
-  } else {
+    for (int k = 0; k < E / V; ++k) {
+      if constexpr (V == 1) {
+        v[k] = reinterpret_cast<const R*>(row)[at[k]];
+      } else {
+        const auto c =
+            *reinterpret_cast<const typename Chunk<T>::Vec*>(row + at[k]);
 #pragma unroll
-    for (int j = 0; j < C::V; ++j)
-      if (i + j < n) put(p + i + j, v[j]);
+        for (int j = 0; j < V; ++j) v[k * V + j] = c[j];
+      }
+    }
   }
-}
-
-// V parameters of type P, `none` where there are none or from n on
-template <int V, typename P>
-GFA_DEV void load_params(float* v, const P* p, int i, int n, float none) {
+  GFA_DEV void store(T* row, const float* v) const {
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    v[j] = p && i + j < n ? to_f32(p[i + j]) : none;
-}
+    for (int k = 0; k < E / V; ++k) {
+      if constexpr (V == 1) {
+        put(row + at[k], v[k]);
+      } else {
+        typename Chunk<T>::Vec c;
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = round_raw<T>(v[k * V + j]);
+        *reinterpret_cast<typename Chunk<T>::Vec*>(row + at[k]) = c;
+      }
+    }
+  }
+  template <typename P>
+  GFA_DEV void params(float* v, const P* p, float none) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p ? to_f32(p[index(e)]) : none;
+  }
+};
 
-template <typename T, typename P, int WAVES, int E>
+template <typename T, typename P, int WAVES, int V, int E, bool TAIL>
 __global__ __launch_bounds__(WAVES == 16 ? 1024 : 256)
 void layer_norm_fwd_rows(T* __restrict__ y, float* __restrict__ mean,
                          float* __restrict__ rstd, const T* __restrict__ x,
                          long x_stride, const P* __restrict__ w,
                          const P* __restrict__ b, long rows, int n, float eps,
                          int lanes) {
-  constexpr int V = Chunk<T>::V;
+  // Blocks of 16 waves take one row each from a grid of all rows: the next
+  // block's loads hide this one's barriers better than a row ahead does.
+  constexpr bool kAhead = WAVES < 16;
   __shared__ float red[WAVES > 1 ? 4 * WAVES : 1];
   int turn = 0;
   const int L = WAVES == 1 ? lanes : WAVES * 64;
   const int li = threadIdx.x & (L - 1);
-  const int per_block = blockDim.x / L;
+  const Lane<T, V, E, TAIL> lane(li, L, n);
   float wv[E], bv[E];
-#pragma unroll
-  for (int c = 0; c < E; c += V) {
-    load_params<V>(wv + c, w, c * L + li * V, n, 1.f);
-    load_params<V>(bv + c, b, c * L + li * V, n, 0.f);
-  }
+  lane.params(wv, w, 1.f);
+  lane.params(bv, b, 0.f);
   // r0: the same for all lanes of a wave, which sum together
-  const int own = threadIdx.x / L;
-  for (long r0 = (long)blockIdx.x * per_block; r0 < rows;
-       r0 += (long)gridDim.x * per_block) {
+  const int own = threadIdx.x / L, per_block = blockDim.x / L;
+  const long step = (long)gridDim.x * per_block;
+  typename Raw<T>::type next[E];
+  long r0 = (long)blockIdx.x * per_block;
+  if (kAhead) lane.load(next, x + min(r0 + own, rows - 1) * x_stride);
+  for (; r0 < rows; r0 += step) {
     const long r = r0 + own;
     const bool live = r < rows;
-    const T* xr = x + (live ? r : r0) * x_stride;
+    if (!kAhead) lane.load(next, x + r * x_stride);
     float v[E];
     float s = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int c = 0; c < E; c += V) {
-      load_chunk<T>(v + c, xr, c * L + li * V, n);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s += v[c + j];
+    for (int e = 0; e < E; ++e) {
+      v[e] = raw_to_f32(next[e]);
+      s += lane.counts(e) ? v[e] : 0.f;
     }
+    // the next row is on its way while this one is summed and written
+    if (kAhead && r0 + step < rows)
+      lane.load(next, x + min(r + step, rows - 1) * x_stride);
     row_sum2<WAVES>(s, s2, lanes, red, turn);
     const float mu = s / n;
     s = s2 = 0.f;
 #pragma unroll
-    for (int c = 0; c < E; c += V) {
-      const int left = n - (c * L + li * V);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[c + j] -= mu;
-        s += j < left ? v[c + j] * v[c + j] : 0.f;
-      }
+    for (int e = 0; e < E; ++e) {
+      v[e] -= mu;
+      s += lane.counts(e) ? v[e] * v[e] : 0.f;
     }
     row_sum2<WAVES>(s, s2, lanes, red, turn);
     const float rs = 1.f / sqrtf(s / n + eps);
@@ -176,18 +195,14 @@ void layer_norm_fwd_rows(T* __restrict__ y, float* __restrict__ mean,
       rstd[r] = rs;
     }
 #pragma unroll
-    for (int c = 0; c < E; c += V) {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        v[c + j] = v[c + j] * rs * wv[c + j] + bv[c + j];
-      store_chunk<T>(y + r * n, v + c, c * L + li * V, n);
-    }
+    for (int e = 0; e < E; ++e) v[e] = v[e] * rs * wv[e] + bv[e];
+    lane.store(y + r * n, v);
   }
 }
 
 // One pass over x and dy: dx, and the block's sums over its rows of dy * xn
 // and dy for the parameters, held in registers until the rows are through.
-template <typename T, typename P, int WAVES, int E>
+template <typename T, typename P, int WAVES, int V, int E, bool TAIL>
 __global__ __launch_bounds__(WAVES == 16 ? 1024 : 256)
 void layer_norm_bwd_rows(T* __restrict__ dx, float* __restrict__ partial,
                          const T* __restrict__ dy, long dy_stride,
@@ -196,89 +211,88 @@ void layer_norm_bwd_rows(T* __restrict__ dx, float* __restrict__ partial,
                          const float* __restrict__ mean,
                          const float* __restrict__ rstd, long rows, int n,
                          int lanes) {
-  constexpr int V = Chunk<T>::V;
   constexpr int kThreads = WAVES == 16 ? 1024 : 256;
+  // a row ahead, except where its registers would spill
+  constexpr bool kAhead = WAVES < 16 || E < 16;
   __shared__ float red[WAVES > 1 ? 4 * WAVES : 1];
   // sums of the waves of a block, where they hold the same columns
   __shared__ float sums[WAVES == 1 ? kThreads * E : 1];
   int turn = 0;
   const int L = WAVES == 1 ? lanes : WAVES * 64;
   const int li = threadIdx.x & (L - 1);
-  const int per_block = kThreads / L;
-  const int own = threadIdx.x / L;
+  const int own = threadIdx.x / L, per_block = kThreads / L;
+  const Lane<T, V, E, TAIL> lane(li, L, n);
   float wv[E], aw[E], ab[E];
+  lane.params(wv, w, 1.f);
 #pragma unroll
-  for (int c = 0; c < E; c += V)
-    load_params<V>(wv + c, w, c * L + li * V, n, 1.f);
-#pragma unroll
-  for (int c = 0; c < E; ++c) aw[c] = ab[c] = 0.f;
-  for (long r0 = (long)blockIdx.x * per_block; r0 < rows;
-       r0 += (long)gridDim.x * per_block) {
+  for (int e = 0; e < E; ++e) aw[e] = ab[e] = 0.f;
+  const long step = (long)gridDim.x * per_block;
+  typename Raw<T>::type next_x[E], next_d[E];
+  float next_mu, next_rs;
+  auto load = [&](long r) {
+    const long at = min(r, rows - 1);
+    lane.load(next_x, x + at * x_stride);
+    lane.load(next_d, dy + at * dy_stride);
+    next_mu = mean[at];
+    next_rs = rstd[at];
+  };
+  long r0 = (long)blockIdx.x * per_block;
+  if (kAhead) load(r0 + own);
+  for (; r0 < rows; r0 += step) {
     const long r = r0 + own;
     const bool live = r < rows;
-    const long at = live ? r : r0;
-    const float mu = mean[at], rs = rstd[at];
+    if (!kAhead) load(r);
+    const float mu = next_mu, rs = next_rs;
     float xn[E], d[E];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int c = 0; c < E; c += V) {
-      load_chunk<T>(xn + c, x + at * x_stride, c * L + li * V, n);
-      load_chunk<T>(d + c, dy + at * dy_stride, c * L + li * V, n);
+    for (int e = 0; e < E; ++e) {
+      xn[e] = raw_to_f32(next_x[e]);
+      d[e] = raw_to_f32(next_d[e]);
     }
-    if (!live) {
+    if (kAhead && r0 + step < rows) load(r + step);
 #pragma unroll
-      for (int c = 0; c < E; ++c) d[c] = xn[c] = 0.f;
-    }
-#pragma unroll
-    for (int c = 0; c < E; ++c) {
-      xn[c] = (xn[c] - mu) * rs;
+    for (int e = 0; e < E; ++e) {
+      xn[e] = (xn[e] - mu) * rs;
       if (live) {
-        aw[c] += d[c] * xn[c];
-        ab[c] += d[c];
+        aw[e] += d[e] * xn[e];
+        ab[e] += d[e];
       }
-      d[c] *= wv[c];
-      s1 += d[c];
-      s2 += d[c] * xn[c];
+      d[e] *= wv[e];
+      const float t = lane.counts(e) ? d[e] : 0.f;
+      s1 += t;
+      s2 += t * xn[e];
     }
     if (!dx) continue;
     row_sum2<WAVES>(s1, s2, lanes, red, turn);
     if (!live) continue;
     const float m1 = s1 / n, m2 = s2 / n;
 #pragma unroll
-    for (int c = 0; c < E; c += V) {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        d[c + j] = rs * (d[c + j] - m1 - xn[c + j] * m2);
-      store_chunk<T>(dx + r * n, d + c, c * L + li * V, n);
-    }
+    for (int e = 0; e < E; ++e) d[e] = rs * (d[e] - m1 - xn[e] * m2);
+    lane.store(dx + r * n, d);
   }
   if (!partial) return;
   float* pw = partial + (long)blockIdx.x * n;
   float* pb = partial + ((long)gridDim.x + blockIdx.x) * n;
   if constexpr (WAVES > 1) {
 #pragma unroll
-    for (int c = 0; c < E; c += V) {
-#pragma unroll
-      for (int h = 0; h < V; h += 4) {
-        store_chunk<float>(pw, aw + c + h, c * L + li * V + h, n);
-        store_chunk<float>(pb, ab + c + h, c * L + li * V + h, n);
+    for (int e = 0; e < E; ++e)
+      if (lane.counts(e)) {
+        pw[lane.index(e)] = aw[e];
+        pb[lane.index(e)] = ab[e];
       }
-    }
   } else {
-    // column i of the block's row group q is at sums[q * width + i]
-    const int width = L * E;
+    // column i of the block's row group q is at sums[q * n + i]: n <= L * E
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       __syncthreads();
 #pragma unroll
-      for (int c = 0; c < E; c += V)
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          sums[own * width + c * L + li * V + j] = k ? ab[c + j] : aw[c + j];
+      for (int e = 0; e < E; ++e)
+        if (lane.counts(e)) sums[own * n + lane.index(e)] = k ? ab[e] : aw[e];
       __syncthreads();
       for (int i = threadIdx.x; i < n; i += kThreads) {
         float s = 0.f;
-        for (int q = 0; q < per_block; ++q) s += sums[q * width + i];
+        for (int q = 0; q < per_block; ++q) s += sums[q * n + i];
         (k ? pb : pw)[i] = s;
       }
     }
@@ -385,70 +399,95 @@ void layer_norm_dwb_kernel(float* __restrict__ partial,
   partial[(long)(groups + blockIdx.y) * n + i] = sb;
 }
 
-// out[i] = scale * sum_g partial[g][i]: 32 columns a block, 8 threads a
-// column, each of which takes every 8th group
+// out[k][i] = scale * sum_g partial[k][g][i] for k of grid y: 32 columns a
+// block and 32 threads a column, four of whose loads are on their way at a
+// time (one after the other, 1024 groups took 40 us).
 template <typename P>
-__global__ __launch_bounds__(256)
-void sum_groups_kernel(P* __restrict__ out, const float* __restrict__ partial,
-                       int groups, int n, float scale) {
-  __shared__ float red[8][33];
+__global__ __launch_bounds__(1024)
+void sum_groups_kernel(P* __restrict__ out0, P* __restrict__ out1,
+                       const float* __restrict__ partial, int groups, int n,
+                       float scale) {
+  __shared__ float red[32][33];
+  P* out = blockIdx.y ? out1 : out0;
+  if (!out) return;
+  partial += (long)blockIdx.y * groups * n;
   const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int i = blockIdx.x * 32 + c;
   float s = 0.f;
   if (i < n)
-    for (int g = q; g < groups; g += 8) s += partial[(long)g * n + i];
+    for (int g = q; g < groups; g += 128) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = g + 32 * k < groups ? partial[(long)(g + 32 * k) * n + i] : 0.f;
+      s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
   red[q][c] = s;
   __syncthreads();
-  if (q == 0 && i < n) {
+  // the 32 sums of a column, side by side in half a wave
+  s = red[c][q];
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += red[k][c];
-    put(out + i, s * scale);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor(s, o, 32);
+  const int col = blockIdx.x * 32 + q;
+  if (c == 0 && col < n) put(out + col, s * scale);
 }
 
 template <typename P>
-void launch_sum_groups(P* out, const float* partial, int groups, int n,
-                       float scale, hipStream_t s) {
-  hipLaunchKernelGGL(sum_groups_kernel<P>, dim3(ceil_div(n, 32)), dim3(256),
-                     0, s, out, partial, groups, n, scale);
+void launch_sum_groups(P* out0, P* out1, const float* partial, int groups,
+                       int n, float scale, hipStream_t s) {
+  hipLaunchKernelGGL(sum_groups_kernel<P>, dim3(ceil_div(n, 32), out1 ? 2 : 1),
+                     dim3(1024), 0, s, out0, out1, partial, groups, n, scale);
 }
 
 namespace {
 
 // How a row of n elements of type T is held: `waves` of a block (1, 4, 16; 0:
-// too wide for registers), `lanes` of one wave, `e` elements a lane.
+// too wide for registers), `lanes` of one wave, `v` elements a chunk and `e`
+// a lane.
 struct RowPlan {
-  int waves, lanes, e, per_block;
+  int waves, lanes, v, e, per_block;
+  bool tail;
 };
 
+// most4: elements a lane of a block of 4 waves may hold
 template <typename T>
-RowPlan row_plan(int n) {
-  const int v = Chunk<T>::V;
-  RowPlan p{0, 64, 16, 1};
+RowPlan row_plan(int n, int most4 = 16) {
+  RowPlan p{0, 64, Chunk<T>::V, 16, 1, true};
+  if (n < p.v) p.v = 1;
   for (int waves : {1, 4, 16})
-    if (!p.waves && n <= waves * 64 * 16) p.waves = waves;
+    if (!p.waves && n <= waves * 64 * (waves == 4 ? most4 : 16))
+      p.waves = waves;
   if (!p.waves) return p;
-  p.e = v;
+  p.e = p.v;
   while (n > p.waves * 64 * p.e) p.e *= 2;
   if (p.waves == 1) {
-    while (p.lanes > 1 && n <= p.lanes / 2 * v) p.lanes /= 2;
+    while (p.lanes > 1 && n <= p.lanes / 2 * p.v) p.lanes /= 2;
     p.per_block = 256 / p.lanes;
   }
+  p.tail = n != (p.waves == 1 ? p.lanes : p.waves * 64) * p.e;
   return p;
 }
 
-// f(waves, e) with both as compile-time constants
-template <typename T, typename F>
+template <int N> using Int = std::integral_constant<int, N>;
+
+// f(waves, v, e, tail) with all four as compile-time constants
+template <typename T, bool FWD, typename F>
 void with_plan(const RowPlan& p, F&& f) {
-  auto with_e = [&](auto waves) {
-    if constexpr (Chunk<T>::V == 4)
-      if (p.e == 4) return f(waves, std::integral_constant<int, 4>{});
-    if (p.e == 8) return f(waves, std::integral_constant<int, 8>{});
-    f(waves, std::integral_constant<int, 16>{});
+  constexpr int V = Chunk<T>::V;
+  auto with_e = [&](auto waves, auto tail) {
+    if (p.e == V) return f(waves, Int<V>{}, Int<V>{}, tail);
+    if (p.e == 2 * V) return f(waves, Int<V>{}, Int<2 * V>{}, tail);
+    if constexpr (V == 4 || (FWD && waves() == 4))
+      f(waves, Int<V>{}, Int<4 * V>{}, tail);
   };
-  if (p.waves == 1) return with_e(std::integral_constant<int, 1>{});
-  if (p.waves == 4) return with_e(std::integral_constant<int, 4>{});
-  with_e(std::integral_constant<int, 16>{});
+  auto with_tail = [&](auto waves) {
+    if (p.tail) return with_e(waves, std::true_type{});
+    with_e(waves, std::false_type{});
+  };
+  if (p.v == 1) return f(Int<1>{}, Int<1>{}, Int<1>{}, std::true_type{});
+  if (p.waves == 1) return with_tail(Int<1>{});
+  if (p.waves == 4) return with_tail(Int<4>{});
+  with_tail(Int<16>{});
 }
 
 }  // namespace
@@ -457,7 +496,8 @@ template <typename T, typename P>
 void launch_layer_norm_fwd(T* y, float* mean, float* rstd, const T* x,
                            long x_stride, const P* w, const P* b, long rows,
                            int n, float eps, hipStream_t s) {
-  const RowPlan p = row_plan<T>(n);
+  // bf16 rows up to 8192 stay in 4 waves (8192x8192: 16 waves 79 us)
+  const RowPlan p = row_plan<T>(n, sizeof(T) == 2 ? 32 : 16);
   if (!p.waves) {
     const unsigned grid = (unsigned)(rows < 65536 ? rows : 65536);
     hipLaunchKernelGGL((layer_norm_fwd_kernel<T, P>), dim3(grid), dim3(256),
@@ -465,12 +505,13 @@ void launch_layer_norm_fwd(T* y, float* mean, float* rstd, const T* x,
     return;
   }
   const long blocks = (rows + p.per_block - 1) / p.per_block;
-  const long most = p.waves == 16 ? 512 : 2048;
+  const long most = p.waves == 16 ? 1 << 20 : 1536;
   const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-  with_plan<T>(p, [&](auto waves, auto e) {
-    hipLaunchKernelGGL((layer_norm_fwd_rows<T, P, waves(), e()>), dim3(grid),
-                       dim3(p.waves == 16 ? 1024 : 256), 0, s, y, mean, rstd,
-                       x, x_stride, w, b, rows, n, eps, p.lanes);
+  with_plan<T, true>(p, [&](auto waves, auto v, auto e, auto tail) {
+    hipLaunchKernelGGL(
+        (layer_norm_fwd_rows<T, P, waves(), v(), e(), tail()>), dim3(grid),
+        dim3(waves() == 16 ? 1024 : 256), 0, s, y, mean, rstd, x, x_stride, w,
+        b, rows, n, eps, p.lanes);
   });
 }
 
@@ -481,7 +522,10 @@ int layer_norm_bwd_groups(long rows, int n, bool f32) {
     return (int)(g < 256 ? g : 256);
   }
   const long blocks = (rows + p.per_block - 1) / p.per_block;
-  const long most = p.waves == 16 ? 512 : 1024;
+  // two blocks a CU (one of 16 waves), each a row ahead, keep the memory
+  // busy; more only add sums to be read again (131072x512 bf16: 80 us with
+  // 512, 82 us with 1024, 91 us with 1536)
+  const long most = p.waves == 16 ? 256 : 512;
   return (int)(blocks < most ? blocks : most);
 }
 
@@ -493,11 +537,11 @@ void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
   const RowPlan p = row_plan<T>(n);
   const int groups = layer_norm_bwd_groups(rows, n, sizeof(T) == 4);
   if (p.waves) {
-    with_plan<T>(p, [&](auto waves, auto e) {
-      hipLaunchKernelGGL((layer_norm_bwd_rows<T, P, waves(), e()>),
-                         dim3(groups), dim3(p.waves == 16 ? 1024 : 256), 0, s,
-                         dx, partial, dy, dy_stride, x, x_stride, w, mean,
-                         rstd, rows, n, p.lanes);
+    with_plan<T, false>(p, [&](auto waves, auto v, auto e, auto tail) {
+      hipLaunchKernelGGL(
+          (layer_norm_bwd_rows<T, P, waves(), v(), e(), tail()>), dim3(groups),
+          dim3(waves() == 16 ? 1024 : 256), 0, s, dx, partial, dy, dy_stride,
+          x, x_stride, w, mean, rstd, rows, n, p.lanes);
     });
   } else {
     if (dx) {
@@ -512,9 +556,8 @@ void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
                          partial, dy, dy_stride, x, x_stride, mean, rstd,
                          rows, n);
   }
-  if (dw) launch_sum_groups<P>(dw, partial, groups, n, 1.f, s);
-  if (db)
-    launch_sum_groups<P>(db, partial + (long)groups * n, groups, n, 1.f, s);
+  if (dw || db)
+    launch_sum_groups<P>(dw, db, partial, groups, n, 1.f, s);
 }
 
 #define INSTANTIATE(T, P)                                                     \
@@ -527,9 +570,9 @@ void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
 INSTANTIATE(float, float)
 INSTANTIATE(bf16, float)
 INSTANTIATE(bf16, bf16)
-template void launch_sum_groups<float>(float*, const float*, int, int, float,
-                                       hipStream_t);
-template void launch_sum_groups<bf16>(bf16*, const float*, int, int, float,
-                                      hipStream_t);
+template void launch_sum_groups<float>(float*, float*, const float*, int, int,
+                                       float, hipStream_t);
+template void launch_sum_groups<bf16>(bf16*, bf16*, const float*, int, int,
+                                      float, hipStream_t);
 
 }  // namespace gfa

@@ -88,10 +88,10 @@ void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
                            const P* w, const float* mean, const float* rstd,
                            long rows, int n, hipStream_t);
 
-// sums partial[g][n] over g, scales and rounds to P
+// out_k[i] = scale * sum_g partial[k][g][i], k = 0, 1; an out may be null
 template <typename P>
-void launch_sum_groups(P* out, const float* partial, int groups, int n,
-                       float scale, hipStream_t);
+void launch_sum_groups(P* out0, P* out1, const float* partial, int groups,
+                       int n, float scale, hipStream_t);
 
 // C[m, n] = epilogue(alpha * sum_k A[m, k] B[n, k]); one of the two strides
 // of A and of B is 1
