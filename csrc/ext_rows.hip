@@ -202,7 +202,7 @@ void check_linear(const Tensor& x, const Tensor& w, const OptTensor& bias) {
   check(w, x, "linear_act: weight");
   TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) &&
                   w.size(0) >= 1 && w.size(1) >= 1 &&
-                  w.size(0) <= (1 << 22) && w.size(1) <= (1 << 22) &&
+                  w.size(0) < (1 << 20) && w.size(1) < (1 << 20) &&
                   w.scalar_type() == x.scalar_type(),
               "linear_act: weight does not fit x");
   check_param(bias, x, w.size(0), "linear_act: bias");
@@ -212,6 +212,34 @@ std::vector<int64_t> out_shape(const Tensor& x, int64_t n) {
   auto s = x.sizes().vec();
   s.back() = n;
   return s;
+}
+
+// The tiles read rows of 16-byte granules: rows elsewhere, or of another
+// width, are copied to padded ones (zeros behind the last element).
+template <typename T>
+Rows tile_rows(const Rows& r, int64_t n) {
+  const int64_t v = 16 / sizeof(T);
+  const int64_t width = (n + 7) / 8 * 8;
+  if (n % v == 0 && r.stride % v == 0 && r.stride < (1 << 20) &&
+      reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0)
+    return r;
+  Rows p{torch::empty({r.count, width}, r.t.options()), r.count, width};
+  gfa::launch_pad_rows<T>(static_cast<T*>(p.t.data_ptr()), cptr<T>(r.t),
+                          r.stride, r.count, (int)n, (int)width, cur_stream());
+  return p;
+}
+
+template <typename T>
+gfa::EpilogueArgs<T> epilogue(const OptTensor& bias, int64_t act, double alpha,
+                              double gain, double clamp, double bias_gain) {
+  gfa::EpilogueArgs<T> e{};
+  if (bias) {
+    e.bias = bias->data_ptr();
+    e.bias_f32 = bias->scalar_type() == torch::kFloat32;
+    e.bias_gain = (float)bias_gain;
+  }
+  e.act = {(int)act, (float)alpha, (float)gain, (float)clamp};
+  return e;
 }
 
 std::tuple<Tensor, OptTensor> linear_act_fwd(
@@ -229,33 +257,27 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(
                 "linear_act: residual does not fit");
   }
   c10::hip::HIPGuard guard(x.get_device());
-  const Rows xr = rows_of(x), wr = rows_of(w);
   const OptTensor bc = bias ? OptTensor(bias->contiguous()) : bias;
   Tensor y = torch::empty(shape, x.options());
   OptTensor z;
-  if (save_z) z = torch::empty(shape, x.options());
-  if (xr.count == 0) return {y, z};
-  const gfa::GemmArgs g{xr.count, n,         k, xr.stride, 1,
-                        wr.stride, 1, (float)weight_gain};
+  if (save_z) z = torch::empty(shape, x.options().dtype(torch::kFloat32));
+  if (y.numel() == 0) return {y, z};
   DISPATCH_FT(x.scalar_type(), {
-    gfa::EpilogueArgs<scalar_t> e{};
-    if (bc) {
-      e.bias = bc->data_ptr();
-      e.bias_f32 = bc->scalar_type() == torch::kFloat32;
-      e.bias_gain = (float)bias_gain;
-    }
+    const Rows xr = tile_rows<scalar_t>(rows_of(x), k);
+    const Rows wr = tile_rows<scalar_t>(rows_of(w), k);
+    auto e = epilogue<scalar_t>(bc, act, alpha, gain, clamp, bias_gain);
     Rows rr;
     if (residual) {
       rr = rows_of(*residual);
       e.residual = cptr<scalar_t>(rr.t);
       e.res_stride = rr.stride;
     }
-    e.z = mptr<scalar_t>(z);
-    e.act = {(int)act, (float)alpha, (float)gain, (float)clamp};
-    gfa::launch_linear_gemm<scalar_t>(static_cast<scalar_t*>(y.data_ptr()),
-                                      cptr<scalar_t>(xr.t),
-                                      cptr<scalar_t>(wr.t), g, e,
-                                      cur_stream());
+    e.z = mptr<float>(z);
+    gfa::launch_linear_forward<scalar_t>(
+        static_cast<scalar_t*>(y.data_ptr()), cptr<scalar_t>(xr.t),
+        cptr<scalar_t>(wr.t),
+        {xr.count, n, k, xr.stride, wr.stride, n, (float)weight_gain, k}, e,
+        cur_stream());
   });
   HIP_CHECK_LAST();
   return {y, z};
@@ -274,17 +296,14 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
   TORCH_CHECK(dy.sizes() == shape && dy.scalar_type() == x.scalar_type(),
               "linear_act: dy does not fit");
   TORCH_CHECK(!need_db || bias, "linear_act: no bias");
-  TORCH_CHECK(z || (act == gfa::kLinear && std::isinf(clamp)),
-              "linear_act: the pre-activation is missing");
   if (z)
     TORCH_CHECK(z->device() == x.device() && z->is_contiguous() &&
                     z->sizes() == shape &&
-                    z->scalar_type() == x.scalar_type(),
+                    z->scalar_type() == torch::kFloat32,
                 "linear_act: z does not fit");
   c10::hip::HIPGuard guard(x.get_device());
-  const Rows xr = rows_of(x), wr = rows_of(w), dr = rows_of(dy);
-  const int64_t m = xr.count;
-  OptTensor dx, dw, db, dz, partial;
+  const int64_t m = dy.numel() / n;
+  OptTensor dx, dw, db;
   if (need_dx) dx = torch::empty(x.sizes(), x.options());
   if (m == 0) {
     if (need_dw) dw = torch::zeros(w.sizes(), w.options());
@@ -293,22 +312,47 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
   }
   if (need_dw) dw = torch::empty(w.sizes(), w.options());
   if (need_db) db = torch::empty({n}, bias->options());
-  // without z the slope is the gain everywhere: dz is dy and the products
-  // carry the factor
-  const double slope = z ? 1.0 : gain;
-  const int groups = gfa::linear_dz_groups(m, (int)n);
   if (!need_dx && !need_dw && !need_db) return {dx, dw, db};
-  if (z) dz = torch::empty(shape, x.options());
-  if (need_db)
-    partial =
-        torch::empty({groups, n}, x.options().dtype(torch::kFloat32));
+  const OptTensor bc = bias ? OptTensor(bias->contiguous()) : bias;
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  // Without an activation or a clamp the slope is the gain everywhere: dz is
+  // dy and the products carry the factor.
+  const bool curved = act != gfa::kLinear || !std::isinf(clamp);
+  const double slope = curved ? 1.0 : gain;
   DISPATCH_FT(x.scalar_type(), {
-    const gfa::ActParams ap{(int)act, (float)alpha, (float)gain,
-                            (float)clamp};
-    if (z || need_db)
+    const Rows xr = tile_rows<scalar_t>(rows_of(x), k);
+    const Rows wr = tile_rows<scalar_t>(rows_of(w), k);
+    Rows dr = rows_of(dy);
+    auto e = epilogue<scalar_t>(bc, act, alpha, gain, clamp, bias_gain);
+    OptTensor partial;
+    int groups = 0;
+    if (curved && !z) {
+      // z again, from the product that made it
+      const int64_t width = (n + 7) / 8 * 8;
+      Rows dz{torch::empty({m, width}, x.options()), m, width};
+      e.dy = cptr<scalar_t>(dr.t);
+      e.dy_stride = dr.stride;
+      groups = gfa::linear_row_tiles(m, n);
+      if (need_db) partial = torch::empty({groups, n}, f32);
+      e.partial = mptr<float>(partial);
+      gfa::launch_linear_slope<scalar_t>(
+          static_cast<scalar_t*>(dz.t.data_ptr()), cptr<scalar_t>(xr.t),
+          cptr<scalar_t>(wr.t),
+          {m, n, k, xr.stride, wr.stride, width, (float)weight_gain, k}, e,
+          cur_stream());
+      dr = dz;
+    } else if (curved || need_db) {
+      const int64_t width = (n + 7) / 8 * 8;
+      Rows dz{Tensor(), m, width};
+      if (curved) dz.t = torch::empty({m, width}, x.options());
+      groups = gfa::linear_dz_groups(m, (int)n);
+      if (need_db) partial = torch::empty({groups, n}, f32);
       gfa::launch_linear_dz<scalar_t>(
-          mptr<scalar_t>(dz), mptr<float>(partial), cptr<scalar_t>(dr.t),
-          dr.stride, cptr<scalar_t>(z), ap, m, (int)n, cur_stream());
+          curved ? static_cast<scalar_t*>(dz.t.data_ptr()) : nullptr, width,
+          mptr<float>(partial), cptr<scalar_t>(dr.t), dr.stride,
+          curved ? mptr<float>(z) : nullptr, e.act, m, (int)n, cur_stream());
+      if (curved) dr = dz;
+    }
     if (need_db) {
       const float scale = (float)(bias_gain * slope);
       if (bias->scalar_type() == torch::kFloat32)
@@ -320,19 +364,22 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
                                           partial->data_ptr<float>(), groups,
                                           (int)n, scale, cur_stream());
     }
-    const scalar_t* d = z ? cptr<scalar_t>(dz) : cptr<scalar_t>(dr.t);
-    const int64_t ds = z ? n : dr.stride;
-    gfa::EpilogueArgs<scalar_t> e{};
-    e.act = {gfa::kLinear, 0.f, 1.f, INFINITY};
     const float scale = (float)(weight_gain * slope);
+    if (need_dx || need_dw) dr = tile_rows<scalar_t>(dr, n);
     if (need_dx)
-      gfa::launch_linear_gemm<scalar_t>(
-          mptr<scalar_t>(dx), d, cptr<scalar_t>(wr.t),
-          {m, k, n, ds, 1, 1, wr.stride, scale}, e, cur_stream());
-    if (need_dw)
-      gfa::launch_linear_gemm<scalar_t>(
-          mptr<scalar_t>(dw), d, cptr<scalar_t>(xr.t),
-          {n, k, m, 1, ds, 1, xr.stride, scale}, e, cur_stream());
+      gfa::launch_linear_dx<scalar_t>(
+          mptr<scalar_t>(dx), cptr<scalar_t>(dr.t), cptr<scalar_t>(wr.t),
+          {m, k, n, dr.stride, wr.stride, k, scale, n}, cur_stream());
+    if (need_dw) {
+      const int splits =
+          gfa::linear_splits(n, k, m, std::is_same_v<scalar_t, float>);
+      OptTensor parts;
+      if (splits > 1) parts = torch::empty({splits, n, k}, f32);
+      gfa::launch_linear_dw<scalar_t>(
+          mptr<scalar_t>(dw), mptr<float>(parts), cptr<scalar_t>(dr.t),
+          cptr<scalar_t>(xr.t),
+          {n, k, m, dr.stride, xr.stride, k, scale, m}, cur_stream());
+    }
   });
   HIP_CHECK_LAST();
   return {dx, dw, db};

@@ -1,92 +1,570 @@
 // Matrix product with bias, activation and residual in its epilogue, and
-// the three products of its backward, for gfx950.
+// the products of its backward, for gfx950.
 //
 //   z  = alpha * A B^T + bias_gain * bias
 //   y  = clamp(act(z) * gain) + residual
 //   dz = dy * slope(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz
 //
-// Every product is one C[m, n] = sum_k A[m, k] B[n, k] over operands whose
-// rows or whose columns are contiguous. Sums in float on the matrix cores;
-// z, y and the gradients are rounded to T once, on their way out.
+// Every product is one C[m, n] = sum_k A[m, k] B[n, k] over operands that are
+// contiguous along k ("rows") or along m or n ("columns"). Sums in float on
+// the matrix cores; what leaves a kernel is rounded to T once.
+#include <type_traits>
+
 #include "rows.h"
 
 namespace gfa {
 
-// 64x64 tile, 4 waves of 32x32; any strides, any sizes.
-template <typename T>
-__global__ __launch_bounds__(256)
-void linear_gemm_kernel(T* __restrict__ c, const T* __restrict__ a,
-                        const T* __restrict__ b, GemmArgs g,
-                        EpilogueArgs<T> e) {
-  using TO = TileOps<T>;
-  constexpr int BK = TO::BK;
-  using elem = typename TO::elem;
-  __shared__ elem As[64 * TO::ROW];
-  __shared__ elem Bs[64 * TO::ROW];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const long m0 = (long)blockIdx.x * 64, n0 = (long)blockIdx.y * 64;
-  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+using LdsPtr = __attribute__((address_space(3))) void*;
 
-  f32x4 acc[2][2] = {};
-  for (long k0 = 0; k0 < g.K; k0 += BK) {
-    __syncthreads();
-    for (int i = t; i < 64 * BK; i += 256) {
-      // neighbouring threads along the contiguous dimension
-      const int ra = g.sak == 1 ? i / BK : i % 64;
-      const int ka = g.sak == 1 ? i % BK : i / 64;
-      const bool oka = m0 + ra < g.M && k0 + ka < g.K;
-      TO::store(As, ra, ka,
-                oka ? to_f32(a[(m0 + ra) * g.sam + (k0 + ka) * g.sak]) : 0.f);
-      const int rb = g.sbk == 1 ? i / BK : i % 64;
-      const int kb = g.sbk == 1 ? i % BK : i / 64;
-      const bool okb = n0 + rb < g.N && k0 + kb < g.K;
-      TO::store(Bs, rb, kb,
-                okb ? to_f32(b[(n0 + rb) * g.sbn + (k0 + kb) * g.sbk]) : 0.f);
+// ---- tiles ----
+// A block computes BM x BN of C with WM x WN waves. Both operands of a k-tile
+// go from memory to LDS without passing through registers, 1 KB a wave and
+// instruction; a k-tile is 128 bytes deep (64 bf16, 32 float) and there are
+// two of them, one being filled while the other is used, with one barrier
+// between. Reads outside the operands return zero (the bounds are those of
+// the buffer descriptor), so any M, N, K take this path as long as rows are
+// 16-byte aligned.
+//
+// LDS layout. Rows: [m][128 bytes], 16-byte granule g of row r at g ^ (r/2
+// mod 8), so that the 16 rows a fragment read touches spread over all 64
+// banks. Columns: [k][BX], granules of row k exchanged likewise; bf16
+// fragments come out of it through the transposing LDS read.
+template <typename T, int BX, bool COLS>
+struct Operand {
+  static constexpr int ES = sizeof(T);
+  static constexpr int BK = 128 / ES;
+  static constexpr int kBytes = BX * 128;
+  static constexpr int kGran = COLS ? BX * ES / 16 : 8;  // granules of a row
+
+  // the granule of global memory that belongs at position p of LDS row r
+  GFA_DEV static int swizzle(int r) {
+    if (!COLS) return (r >> 1) & 7;
+    // the rows that one fragment read touches: bf16 r mod 4 and r/8 mod 2,
+    // float r/4 mod 4
+    const int s = ES == 2 ? 2 * ((r & 3) | ((r >> 1) & 4)) : 4 * ((r >> 2) & 3);
+    return s & (kGran - 1);
+  }
+
+  // byte offset from the tile's corner for a lane of the wave's i-th piece
+  template <int WAVES>
+  GFA_DEV static int source(int wave, int i, int lane, int stride) {
+    const int idx = (i * WAVES + wave) * 64 + lane;
+    const int r = idx / kGran, p = idx % kGran;
+    return r * stride * ES + ((p ^ swizzle(r)) << 4);
+  }
+};
+
+// fragments of 16 (m or n) x 128 bits of k: what one lane gives to the
+// matrix cores for a step of kStep
+template <typename T> struct Frag;
+template <> struct Frag<bf16> {
+  static constexpr int kStep = 32;
+  using Type = s16x8;
+  template <int BX, bool COLS>
+  GFA_DEV static Type read(const char* lds, int row0, int step, int lane) {
+    using O = Operand<bf16, BX, COLS>;
+    if constexpr (!COLS) {
+      const int r = row0 + (lane & 15);
+      const int g = step * 4 + (lane >> 4);
+      return *reinterpret_cast<const Type*>(lds + r * 128 +
+                                            ((g ^ O::swizzle(r)) << 4));
+    } else {
+      // four k of 16 columns each: lane i of 16 points at four columns of
+      // row i / 4 and gets the four rows of column i
+      s16x4 h[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int k = step * 32 + (lane >> 4) * 8 + q * 4 + ((lane & 15) >> 2);
+        const int c = row0 + 4 * (lane & 3);
+        h[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(
+                lds + k * (BX * 2) + (((c >> 3) ^ O::swizzle(k)) << 4) +
+                (c & 7) * 2));
+      }
+      return Type{h[0][0], h[0][1], h[0][2], h[0][3],
+                  h[1][0], h[1][1], h[1][2], h[1][3]};
     }
+  }
+  GFA_DEV static f32x4 mma(Type a, Type b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+        0);
+  }
+};
+template <> struct Frag<float> {
+  static constexpr int kStep = 16;  // k = 4 * (lane / 16) + j in step j of 4
+  using Type = f32x4;
+  template <int BX, bool COLS>
+  GFA_DEV static Type read(const char* lds, int row0, int step, int lane) {
+    using O = Operand<float, BX, COLS>;
+    if constexpr (!COLS) {
+      const int r = row0 + (lane & 15);
+      const int g = step * 4 + (lane >> 4);
+      return *reinterpret_cast<const Type*>(lds + r * 128 +
+                                            ((g ^ O::swizzle(r)) << 4));
+    } else {
+      Type v;
+      const int c = row0 + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = step * 16 + (lane >> 4) * 4 + j;
+        v[j] = *reinterpret_cast<const float*>(
+            lds + k * (BX * 4) + (((c >> 2) ^ O::swizzle(k)) << 4) +
+            (c & 3) * 4);
+      }
+      return v;
+    }
+  }
+  GFA_DEV static f32x4 mma(Type a, Type b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// Eight values of a row, at any alignment, as they are stored; zero from
+// `left` on. Kept so until they are used: a conversion would wait for them.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  typedef float Half __attribute__((ext_vector_type(4), aligned(4)));
+  Half a, b;
+  GFA_DEV float operator[](int j) const { return j < 4 ? a[j] : b[j - 4]; }
+  GFA_DEV void load(const float* p) {
+    a = *reinterpret_cast<const Half*>(p);
+    b = *reinterpret_cast<const Half*>(p + 4);
+  }
+  GFA_DEV void load(const float* p, int left) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = j < left ? p[j] : 0.f;
+      b[j] = j + 4 < left ? p[j + 4] : 0.f;
+    }
+  }
+};
+template <> struct Eight<bf16> {
+  typedef u16 Vec __attribute__((ext_vector_type(8), aligned(2)));
+  Vec a;
+  GFA_DEV float operator[](int j) const { return bf16_bits_to_f32(a[j]); }
+  GFA_DEV void load(const bf16* p) { a = *reinterpret_cast<const Vec*>(p); }
+  GFA_DEV void load(const bf16* p, int left) {
+    const u16* q = reinterpret_cast<const u16*>(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = j < left ? q[j] : (u16)0;
+  }
+};
+template <typename T>
+GFA_DEV void load8(float* v, const T* p, int left) {
+  Eight<T> e;
+  if (left >= 8)
+    e.load(p);
+  else
+    e.load(p, left);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = e[j];
+}
+GFA_DEV void store8(float* p, const float* v, int left) {
+  using H = typename Eight<float>::Half;
+  if (left >= 8) {
+    *reinterpret_cast<H*>(p) = H{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<H*>(p + 4) = H{v[4], v[5], v[6], v[7]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) p[j] = v[j];
+  }
+}
+GFA_DEV void store8(bf16* p, const float* v, int left) {
+  using V = typename Eight<bf16>::Vec;
+  if (left >= 8) {
+    V a;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = round_raw<bf16>(v[j]);
+    *reinterpret_cast<V*>(p) = a;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) put(p + j, v[j]);
+  }
+}
+
+GFA_DEV auto buffer_at(const void* p, long bytes) {
+  const long most = 0x7ffffff0;
+  return __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<void*>(p), 0, (int)(bytes < most ? bytes : most),
+      0x00020000);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool ACOLS, bool BCOLS,
+          int EPI>
+__global__ __launch_bounds__(WM * WN * 64)
+void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
+                 const T* __restrict__ a, const T* __restrict__ b) {
+  using OA = Operand<T, BM, ACOLS>;
+  using OB = Operand<T, BN, BCOLS>;
+  using F = Frag<T>;
+  constexpr int ES = sizeof(T), BK = OA::BK, WAVES = WM * WN;
+  constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  constexpr int PA = BM / 8 / WAVES, PB = BN / 8 / WAVES;
+  constexpr int kStage = OA::kBytes + OB::kBytes;
+  // the epilogue turns 32 rows of a wave at a time in LDS
+  constexpr int EROW = TN * 4 + 16;
+  constexpr int kEpi = WAVES * 32 * EROW;
+  constexpr int kLds = 2 * kStage > kEpi ? 2 * kStage : kEpi;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // Tiles: an XCD's blocks (every eighth) take neighbouring tiles, in
+  // groups of 4 rows of tiles, so that they share operands in its L2.
+  const int tm = (int)((g.M + BM - 1) / BM), tn = (int)((g.N + BN - 1) / BN);
+  const int total = tm * tn, per = (total + 7) / 8;
+  const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;
+  const int group = tile / (4 * tn), in_group = tile - group * 4 * tn;
+  const int rows = min(4, tm - group * 4);
+  const int mt = group * 4 + in_group % rows;
+  const long m0 = (long)mt * BM;
+  const long n0 = (long)(in_group / rows) * BN;
+  // the block's part of k
+  const long kb = (long)blockIdx.y * g.k_split;
+  const int kn = (int)min(g.K - kb, g.k_split);
+
+  const char* pa = reinterpret_cast<const char*>(
+      ACOLS ? a + kb * g.lda + m0 : a + m0 * g.lda + kb);
+  const char* pb = reinterpret_cast<const char*>(
+      BCOLS ? b + kb * g.ldb + n0 : b + n0 * g.ldb + kb);
+  // bytes from the corner of the tile to the end of the operand, whose rows
+  // end with a whole granule
+  auto whole16 = [](long v) { return (v * ES + 15) & ~15l; };
+  const long la = ACOLS ? (kn - 1) * g.lda * ES + whole16(g.M) - m0 * ES
+                        : (g.M - m0 - 1) * g.lda * ES + whole16(kn);
+  const long lb = BCOLS ? (kn - 1) * g.ldb * ES + whole16(g.N) - n0 * ES
+                        : (g.N - n0 - 1) * g.ldb * ES + whole16(kn);
+  const long sa = (ACOLS ? BK * g.lda : BK) * ES;
+  const long sb = (BCOLS ? BK * g.ldb : BK) * ES;
+
+  int va[PA], vb[PB];
+#pragma unroll
+  for (int i = 0; i < PA; ++i)
+    va[i] = OA::template source<WAVES>(wave, i, lane, (int)g.lda);
+#pragma unroll
+  for (int i = 0; i < PB; ++i)
+    vb[i] = OB::template source<WAVES>(wave, i, lane, (int)g.ldb);
+  // rows: the lane's k within a k-tile, past which the last one is cut off
+  auto k_of = [&](int i) {
+    const int idx = (i * WAVES + wave) * 64 + lane;
+    return ((idx & 7) ^ ((idx >> 4) & 7)) * (16 / ES);
+  };
+
+  auto fetch = [&](int t, int stage) {
+    char* base = lds + stage * kStage;
+    const auto ra = buffer_at(pa + t * sa, la - t * sa);
+    const auto rb = buffer_at(pb + t * sb, lb - t * sb);
+    const int left = kn - t * BK;
+#pragma unroll
+    for (int i = 0; i < PA; ++i) {
+      const int off = !ACOLS && left < BK && k_of(i) >= left ? 0x7ffffff8
+                                                             : va[i];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          ra, (LdsPtr)(base + (i * WAVES + wave) * 1024), 16, off, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      const int off = !BCOLS && left < BK && k_of(i) >= left ? 0x7ffffff8
+                                                             : vb[i];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rb, (LdsPtr)(base + OA::kBytes + (i * WAVES + wave) * 1024), 16,
+          off, 0, 0, 0);
+    }
+  };
+
+  const int wm = wave / WN * TM, wn = wave % WN * TN;
+  f32x4 acc[FM][FN] = {};
+  const int tiles = (kn + BK - 1) / BK;
+  fetch(0, 0);
+  for (int t = 0; t < tiles; ++t) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces
     __syncthreads();
+    if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+    const char* la_ = lds + (t & 1) * kStage;
+    const char* lb_ = la_ + OA::kBytes;
+#pragma unroll
+    for (int s = 0; s < BK / F::kStep; ++s) {
+      typename F::Type fa[FM], fb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        fb[j] = F::template read<BN, BCOLS>(lb_, wn + j * 16, s, lane);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        fa[i] = F::template read<BM, ACOLS>(la_, wm + i * 16, s, lane);
+      // n along the rows of the result: a lane holds four neighbours
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
+    }
+  }
+  __syncthreads();
+
+  // ---- epilogue ----
+  // Each wave passes 32 rows at a time through LDS of its own, from the
+  // matrix cores' layout to eight neighbouring n a lane: full lines to and
+  // from memory, and the activation once in a loop instead of unrolled over
+  // all accumulators.
+  constexpr int LPR = TN / 8, RPI = 64 / LPR, ITER = 32 / RPI;
+  char* mine = lds + wave * 32 * EROW;
+  const long n = n0 + wn + (lane % LPR) * 8;
+  const int left = (int)max(0l, min(8l, g.N - n));
+  const bool whole = n0 + wn + TN <= g.N;
+  float bias[8] = {};
+  if (EPI != kPlain && EPI != kPartial && e.bias && left) {
+    if (e.bias_f32)
+      load8(bias, static_cast<const float*>(e.bias) + n, left);
+    else
+      load8(bias, static_cast<const T*>(e.bias) + n, left);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bias[j] *= e.bias_gain;
+  }
+  float sums[8] = {};
+#pragma unroll
+  for (int h = 0; h < FM / 2; ++h) {
+    const long mh = m0 + wm + h * 32 + lane / LPR;
+    // on its way while the activation is computed
+    Eight<T> other[ITER];
+    const T* op = EPI == kForward ? e.residual : EPI == kSlope ? e.dy : nullptr;
+    const long os = EPI == kForward ? e.res_stride : e.dy_stride;
+    if (op && whole) {
+#pragma unroll
+      for (int q = 0; q < ITER; ++q)
+        other[q].load(op + min(mh + q * RPI, g.M - 1) * os + n);
+    } else if (op) {
+#pragma unroll
+      for (int q = 0; q < ITER; ++q)
+        other[q].load(op + min(mh + q * RPI, g.M - 1) * os + n, left);
+    }
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        acc[i][j] = TO::mfma(As, Bs, wm + i * 16, wn + j * 16, lane,
-                             acc[i][j]);
+      for (int j = 0; j < FN; ++j)
+        *reinterpret_cast<f32x4*>(mine + (i * 16 + (lane & 15)) * EROW +
+                                  (j * 16 + (lane >> 4) * 4) * 4) =
+            acc[h * 2 + i][j];
+    __builtin_amdgcn_wave_barrier();
+    char* at = mine + lane / LPR * EROW + (lane % LPR) * 32;
+    if (EPI == kForward || EPI == kSlope) {
+#pragma unroll 1
+      for (int q = 0; q < ITER; ++q) {
+        f32x4* p = reinterpret_cast<f32x4*>(at + q * RPI * EROW);
+        f32x4 v[2] = {p[0], p[1]};
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          z[j] = g.alpha * v[j / 4][j % 4] + bias[j];
+        const long m = mh + q * RPI;
+        if (EPI == kForward && e.z && m < g.M) store8(e.z + m * g.N + n, z, left);
+        if (EPI == kForward)
+          act_values(z, e.act);
+        else
+          act_slopes(z, e.act);
+        p[0] = f32x4{z[0], z[1], z[2], z[3]};
+        p[1] = f32x4{z[4], z[5], z[6], z[7]};
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < ITER; ++q) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(at + q * RPI * EROW);
+      const f32x4 v[2] = {p[0], p[1]};
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        o[j] = v[j / 4][j % 4];
+        if (EPI == kPlain) o[j] *= g.alpha;
+      }
+      const long m = mh + q * RPI;
+      if (m >= g.M) continue;
+      if (EPI == kForward && op) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] += other[q][j];
+      }
+      if (EPI == kSlope) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          o[j] *= other[q][j];
+          sums[j] += o[j];
+        }
+      }
+      if constexpr (EPI == kPartial)
+        store8(e.partial + ((long)blockIdx.y * g.M + m) * g.N + n, o, left);
+      else
+        store8(c + m * g.ldc + n, o, left);
+    }
+  }
+  if (EPI == kSlope && e.partial) {
+    // the block's sums over its rows: lanes of the same columns, then the
+    // waves one above the other
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      for (int o = LPR; o < 64; o <<= 1) sums[j] += __shfl_xor(sums[j], o);
+    __syncthreads();
+    float* s = reinterpret_cast<float*>(lds);
+    if (lane < LPR)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        s[wave / WN * BN + wn + lane * 8 + j] = sums[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < BN; i += WAVES * 64) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < WM; ++w) v += s[w * BN + i];
+      if (n0 + i < g.N) e.partial[(long)mt * g.N + n0 + i] = v;
+    }
+  }
+}
+
+// C = alpha * sum of the splits
+template <typename T>
+__global__ __launch_bounds__(256)
+void sum_splits(T* __restrict__ c, const float* __restrict__ partial,
+                int splits, long count, float alpha) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= count) return;
+  const int left = (int)min(8l, count - i);
+  float s[8] = {};
+  for (int q = 0; q < splits; ++q) {
+    float v[8];
+    load8(v, partial + q * count + i, left);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += v[j];
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const long m = m0 + wm + i * 16 + (lane >> 4) * 4 + q;
-        const long n = n0 + wn + j * 16 + (lane & 15);
-        if (m >= g.M || n >= g.N) continue;
-        float z = g.alpha * acc[i][j][q];
-        if (e.bias)
-          z += e.bias_gain * (e.bias_f32
-                                  ? static_cast<const float*>(e.bias)[n]
-                                  : to_f32(static_cast<const T*>(e.bias)[n]));
-        if (e.z) put(e.z + m * g.N + n, z);
-        float y = act_value(z, e.act);
-        if (e.residual) y += to_f32(e.residual[m * e.res_stride + n]);
-        put(c + m * g.N + n, y);
-      }
+  for (int j = 0; j < 8; ++j) s[j] *= alpha;
+  store8(c + i, s, left);
+}
+
+// dst[r][0..width) = src[r][0..n), zero behind: 16-byte rows for the tiles
+template <typename T>
+__global__ __launch_bounds__(256)
+void pad_rows(T* __restrict__ dst, const T* __restrict__ src, long stride,
+              long rows, int n, int width) {
+  const long count = rows * (width / 8);
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count;
+       i += (long)gridDim.x * 256) {
+    const long r = i / (width / 8);
+    const int col = (int)(i % (width / 8)) * 8;
+    float v[8];
+    load8(v, src + r * stride + col, min(8, n - col));
+    store8(dst + r * width + col, v, 8);
+  }
 }
 
 template <typename T>
-void launch_linear_gemm(T* c, const T* a, const T* b, const GemmArgs& g,
-                        const EpilogueArgs<T>& e, hipStream_t s) {
-  hipLaunchKernelGGL(linear_gemm_kernel<T>,
-                     dim3(ceil_div(g.M, 64), ceil_div(g.N, 64)), dim3(256), 0,
-                     s, c, a, b, g, e);
+void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
+                     int width, hipStream_t s) {
+  const long blocks = (rows * (width / 8) + 255) / 256;
+  hipLaunchKernelGGL(pad_rows<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)),
+                     dim3(256), 0, s, dst, src, stride, rows, n, width);
 }
 
+namespace {
+
+struct Tile {
+  int bm, bn;
+};
+
+// The largest tile that still gives every CU a block: large tiles read
+// their operands less often, small ones spread a small product wider.
+Tile tile_for(long M, long N, int splits) {
+  auto blocks = [&](int b) {
+    return ((M + b - 1) / b) * ((N + b - 1) / b) * splits;
+  };
+  if (blocks(256) >= 256) return {256, 256};
+  if (blocks(128) >= 192) return {128, 128};
+  return {64, 64};
+}
+
+template <typename T, bool ACOLS, bool BCOLS, int EPI>
+void launch_tile(T* c, const T* a, const T* b, const GemmArgs& g,
+                 const EpilogueArgs<T>& e, int splits, hipStream_t s) {
+  const Tile t = tile_for(g.M, g.N, splits);
+  const long tiles = ceil_div(g.M, t.bm) * (long)ceil_div(g.N, t.bn);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), splits);
+  if (t.bm == 256)
+    hipLaunchKernelGGL((linear_tile<T, 256, 256, 2, 4, ACOLS, BCOLS, EPI>),
+                       grid, dim3(512), 0, s, g, e, c, a, b);
+  else if (t.bm == 128)
+    hipLaunchKernelGGL((linear_tile<T, 128, 128, 2, 2, ACOLS, BCOLS, EPI>),
+                       grid, dim3(256), 0, s, g, e, c, a, b);
+  else
+    hipLaunchKernelGGL((linear_tile<T, 64, 64, 2, 2, ACOLS, BCOLS, EPI>),
+                       grid, dim3(256), 0, s, g, e, c, a, b);
+}
+
+}  // namespace
+
+int linear_row_tiles(long M, long N) {
+  return ceil_div(M, tile_for(M, N, 1).bm);
+}
+
+// Splits of a long k where the tiles of C alone leave CUs idle: enough for
+// about two blocks of 128x128 a CU, at least 16 k-tiles each.
+int linear_splits(long M, long N, long K, bool f32) {
+  const long tiles = (long)ceil_div(M, 128) * ceil_div(N, 128);
+  const long depth = f32 ? 512 : 1024;
+  const long want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+  const long most = (K + depth - 1) / depth;
+  return (int)(want < most ? want : most);
+}
+
+template <typename T>
+void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
+                           const EpilogueArgs<T>& e, hipStream_t s) {
+  launch_tile<T, false, false, kForward>(y, x, w, g, e, 1, s);
+}
+
+template <typename T>
+void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
+                         const EpilogueArgs<T>& e, hipStream_t s) {
+  launch_tile<T, false, false, kSlope>(dz, x, w, g, e, 1, s);
+}
+
+template <typename T>
+void launch_linear_dx(T* dx, const T* dz, const T* w, const GemmArgs& g,
+                      hipStream_t s) {
+  launch_tile<T, false, true, kPlain>(dx, dz, w, g, EpilogueArgs<T>{}, 1, s);
+}
+
+template <typename T>
+void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
+                      GemmArgs g, hipStream_t s) {
+  const int splits = linear_splits(g.M, g.N, g.K, sizeof(T) == 4);
+  EpilogueArgs<T> e{};
+  if (splits == 1) {
+    launch_tile<T, true, true, kPlain>(dw, dz, x, g, e, 1, s);
+    return;
+  }
+  const long bk = 128 / sizeof(T);
+  g.k_split = ((g.K + splits - 1) / splits + bk - 1) / bk * bk;
+  const int used = (int)((g.K + g.k_split - 1) / g.k_split);
+  e.partial = partial;
+  launch_tile<T, true, true, kPartial>(dw, dz, x, g, e, used, s);
+  const long count = g.M * g.N;
+  hipLaunchKernelGGL(sum_splits<T>, dim3(ceil_div(count, 2048)), dim3(256), 0,
+                     s, dw, partial, used, count, g.alpha);
+}
+
+// ---- dz from a kept z, and sums over rows ----
 // thread: one column; block: 256 columns of one group of rows
 template <typename T>
 __global__ __launch_bounds__(256)
-void linear_dz_kernel(T* __restrict__ dz, float* __restrict__ partial,
-                      const T* __restrict__ dy, long dy_stride,
-                      const T* __restrict__ z, ActParams act, long rows,
-                      int n) {
+void linear_dz_kernel(T* __restrict__ dz, long dz_stride,
+                      float* __restrict__ partial, const T* __restrict__ dy,
+                      long dy_stride, const float* __restrict__ z,
+                      ActParams act, long rows, int n) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   const int groups = gridDim.y;
   const long per = (rows + groups - 1) / groups;
@@ -96,8 +574,8 @@ void linear_dz_kernel(T* __restrict__ dz, float* __restrict__ partial,
   for (long r = r0; r < r1; ++r) {
     float d = to_f32(dy[r * dy_stride + i]);
     if (z) {
-      d *= act_slope(to_f32(z[r * n + i]), act);
-      put(dz + r * n + i, d);
+      d *= act_slope(z[r * n + i], act);
+      put(dz + r * dz_stride + i, d);
     }
     sum += d;  // before its rounding
   }
@@ -110,21 +588,32 @@ int linear_dz_groups(long rows, int n) {
 }
 
 template <typename T>
-void launch_linear_dz(T* dz, float* partial, const T* dy, long dy_stride,
-                      const T* z, const ActParams& act, long rows, int n,
-                      hipStream_t s) {
+void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
+                      long dy_stride, const float* z, const ActParams& act,
+                      long rows, int n, hipStream_t s) {
   hipLaunchKernelGGL(linear_dz_kernel<T>,
                      dim3(ceil_div(n, 256), linear_dz_groups(rows, n)),
-                     dim3(256), 0, s, dz, partial, dy, dy_stride, z, act,
-                     rows, n);
+                     dim3(256), 0, s, dz, dz_stride, partial, dy, dy_stride, z,
+                     act, rows, n);
 }
 
 #define INSTANTIATE(T)                                                       \
-  template void launch_linear_gemm<T>(T*, const T*, const T*,                \
-                                      const GemmArgs&,                       \
-                                      const EpilogueArgs<T>&, hipStream_t);  \
-  template void launch_linear_dz<T>(T*, float*, const T*, long, const T*,    \
-                                    const ActParams&, long, int, hipStream_t);
+  template void launch_linear_forward<T>(T*, const T*, const T*,             \
+                                         const GemmArgs&,                    \
+                                         const EpilogueArgs<T>&,             \
+                                         hipStream_t);                       \
+  template void launch_linear_slope<T>(T*, const T*, const T*,               \
+                                       const GemmArgs&,                      \
+                                       const EpilogueArgs<T>&, hipStream_t); \
+  template void launch_linear_dx<T>(T*, const T*, const T*, const GemmArgs&, \
+                                    hipStream_t);                            \
+  template void launch_linear_dw<T>(T*, float*, const T*, const T*,          \
+                                    GemmArgs, hipStream_t);                  \
+  template void launch_pad_rows<T>(T*, const T*, long, long, int, int,       \
+                                   hipStream_t);                             \
+  template void launch_linear_dz<T>(T*, long, float*, const T*, long,        \
+                                    const float*, const ActParams&, long,    \
+                                    int, hipStream_t);
 INSTANTIATE(float)
 INSTANTIATE(bf16)
 

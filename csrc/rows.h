@@ -24,55 +24,87 @@ struct ActParams {
   float alpha, gain, clamp;  // clamp: infinity for none
 };
 
+// f(v[j]) for eight values behind one switch over the activation.
 // Comparisons are written so that a NaN takes the branch that keeps it.
-GFA_DEV float act_value(float z, const ActParams& p) {
-  float a = z;
+template <int N>
+GFA_DEV void act_values(float (&z)[N], const ActParams& p) {
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = f(z[j]);
+  };
   switch (p.act) {
-    case kRelu: a = z <= 0.f ? 0.f : z; break;
-    case kLrelu: a = z <= 0.f ? p.alpha * z : z; break;
-    case kTanh: a = tanhf(z); break;
-    case kSigmoid: a = 1.f / (1.f + expf(-z)); break;
-    case kGelu: a = 0.5f * z * (1.f + erff(z * 0.70710678f)); break;
-    case kSilu: a = z / (1.f + expf(-z)); break;
+    case kRelu: each([](float z) { return z <= 0.f ? 0.f : z; }); break;
+    case kLrelu:
+      each([&](float z) { return z <= 0.f ? p.alpha * z : z; });
+      break;
+    case kTanh: each([](float z) { return tanhf(z); }); break;
+    case kSigmoid: each([](float z) { return 1.f / (1.f + expf(-z)); }); break;
+    case kGelu:
+      each([](float z) { return 0.5f * z * (1.f + erff(z * 0.70710678f)); });
+      break;
+    case kSilu: each([](float z) { return z / (1.f + expf(-z)); }); break;
   }
-  a *= p.gain;
-  return a > p.clamp ? p.clamp : a < -p.clamp ? -p.clamp : a;
+  each([&](float a) {
+    a *= p.gain;
+    return a > p.clamp ? p.clamp : a < -p.clamp ? -p.clamp : a;
+  });
 }
 
 // d y / d z at z, zero where the clamp holds
-GFA_DEV float act_slope(float z, const ActParams& p) {
-  float a = z, s = 1.f;
+template <int N>
+GFA_DEV void act_slopes(float (&z)[N], const ActParams& p) {
+  // f: activation and slope
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float a, s;
+      f(z[j], a, s);
+      z[j] = fabsf(a * p.gain) >= p.clamp ? 0.f : s * p.gain;
+    }
+  };
   switch (p.act) {
+    case kLinear:
+      each([](float z, float& a, float& s) { s = 1.f, a = z; });
+      break;
     case kRelu:
-      s = z <= 0.f ? 0.f : 1.f;
-      a = s * z;
+      each([](float z, float& a, float& s) {
+        s = z <= 0.f ? 0.f : 1.f, a = s * z;
+      });
       break;
     case kLrelu:
-      s = z <= 0.f ? p.alpha : 1.f;
-      a = s * z;
+      each([&](float z, float& a, float& s) {
+        s = z <= 0.f ? p.alpha : 1.f, a = s * z;
+      });
       break;
     case kTanh:
-      a = tanhf(z);
-      s = 1.f - a * a;
+      each([](float z, float& a, float& s) {
+        a = tanhf(z), s = 1.f - a * a;
+      });
       break;
     case kSigmoid:
-      a = 1.f / (1.f + expf(-z));
-      s = a * (1.f - a);
+      each([](float z, float& a, float& s) {
+        a = 1.f / (1.f + expf(-z)), s = a * (1.f - a);
+      });
       break;
-    case kGelu: {
-      const float cdf = 0.5f * (1.f + erff(z * 0.70710678f));
-      a = z * cdf;
-      s = cdf + z * 0.39894228f * expf(-0.5f * z * z);
+    case kGelu:
+      each([](float z, float& a, float& s) {
+        const float cdf = 0.5f * (1.f + erff(z * 0.70710678f));
+        a = z * cdf, s = cdf + z * 0.39894228f * expf(-0.5f * z * z);
+      });
       break;
-    }
-    case kSilu: {
-      const float g = 1.f / (1.f + expf(-z));
-      a = z * g;
-      s = g * (1.f + z * (1.f - g));
+    case kSilu:
+      each([](float z, float& a, float& s) {
+        const float g = 1.f / (1.f + expf(-z));
+        a = z * g, s = g * (1.f + z * (1.f - g));
+      });
       break;
-    }
   }
-  return fabsf(a * p.gain) >= p.clamp ? 0.f : s * p.gain;
+}
+
+GFA_DEV float act_slope(float z, const ActParams& p) {
+  float v[1] = {z};
+  act_slopes(v, p);
+  return v[0];
 }
 
 // T: float or bf16. P: type of the parameters (null pointer for none).
@@ -93,34 +125,57 @@ template <typename P>
 void launch_sum_groups(P* out0, P* out1, const float* partial, int groups,
                        int n, float scale, hipStream_t);
 
-// C[m, n] = epilogue(alpha * sum_k A[m, k] B[n, k]); one of the two strides
-// of A and of B is 1
+// C[m, n] = epilogue(alpha * sum_k A[m, k] B[n, k]). lda, ldb: strides of
+// the operands' rows (or columns), multiples of 16 bytes below 2^20.
 struct GemmArgs {
   long M, N, K;
-  long sam, sak;  // strides of A
-  long sbn, sbk;  // strides of B
+  long lda, ldb, ldc;
   float alpha;
+  long k_split;  // k of one split, a multiple of the tiles' depth
 };
+enum Epilogue { kPlain = 0, kForward, kSlope, kPartial };
 template <typename T>
 struct EpilogueArgs {
   const void* bias;  // [N] or null
   bool bias_f32;
   float bias_gain;
-  const T* residual;  // [M, N] with rows of res_stride, or null
-  long res_stride;
-  T* z;  // [M, N] or null
   ActParams act;
+  const T* residual;  // forward: [M, N] with rows of res_stride, or null
+  long res_stride;
+  float* z;     // forward: [M, N] or null
+  const T* dy;  // slope: [M, N] with rows of dy_stride
+  long dy_stride;
+  float* partial;  // slope: sums over the rows of each row of tiles, or null
 };
+// y = clamp(act(alpha x W^T + bias) * gain) + residual
 template <typename T>
-void launch_linear_gemm(T* c, const T* a, const T* b, const GemmArgs& g,
-                        const EpilogueArgs<T>& e, hipStream_t);
+void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
+                           const EpilogueArgs<T>& e, hipStream_t);
+// dz = dy * slope(alpha x W^T + bias); linear_row_tiles sums of rows
+int linear_row_tiles(long M, long N);
+template <typename T>
+void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
+                         const EpilogueArgs<T>& e, hipStream_t);
+// dx[M, N] = alpha dz[M, K] W[K, N]
+template <typename T>
+void launch_linear_dx(T* dx, const T* dz, const T* w, const GemmArgs& g,
+                      hipStream_t);
+// dw[M, N] = alpha dz[K, M]^T x[K, N]; partial: linear_splits * M * N floats,
+// unused for one split
+int linear_splits(long M, long N, long K, bool f32);
+template <typename T>
+void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
+                      GemmArgs g, hipStream_t);
+template <typename T>
+void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
+                     int width, hipStream_t);
 
 // dz = dy * slope(z) (z and dz null: dz = dy) and, unless partial is null,
 // partial[g][n] = sums of dz over the rows of group g
 int linear_dz_groups(long rows, int n);
 template <typename T>
-void launch_linear_dz(T* dz, float* partial, const T* dy, long dy_stride,
-                      const T* z, const ActParams& act, long rows, int n,
-                      hipStream_t);
+void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
+                      long dy_stride, const float* z, const ActParams& act,
+                      long rows, int n, hipStream_t s);
 
 }  // namespace gfa
