@@ -26,22 +26,32 @@ hipStream_t cur_stream() {
   return c10::hip::getCurrentHIPStream().stream();
 }
 
-void check(const Tensor& t, const Tensor& x, const char* what) {
-  TORCH_CHECK(t.is_cuda() && t.device() == x.device(), what,
-              ": on another device than x");
-  TORCH_CHECK(t.scalar_type() == torch::kFloat32 ||
-                  t.scalar_type() == torch::kBFloat16,
-              what, ": expected float32 or bfloat16, got ", t.scalar_type());
+// Arguments that do not fit raise ValueError, as the Python side does.
+#define CHECK_ARG TORCH_CHECK_VALUE
+
+void check_device(const Tensor& t, const Tensor& x, const char* op,
+                  const char* what) {
+  CHECK_ARG(t.device() == x.device(), op, ": ", what, " is on ", t.device(),
+            ", x on ", x.device());
+}
+
+void check_x(const Tensor& x, const char* op) {
+  CHECK_ARG(x.is_cuda() && (x.scalar_type() == torch::kFloat32 ||
+                            x.scalar_type() == torch::kBFloat16),
+            op, ": expected float32 or bfloat16 on the GPU, got ",
+            x.scalar_type(), " on ", x.device());
 }
 
 void check_param(const OptTensor& p, const Tensor& x, int64_t n,
-                 const char* what) {
+                 const char* op, const char* what) {
   if (!p) return;
-  check(*p, x, what);
-  TORCH_CHECK(p->dim() == 1 && p->size(0) == n, what, ": expected [", n, "]");
-  TORCH_CHECK(p->scalar_type() == x.scalar_type() ||
-                  p->scalar_type() == torch::kFloat32,
-              what, ": expected x's dtype or float32");
+  CHECK_ARG(p->dim() == 1 && p->size(0) == n, op, ": ", what,
+            ": expected shape [", n, "], got ", p->sizes());
+  check_device(*p, x, op, what);
+  CHECK_ARG(p->scalar_type() == x.scalar_type() ||
+                p->scalar_type() == torch::kFloat32,
+            op, ": ", what, ": expected ", x.scalar_type(),
+            " or float32, got ", p->scalar_type());
 }
 
 // A tensor [..., n] as rows of n contiguous elements at one stride
@@ -108,21 +118,27 @@ T* mptr(const OptTensor& t) {
   } while (0)
 
 bool params_f32(const OptTensor& w, const OptTensor& b) {
-  TORCH_CHECK(!w || !b || w->scalar_type() == b->scalar_type(),
-              "layer_norm: weight and bias differ in dtype");
   return w ? w->scalar_type() == torch::kFloat32
            : !b || b->scalar_type() == torch::kFloat32;
+}
+
+void check_layer_norm(const Tensor& x, const OptTensor& w,
+                      const OptTensor& b) {
+  const char* op = "layer_norm";
+  check_x(x, op);
+  CHECK_ARG(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1 << 30), op,
+            ": x needs a last dimension of at least 1 (and below 2^30), got "
+            "shape ", x.sizes());
+  check_param(w, x, x.size(-1), op, "weight");
+  check_param(b, x, x.size(-1), op, "bias");
+  CHECK_ARG(!w || !b || w->scalar_type() == b->scalar_type(), op,
+            ": weight is ", w->scalar_type(), ", bias ", b->scalar_type());
 }
 
 std::tuple<Tensor, OptTensor, OptTensor> layer_norm_fwd(
     const Tensor& x, const OptTensor& w, const OptTensor& b, double eps,
     bool save) {
-  check(x, x, "layer_norm: x");
-  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1 << 30),
-              "layer_norm: size of the last dimension");
   const int n = (int)x.size(-1);
-  check_param(w, x, n, "layer_norm: weight");
-  check_param(b, x, n, "layer_norm: bias");
   const bool p32 = params_f32(w, b);
   c10::hip::HIPGuard guard(x.get_device());
   const OptTensor wc = w ? OptTensor(w->contiguous()) : w;
@@ -150,24 +166,14 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
     const Tensor& dy, const Tensor& x, const OptTensor& w, const OptTensor& b,
     const Tensor& mean, const Tensor& rstd, bool need_dx, bool need_dw,
     bool need_db) {
-  check(x, x, "layer_norm: x");
-  check(dy, x, "layer_norm: dy");
-  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < (1 << 30),
-              "layer_norm: size of the last dimension");
-  TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(),
+  TORCH_CHECK(dy.device() == x.device() && dy.sizes() == x.sizes() &&
+                  dy.scalar_type() == x.scalar_type(),
               "layer_norm: dy does not fit x");
   const int n = (int)x.size(-1);
-  check_param(w, x, n, "layer_norm: weight");
-  check_param(b, x, n, "layer_norm: bias");
   const bool p32 = params_f32(w, b);
   c10::hip::HIPGuard guard(x.get_device());
   const OptTensor wc = w ? OptTensor(w->contiguous()) : w;
   const Rows xr = rows_of(x), dr = rows_of(dy);
-  for (const Tensor& s : {mean, rstd})
-    TORCH_CHECK(s.device() == x.device() && s.is_contiguous() &&
-                    s.scalar_type() == torch::kFloat32 &&
-                    s.numel() == xr.count,
-                "layer_norm: statistics do not fit x");
   const auto f32 = x.options().dtype(torch::kFloat32);
   const auto popt = p32 ? f32 : x.options();
   OptTensor dx, dw, db, partial;
@@ -197,16 +203,36 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
 
 // ---- linear ----
 
-void check_linear(const Tensor& x, const Tensor& w, const OptTensor& bias) {
-  check(x, x, "linear_act: x");
-  check(w, x, "linear_act: weight");
-  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) &&
-                  w.size(0) >= 1 && w.size(1) >= 1 &&
-                  w.size(0) < (1 << 20) && w.size(1) < (1 << 20) &&
-                  w.scalar_type() == x.scalar_type(),
-              "linear_act: weight does not fit x");
-  check_param(bias, x, w.size(0), "linear_act: bias");
+void check_linear(const Tensor& x, const Tensor& w, const OptTensor& bias,
+                  const OptTensor& residual) {
+  const char* op = "linear_act";
+  check_x(x, op);
+  CHECK_ARG(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1), op,
+            ": x ", x.sizes(), " and weight ", w.sizes(), " do not fit");
+  CHECK_ARG(w.size(0) >= 1 && w.size(1) >= 1, op, ": empty weight ",
+            w.sizes());
+  CHECK_ARG(w.size(0) < (1 << 20) && w.size(1) < (1 << 20), op,
+            ": weight of ", w.sizes(), ": sizes below 2^20 are served");
+  check_device(w, x, op, "weight");
+  CHECK_ARG(w.scalar_type() == x.scalar_type(), op, ": weight is ",
+            w.scalar_type(), ", x ", x.scalar_type());
+  check_param(bias, x, w.size(0), op, "bias");
+  if (!residual) return;
+  CHECK_ARG(residual->dim() == x.dim() && residual->size(-1) == w.size(0) &&
+                residual->sizes().slice(0, x.dim() - 1) ==
+                    x.sizes().slice(0, x.dim() - 1),
+            op, ": residual ", residual->sizes(), " does not fit the output");
+  check_device(*residual, x, op, "residual");
+  CHECK_ARG(residual->scalar_type() == x.scalar_type(), op, ": residual is ",
+            residual->scalar_type(), ", x ", x.scalar_type());
 }
+
+struct LinearParams {
+  int64_t act;
+  double alpha, gain, clamp, weight_gain, bias_gain;
+  // Without an activation or a clamp the slope is the gain everywhere.
+  bool curved() const { return act != gfa::kLinear || !std::isinf(clamp); }
+};
 
 std::vector<int64_t> out_shape(const Tensor& x, int64_t n) {
   auto s = x.sizes().vec();
@@ -230,32 +256,24 @@ Rows tile_rows(const Rows& r, int64_t n) {
 }
 
 template <typename T>
-gfa::EpilogueArgs<T> epilogue(const OptTensor& bias, int64_t act, double alpha,
-                              double gain, double clamp, double bias_gain) {
+gfa::EpilogueArgs<T> epilogue(const OptTensor& bias, const LinearParams& p) {
   gfa::EpilogueArgs<T> e{};
   if (bias) {
     e.bias = bias->data_ptr();
     e.bias_f32 = bias->scalar_type() == torch::kFloat32;
-    e.bias_gain = (float)bias_gain;
+    e.bias_gain = (float)p.bias_gain;
   }
-  e.act = {(int)act, (float)alpha, (float)gain, (float)clamp};
+  e.act = {(int)p.act, (float)p.alpha, (float)p.gain, (float)p.clamp};
   return e;
 }
 
-std::tuple<Tensor, OptTensor> linear_act_fwd(
-    const Tensor& x, const Tensor& w, const OptTensor& bias,
-    const OptTensor& residual, int64_t act, double alpha, double gain,
-    double clamp, double weight_gain, double bias_gain, bool save_z) {
-  check_linear(x, w, bias);
-  TORCH_CHECK(act >= 0 && act <= gfa::kSilu, "linear_act: activation");
+std::tuple<Tensor, OptTensor> linear_act_fwd(const Tensor& x, const Tensor& w,
+                                             const OptTensor& bias,
+                                             const OptTensor& residual,
+                                             const LinearParams& p,
+                                             bool save_z) {
   const int64_t n = w.size(0), k = w.size(1);
   const auto shape = out_shape(x, n);
-  if (residual) {
-    check(*residual, x, "linear_act: residual");
-    TORCH_CHECK(residual->sizes() == shape &&
-                    residual->scalar_type() == x.scalar_type(),
-                "linear_act: residual does not fit");
-  }
   c10::hip::HIPGuard guard(x.get_device());
   const OptTensor bc = bias ? OptTensor(bias->contiguous()) : bias;
   Tensor y = torch::empty(shape, x.options());
@@ -265,7 +283,7 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(
   DISPATCH_FT(x.scalar_type(), {
     const Rows xr = tile_rows<scalar_t>(rows_of(x), k);
     const Rows wr = tile_rows<scalar_t>(rows_of(w), k);
-    auto e = epilogue<scalar_t>(bc, act, alpha, gain, clamp, bias_gain);
+    auto e = epilogue<scalar_t>(bc, p);
     Rows rr;
     if (residual) {
       rr = rows_of(*residual);
@@ -276,7 +294,7 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(
     gfa::launch_linear_forward<scalar_t>(
         static_cast<scalar_t*>(y.data_ptr()), cptr<scalar_t>(xr.t),
         cptr<scalar_t>(wr.t),
-        {xr.count, n, k, xr.stride, wr.stride, n, (float)weight_gain, k}, e,
+        {xr.count, n, k, xr.stride, wr.stride, n, (float)p.weight_gain, k}, e,
         cur_stream());
   });
   HIP_CHECK_LAST();
@@ -285,22 +303,12 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(
 
 std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     const Tensor& dy, const OptTensor& z, const Tensor& x, const Tensor& w,
-    const OptTensor& bias, int64_t act, double alpha, double gain,
-    double clamp, double weight_gain, double bias_gain, bool need_dx,
-    bool need_dw, bool need_db) {
-  check_linear(x, w, bias);
-  TORCH_CHECK(act >= 0 && act <= gfa::kSilu, "linear_act: activation");
+    const OptTensor& bias, const LinearParams& p, bool need_dx, bool need_dw,
+    bool need_db) {
   const int64_t n = w.size(0), k = w.size(1);
-  const auto shape = out_shape(x, n);
-  check(dy, x, "linear_act: dy");
-  TORCH_CHECK(dy.sizes() == shape && dy.scalar_type() == x.scalar_type(),
+  TORCH_CHECK(dy.device() == x.device() && dy.sizes() == out_shape(x, n) &&
+                  dy.scalar_type() == x.scalar_type(),
               "linear_act: dy does not fit");
-  TORCH_CHECK(!need_db || bias, "linear_act: no bias");
-  if (z)
-    TORCH_CHECK(z->device() == x.device() && z->is_contiguous() &&
-                    z->sizes() == shape &&
-                    z->scalar_type() == torch::kFloat32,
-                "linear_act: z does not fit");
   c10::hip::HIPGuard guard(x.get_device());
   const int64_t m = dy.numel() / n;
   OptTensor dx, dw, db;
@@ -315,15 +323,14 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
   if (!need_dx && !need_dw && !need_db) return {dx, dw, db};
   const OptTensor bc = bias ? OptTensor(bias->contiguous()) : bias;
   const auto f32 = x.options().dtype(torch::kFloat32);
-  // Without an activation or a clamp the slope is the gain everywhere: dz is
-  // dy and the products carry the factor.
-  const bool curved = act != gfa::kLinear || !std::isinf(clamp);
-  const double slope = curved ? 1.0 : gain;
+  // a slope that is the same everywhere goes into the products: dz is dy
+  const bool curved = p.curved();
+  const double slope = curved ? 1.0 : p.gain;
   DISPATCH_FT(x.scalar_type(), {
     const Rows xr = tile_rows<scalar_t>(rows_of(x), k);
     const Rows wr = tile_rows<scalar_t>(rows_of(w), k);
     Rows dr = rows_of(dy);
-    auto e = epilogue<scalar_t>(bc, act, alpha, gain, clamp, bias_gain);
+    auto e = epilogue<scalar_t>(bc, p);
     OptTensor partial;
     int groups = 0;
     if (curved && !z) {
@@ -338,7 +345,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
       gfa::launch_linear_slope<scalar_t>(
           static_cast<scalar_t*>(dz.t.data_ptr()), cptr<scalar_t>(xr.t),
           cptr<scalar_t>(wr.t),
-          {m, n, k, xr.stride, wr.stride, width, (float)weight_gain, k}, e,
+          {m, n, k, xr.stride, wr.stride, width, (float)p.weight_gain, k}, e,
           cur_stream());
       dr = dz;
     } else if (curved || need_db) {
@@ -354,7 +361,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
       if (curved) dr = dz;
     }
     if (need_db) {
-      const float scale = (float)(bias_gain * slope);
+      const float scale = (float)(p.bias_gain * slope);
       if (bias->scalar_type() == torch::kFloat32)
         gfa::launch_sum_groups<float>(mptr<float>(db), nullptr,
                                       partial->data_ptr<float>(), groups,
@@ -364,7 +371,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
                                           partial->data_ptr<float>(), groups,
                                           (int)n, scale, cur_stream());
     }
-    const float scale = (float)(weight_gain * slope);
+    const float scale = (float)(p.weight_gain * slope);
     if (need_dx || need_dw) dr = tile_rows<scalar_t>(dr, n);
     if (need_dx)
       gfa::launch_linear_dx<scalar_t>(
@@ -385,13 +392,172 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
   return {dx, dw, db};
 }
 
+// ---- autograd ----
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor plain(const OptTensor& t) { return t ? *t : Tensor(); }
+bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
+
+// Which of the tensors (null: not given) need a gradient. The context counts
+// only those that are there.
+std::vector<bool> needed(AutogradContext* ctx, const variable_list& in) {
+  std::vector<bool> need;
+  size_t k = 0;
+  for (const Tensor& t : in)
+    need.push_back(t.defined() && ctx->needs_input_grad(k++));
+  return need;
+}
+
+// Differentiable gradients of f(inputs) in those that need one, for a
+// backward that is itself differentiated. Through a view of each input: one
+// may come from another (a residual and what was made from it), and this
+// operator's gradient must not run on into that history.
+template <typename F>
+variable_list composed_grads(const variable_list& in,
+                             const std::vector<bool>& need, const Tensor& dy,
+                             F&& f) {
+  variable_list views, wanted;
+  for (size_t i = 0; i < in.size(); ++i) {
+    views.push_back(in[i].defined() ? in[i].view_as(in[i]) : Tensor());
+    if (need[i]) wanted.push_back(views.back());
+  }
+  const variable_list got = torch::autograd::grad(
+      {f(views)}, wanted, {dy}, /*retain_graph=*/std::nullopt,
+      /*create_graph=*/true);
+  variable_list out(in.size());
+  size_t k = 0;
+  for (size_t i = 0; i < in.size(); ++i)
+    if (need[i]) out[i] = got[k++];
+  return out;
+}
+
+Tensor composed_layer_norm(const variable_list& in, double eps) {
+  const Tensor x = in[0].to(torch::kFloat32);
+  const Tensor xc = x - x.mean(-1, true);
+  Tensor y = xc * (xc.square().mean(-1, true) + eps).rsqrt();
+  if (in[1].defined()) y = y * in[1];
+  if (in[2].defined()) y = y + in[2];
+  return y.to(in[0].scalar_type());
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x,
+                        const OptTensor& w, const OptTensor& b, double eps) {
+    auto [y, mean, rstd] = layer_norm_fwd(x, w, b, eps, true);
+    ctx->save_for_backward({x, plain(w), plain(b), *mean, *rstd});
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto s = ctx->get_saved_variables();
+    const variable_list in{s[0], s[1], s[2]};
+    const auto need = needed(ctx, in);
+    if (torch::GradMode::is_enabled()) {
+      const double eps = ctx->saved_data["eps"].toDouble();
+      auto out = composed_grads(in, need, dy[0], [&](const variable_list& v) {
+        return composed_layer_norm(v, eps);
+      });
+      out.emplace_back();
+      return out;
+    }
+    const auto [dx, dw, db] =
+        layer_norm_bwd(dy[0], s[0], opt(s[1]), opt(s[2]), s[3], s[4], need[0],
+                       need[1], need[2]);
+    return {plain(dx), plain(dw), plain(db), Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b,
+                  double eps) {
+  check_layer_norm(x, w, b);
+  if (torch::GradMode::is_enabled() &&
+      (x.requires_grad() || wants_grad(w) || wants_grad(b)))
+    return LayerNorm::apply(x, w, b, eps);
+  return std::get<0>(layer_norm_fwd(x, w, b, eps, false));
+}
+
+Tensor composed_linear_act(const variable_list& in, const LinearParams& p) {
+  Tensor z = torch::matmul(in[0].to(torch::kFloat32),
+                           in[1].to(torch::kFloat32).t()) * p.weight_gain;
+  if (in[2].defined()) z = z + in[2].to(torch::kFloat32) * p.bias_gain;
+  Tensor y = z;
+  switch (p.act) {
+    case gfa::kRelu: y = torch::relu(z); break;
+    case gfa::kLrelu: y = torch::leaky_relu(z, p.alpha); break;
+    case gfa::kTanh: y = torch::tanh(z); break;
+    case gfa::kSigmoid: y = torch::sigmoid(z); break;
+    case gfa::kGelu: y = z * 0.5 * (1.0 + torch::erf(z * M_SQRT1_2)); break;
+    case gfa::kSilu: y = z * torch::sigmoid(z); break;
+  }
+  y = y * p.gain;
+  if (!std::isinf(p.clamp)) y = y.clamp(-p.clamp, p.clamp);
+  if (in[3].defined()) y = y + in[3];
+  return y.to(in[0].scalar_type());
+}
+
+// Whether the forward keeps z for the backward, in 32 bits (a rounded z
+// would cost the slopes, and the bias's gradient, their digits). Keeping it
+// moves 8 bytes an element and a pass over dz; computing it again costs k
+// multiplications an element and happens where dz is made. The two meet at
+// about 1500 (bf16) and 128 (float) multiplications.
+bool keeps_z(const Tensor& x, const LinearParams& p) {
+  return p.curved() &&
+         x.size(-1) > (x.scalar_type() == torch::kFloat32 ? 128 : 1536);
+}
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
+                        const OptTensor& bias, const OptTensor& residual,
+                        const LinearParams& p) {
+    auto [y, z] = linear_act_fwd(x, w, bias, residual, p, keeps_z(x, p));
+    ctx->save_for_backward({x, w, plain(bias), plain(residual), plain(z)});
+    ctx->saved_data["params"] =
+        std::vector<double>{(double)p.act, p.alpha,       p.gain,
+                            p.clamp,       p.weight_gain, p.bias_gain};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dy) {
+    const auto s = ctx->get_saved_variables();
+    const auto d = ctx->saved_data["params"].toDoubleVector();
+    const LinearParams p{(int64_t)d[0], d[1], d[2], d[3], d[4], d[5]};
+    const variable_list in{s[0], s[1], s[2], s[3]};
+    const auto need = needed(ctx, in);
+    if (torch::GradMode::is_enabled()) {
+      auto out = composed_grads(in, need, dy[0], [&](const variable_list& v) {
+        return composed_linear_act(v, p);
+      });
+      out.emplace_back();
+      return out;
+    }
+    const auto [dx, dw, db] =
+        linear_act_bwd(dy[0], opt(s[4]), s[0], s[1], opt(s[2]), p, need[0],
+                       need[1], need[2]);
+    return {plain(dx), plain(dw), plain(db), need[3] ? dy[0] : Tensor(),
+            Tensor()};
+  }
+};
+
+Tensor linear_act(const Tensor& x, const Tensor& w, const OptTensor& bias,
+                  const OptTensor& residual, int64_t act, double alpha,
+                  double gain, double clamp, double weight_gain,
+                  double bias_gain) {
+  check_linear(x, w, bias, residual);
+  CHECK_ARG(act >= 0 && act <= gfa::kSilu, "linear_act: activation ", act);
+  const LinearParams p{act, alpha, gain, clamp, weight_gain, bias_gain};
+  if (torch::GradMode::is_enabled() &&
+      (x.requires_grad() || w.requires_grad() || wants_grad(bias) ||
+       wants_grad(residual)))
+    return LinearAct::apply(x, w, bias, residual, p);
+  return std::get<0>(linear_act_fwd(x, w, bias, residual, p, false));
+}
+
 }  // namespace
 
 void bind_rows(pybind11::module& m) {
-  m.def("layer_norm_fwd", &layer_norm_fwd,
-        "layer norm -> (y, mean, rstd)");
-  m.def("layer_norm_bwd", &layer_norm_bwd, "layer norm -> (dx, dw, db)");
-  m.def("linear_act_fwd", &linear_act_fwd,
-        "clamp(act(x W^T + b) * gain) + residual -> (y, z)");
-  m.def("linear_act_bwd", &linear_act_bwd, "linear_act -> (dx, dW, db)");
+  m.def("layer_norm", &layer_norm, "layer norm over the last dimension");
+  m.def("linear_act", &linear_act,
+        "clamp(act(wg x W^T + bg b) * gain) + residual");
 }

@@ -20,9 +20,9 @@ using LdsPtr = __attribute__((address_space(3))) void*;
 // ---- tiles ----
 // A block computes BM x BN of C with WM x WN waves. Both operands of a k-tile
 // go from memory to LDS without passing through registers, 1 KB a wave and
-// instruction; a k-tile is 128 bytes deep (64 bf16, 32 float) and there are
-// two of them, one being filled while the other is used, with one barrier
-// between. Reads outside the operands return zero (the bounds are those of
+// instruction; a k-tile is 128 bytes deep (64 bf16, 32 float) and STAGES of
+// them are in LDS, one being used while the others are filled, with one
+// barrier a k-tile. Reads outside the operands return zero (the bounds are those of
 // the buffer descriptor), so any M, N, K take this path as long as rows are
 // 16-byte aligned.
 //
@@ -192,12 +192,21 @@ GFA_DEV void store8(bf16* p, const float* v, int left) {
 GFA_DEV auto buffer_at(const void* p, long bytes) {
   const long most = 0x7ffffff0;
   return __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<void*>(p), 0, (int)(bytes < most ? bytes : most),
+      const_cast<void*>(p), 0, (int)max(0l, min(bytes, most)),
       0x00020000);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ACOLS, bool BCOLS,
-          int EPI>
+// waits until at most N of the wave's pieces are under way and its LDS reads
+// are done, then for the block's other waves
+template <int N>
+GFA_DEV void wait_pieces() {
+  static_assert(N < 64, "six bits of vmcnt");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N)
+               : "memory");
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool ACOLS,
+          bool BCOLS, int EPI>
 __global__ __launch_bounds__(WM * WN * 64)
 void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
                  const T* __restrict__ a, const T* __restrict__ b) {
@@ -211,7 +220,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   // the epilogue turns 32 rows of a wave at a time in LDS
   constexpr int EROW = TN * 4 + 16;
   constexpr int kEpi = WAVES * 32 * EROW;
-  constexpr int kLds = 2 * kStage > kEpi ? 2 * kStage : kEpi;
+  constexpr int kLds = STAGES * kStage > kEpi ? STAGES * kStage : kEpi;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
 
   const int lane = threadIdx.x & 63;
@@ -261,6 +270,8 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 
   auto fetch = [&](int t, int stage) {
     char* base = lds + stage * kStage;
+    // past the last k-tile: nothing is read, zeros arrive, the counts of
+    // pieces under way stay what the waits expect
     const auto ra = buffer_at(pa + t * sa, la - t * sa);
     const auto rb = buffer_at(pb + t * sb, lb - t * sb);
     const int left = kn - t * BK;
@@ -284,13 +295,16 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const int wm = wave / WN * TM, wn = wave % WN * TN;
   f32x4 acc[FM][FN] = {};
   const int tiles = (kn + BK - 1) / BK;
-  fetch(0, 0);
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) fetch(t, t);
+  int use = 0, fill = STAGES - 1;
   for (int t = 0; t < tiles; ++t) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's pieces
-    __syncthreads();
-    if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
-    const char* la_ = lds + (t & 1) * kStage;
+    wait_pieces<(STAGES - 2) * (PA + PB)>();
+    if (STAGES > 2 || t + 1 < tiles) fetch(t + STAGES - 1, fill);
+    const char* la_ = lds + use * kStage;
     const char* lb_ = la_ + OA::kBytes;
+    use = use + 1 == STAGES ? 0 : use + 1;
+    fill = fill + 1 == STAGES ? 0 : fill + 1;
 #pragma unroll
     for (int s = 0; s < BK / F::kStep; ++s) {
       typename F::Type fa[FM], fb[FN];
@@ -308,7 +322,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
           acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
     }
   }
-  __syncthreads();
+  wait_pieces<0>();  // the epilogue writes where the pieces go
 
   // ---- epilogue ----
   // Each wave passes 32 rows at a time through LDS of its own, from the
@@ -398,7 +412,10 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
           sums[j] += o[j];
         }
       }
-      if constexpr (EPI == kPartial)
+      // dz has padded rows, zero behind the last element
+      if constexpr (EPI == kSlope) {
+        if (left) store8(c + m * g.ldc + n, o, 8);
+      } else if constexpr (EPI == kPartial)
         store8(e.partial + ((long)blockIdx.y * g.M + m) * g.N + n, o, left);
       else
         store8(c + m * g.ldc + n, o, left);
@@ -426,24 +443,38 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   }
 }
 
-// C = alpha * sum of the splits
+// C = alpha * sum of the splits: 256 elements a block, 32 threads of eight
+// side by side, blockDim / 32 of them for every so manieth split
 template <typename T>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(1024)
 void sum_splits(T* __restrict__ c, const float* __restrict__ partial,
                 int splits, long count, float alpha) {
-  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= count) return;
-  const int left = (int)min(8l, count - i);
+  __shared__ float red[32][257];
+  const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int groups = blockDim.x >> 5;
+  const long i0 = (long)blockIdx.x * 256, i = i0 + lane * 8;
+  const int left = (int)max(0l, min(8l, count - i));
   float s[8] = {};
-  for (int q = 0; q < splits; ++q) {
-    float v[8];
-    load8(v, partial + q * count + i, left);
+  if (left) {
+#pragma unroll 4
+    for (int k = q; k < splits; k += groups) {
+      Eight<float> v;
+      if (left == 8)
+        v.load(partial + k * count + i);
+      else
+        v.load(partial + k * count + i, left);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] += v[j];
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s[j] *= alpha;
-  store8(c + i, s, left);
+  for (int j = 0; j < 8; ++j) red[q][lane * 8 + j] = s[j];
+  __syncthreads();
+  for (int k = threadIdx.x; k < 256 && i0 + k < count; k += blockDim.x) {
+    float v = 0.f;
+    for (int g = 0; g < groups; ++g) v += red[g][k];
+    put(c + i0 + k, alpha * v);
+  }
 }
 
 // dst[r][0..width) = src[r][0..n), zero behind: 16-byte rows for the tiles
@@ -473,18 +504,18 @@ void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
 namespace {
 
 struct Tile {
-  int bm, bn;
+  int bm, bn, stages;
 };
 
-// The largest tile that still gives every CU a block: large tiles read
-// their operands less often, small ones spread a small product wider.
+static int LT = getenv("LT") ? atoi(getenv("LT")) : 0;
 Tile tile_for(long M, long N, int splits) {
   auto blocks = [&](int b) {
     return ((M + b - 1) / b) * ((N + b - 1) / b) * splits;
   };
-  if (blocks(256) >= 256) return {256, 256};
-  if (blocks(128) >= 192) return {128, 128};
-  return {64, 64};
+  if (LT) return {LT / 10, LT / 10, LT % 10};
+  if (blocks(256) >= 256) return {256, 256, 2};
+  if (blocks(128) >= 192) return {128, 128, 2};
+  return {64, 64, 4};
 }
 
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
@@ -493,15 +524,22 @@ void launch_tile(T* c, const T* a, const T* b, const GemmArgs& g,
   const Tile t = tile_for(g.M, g.N, splits);
   const long tiles = ceil_div(g.M, t.bm) * (long)ceil_div(g.N, t.bn);
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8), splits);
+#define LAUNCH(B, WM, WN, ST)                                                 \
+  hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, ST, ACOLS, BCOLS, EPI>),   \
+                     grid, dim3(WM * WN * 64), 0, s, g, e, c, a, b)
   if (t.bm == 256)
-    hipLaunchKernelGGL((linear_tile<T, 256, 256, 2, 4, ACOLS, BCOLS, EPI>),
-                       grid, dim3(512), 0, s, g, e, c, a, b);
+    LAUNCH(256, 2, 4, 2);
+  else if (t.bm == 128 && t.stages == 2)
+    LAUNCH(128, 2, 2, 2);
   else if (t.bm == 128)
-    hipLaunchKernelGGL((linear_tile<T, 128, 128, 2, 2, ACOLS, BCOLS, EPI>),
-                       grid, dim3(256), 0, s, g, e, c, a, b);
+    LAUNCH(128, 2, 2, 4);
+  else if (t.stages == 4)
+    LAUNCH(64, 2, 2, 4);
+  else if (t.stages == 2)
+    LAUNCH(64, 2, 2, 2);
   else
-    hipLaunchKernelGGL((linear_tile<T, 64, 64, 2, 2, ACOLS, BCOLS, EPI>),
-                       grid, dim3(256), 0, s, g, e, c, a, b);
+    LAUNCH(64, 2, 2, 8);
+#undef LAUNCH
 }
 
 }  // namespace
@@ -553,48 +591,107 @@ void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
   e.partial = partial;
   launch_tile<T, true, true, kPartial>(dw, dz, x, g, e, used, s);
   const long count = g.M * g.N;
-  hipLaunchKernelGGL(sum_splits<T>, dim3(ceil_div(count, 2048)), dim3(256), 0,
-                     s, dw, partial, used, count, g.alpha);
+  int groups = 1;
+  while (groups < 32 && groups * 4 < used) groups *= 2;
+  hipLaunchKernelGGL(sum_splits<T>, dim3(ceil_div(count, 256)),
+                     dim3(32 * groups), 0, s, dw, partial, used, count,
+                     g.alpha);
 }
 
 // ---- dz from a kept z, and sums over rows ----
-// thread: one column; block: 256 columns of one group of rows
+// A block takes every so manieth row: `wide` threads of eight columns side
+// by side, 256 / wide rows at a time, four of them under way.
 template <typename T>
 __global__ __launch_bounds__(256)
 void linear_dz_kernel(T* __restrict__ dz, long dz_stride,
                       float* __restrict__ partial, const T* __restrict__ dy,
                       long dy_stride, const float* __restrict__ z,
-                      ActParams act, long rows, int n) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const int groups = gridDim.y;
-  const long per = (rows + groups - 1) / groups;
-  const long r0 = blockIdx.y * per, r1 = min(r0 + per, rows);
-  if (i >= n) return;
-  float sum = 0.f;
-  for (long r = r0; r < r1; ++r) {
-    float d = to_f32(dy[r * dy_stride + i]);
-    if (z) {
-      d *= act_slope(z[r * n + i], act);
-      put(dz + r * dz_stride + i, d);
+                      ActParams act, long rows, int n, int wide) {
+  constexpr int U = 4;
+  __shared__ float red[256][9];
+  const int high = 256 / wide, q = threadIdx.x / wide;
+  const int i = (blockIdx.x * wide + threadIdx.x % wide) * 8;
+  const int left = max(0, min(8, n - i));
+  const long step = (long)gridDim.y * high;
+  float sum[8] = {};
+  for (long r = (long)blockIdx.y * high + q; left && r < rows; r += U * step) {
+    Eight<T> d[U];
+    Eight<float> zz[U];
+    // rows past the last repeat it and are not counted
+    if (left == 8) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long at = min(r + u * step, rows - 1);
+        d[u].load(dy + at * dy_stride + i);
+        if (z) zz[u].load(z + at * n + i);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long at = min(r + u * step, rows - 1);
+        d[u].load(dy + at * dy_stride + i, left);
+        if (z) zz[u].load(z + at * n + i, left);
+      }
     }
-    sum += d;  // before its rounding
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r + u * step >= rows) break;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = d[u][j];
+      if (z) {
+        float s[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = zz[u][j];
+        act_slopes(s, act);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= s[j];
+        // padded rows, zero behind the last element
+        store8(dz + (r + u * step) * dz_stride + i, v, 8);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += v[j];  // before their rounding
+    }
   }
-  if (partial) partial[(long)blockIdx.y * n + i] = sum;
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[threadIdx.x][j] = sum[j];
+  __syncthreads();
+  for (int k = threadIdx.x; k < wide * 8; k += 256) {
+    const int col = blockIdx.x * wide * 8 + k;
+    if (col >= n) break;
+    float v = 0.f;
+    for (int h = 0; h < high; ++h) v += red[h * wide + k / 8][k % 8];
+    partial[(long)blockIdx.y * n + col] = v;
+  }
 }
 
+namespace {
+// threads side by side: as many as a row of n needs, at most a wave's half
+int dz_wide(int n) {
+  int wide = 1;
+  while (wide < 32 && wide * 8 < n) wide *= 2;
+  return wide;
+}
+}  // namespace
+
+// Row groups: at most about two blocks a CU, at least four rows a thread.
 int linear_dz_groups(long rows, int n) {
-  const long g = (rows + 63) / 64;
-  return (int)(g < 256 ? g : 256);
+  const int wide = dz_wide(n), high = 256 / wide;
+  const long most = (rows + 4 * high - 1) / (4 * high);
+  const long want = (512 + ceil_div(n, wide * 8) - 1) / ceil_div(n, wide * 8);
+  return (int)(most < want ? most : want);
 }
 
 template <typename T>
 void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
                       long dy_stride, const float* z, const ActParams& act,
                       long rows, int n, hipStream_t s) {
+  const int wide = dz_wide(n);
   hipLaunchKernelGGL(linear_dz_kernel<T>,
-                     dim3(ceil_div(n, 256), linear_dz_groups(rows, n)),
+                     dim3(ceil_div(n, wide * 8), linear_dz_groups(rows, n)),
                      dim3(256), 0, s, dz, dz_stride, partial, dy, dy_stride, z,
-                     act, rows, n);
+                     act, rows, n, wide);
 }
 
 #define INSTANTIATE(T)                                                       \

@@ -8,7 +8,8 @@ Stands beside `modnorm` (instance norm over the pixels of a channel with
 a scale and shift per element) as the normalization of a TOKEN over its
 channels. The HIP kernels (csrc/layer_norm.hip) run forward and first-order
 backward, the sums over the rows for the parameters' gradients included;
-a create_graph backward goes through the differentiable composition.
+their autograd function (csrc/ext_rows.hip) sends a create_graph backward
+through a differentiable composition.
 """
 
 from __future__ import annotations
@@ -30,44 +31,6 @@ def _eager_layer_norm(x, weight, bias, eps):
     return y.to(x.dtype)
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = native.require_ext().layer_norm_fwd(
-            x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.eps = eps
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        if torch.is_grad_enabled():
-            # create_graph: differentiate the composition again, from the
-            # inputs (the saved statistics are constants to autograd)
-            return _eager_grads(
-                lambda *t: _eager_layer_norm(*t, ctx.eps),
-                (x, weight, bias), need, dy) + (None,)
-        dx, dw, db = native.require_ext().layer_norm_bwd(
-            dy, x, weight, bias, mean, rstd, need[0], need[1], need[2])
-        return dx, dw, db, None
-
-
-def _eager_grads(fn, inputs, need, dy):
-    """Differentiable gradients of fn(*inputs) in those that need one.
-
-    Through a view of each input: one input may come from another (a
-    residual and the normalized residual), and the gradient of this
-    operator alone must not run on into that history.
-    """
-    views = [None if t is None else t.view_as(t) for t in inputs]
-    got = iter(torch.autograd.grad(
-        fn(*views), [t for t, n in zip(views, need) if n], dy,
-        create_graph=True))
-    return tuple(next(got) if n else None for n in need[:len(inputs)])
-
-
 def _check_param(name, p, x, shape):
     if p is None:
         return
@@ -81,9 +44,6 @@ def _check_param(name, p, x, shape):
                          f"got {p.dtype}")
 
 
-_GPU_DTYPES = (torch.float32, torch.bfloat16)
-
-
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Normalize x [..., N] over its last dimension.
 
@@ -93,6 +53,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     bfloat16. Rows may be strided (a slice of a wider tensor is read in
     place as long as its last dimension is contiguous).
     """
+    if x.is_cuda:  # checks its arguments likewise
+        return native.require_ext().layer_norm(x, weight, bias, eps)
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm: x needs a last dimension of at "
                          f"least 1, got shape {tuple(x.shape)}")
@@ -102,14 +64,4 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError(f"layer_norm: weight is {weight.dtype}, "
                          f"bias {bias.dtype}")
-    if not native.use_native(x):
-        return _eager_layer_norm(x, weight, bias, eps)
-    if x.dtype not in _GPU_DTYPES:
-        raise ValueError(f"layer_norm: expected float32 or bfloat16 on the "
-                         f"GPU, got {x.dtype}")
-    if torch.is_grad_enabled() and (
-            x.requires_grad or (weight is not None and weight.requires_grad)
-            or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, float(eps))
-    return native.require_ext().layer_norm_fwd(x, weight, bias, eps,
-                                               False)[0]
+    return _eager_layer_norm(x, weight, bias, eps)

@@ -10,9 +10,10 @@ weight, a library product, a bias/activation pass and an addition. Backward:
     dx = weight_gain * dz @ weight      dweight = weight_gain * dz^T @ x
     dbias = bias_gain * sum_rows dz     dresidual = dy
 
-z is kept for the backward in x's dtype where the activation (or a clamp)
-needs it. All four products run on the kernels of csrc/linear_act.hip; a
-create_graph backward goes through the differentiable composition.
+All products run on the kernels of csrc/linear_act.hip. A backward that
+needs z takes it from the product again, or from 32 bits kept by the forward
+where that is quicker. The autograd function (csrc/ext_rows.hip) sends a
+create_graph backward through a differentiable composition.
 """
 
 from __future__ import annotations
@@ -23,7 +24,7 @@ import torch
 
 from . import native
 from .fused_act import _eager_act, activation_defs
-from .layer_norm import _GPU_DTYPES, _check_param, _eager_grads
+from .layer_norm import _check_param
 
 # bias_act's activations and the two smooth ones of feed-forward layers:
 # gelu(z) = z * Phi(z) (exact, by erf) and silu(z) = z * sigmoid(z)
@@ -56,37 +57,6 @@ def _eager_linear_act(x, weight, bias, residual, act, alpha, gain, clamp,
     return y.to(x.dtype)
 
 
-class _LinearAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, alpha, gain, clamp,
-                weight_gain, bias_gain):
-        code = linear_activations[act][0]
-        # a linear layer's slope is the gain everywhere
-        keep = act != "linear" or clamp is not None
-        y, z = native.require_ext().linear_act_fwd(
-            x, weight, bias, residual, code, alpha, gain,
-            math.inf if clamp is None else clamp, weight_gain, bias_gain,
-            keep)
-        ctx.save_for_backward(x, weight, bias, residual, z)
-        ctx.params = (act, alpha, gain, clamp, weight_gain, bias_gain)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight, bias, residual, z = ctx.saved_tensors
-        act, alpha, gain, clamp, weight_gain, bias_gain = ctx.params
-        need = ctx.needs_input_grad
-        if torch.is_grad_enabled():
-            return _eager_grads(
-                lambda *t: _eager_linear_act(*t, *ctx.params),
-                (x, weight, bias, residual), need, dy) + (None,) * 6
-        dx, dw, db = native.require_ext().linear_act_bwd(
-            dy, z, x, weight, bias, linear_activations[act][0], alpha, gain,
-            math.inf if clamp is None else clamp, weight_gain, bias_gain,
-            need[0], need[1], need[2])
-        return (dx, dw, db, dy if need[3] else None) + (None,) * 6
-
-
 def linear_act(x, weight, bias=None, act="linear", residual=None, alpha=None,
                gain=None, clamp=None, weight_gain=1.0, bias_gain=1.0):
     """clamp(act(weight_gain * x @ weight^T + bias_gain * bias) * gain)
@@ -99,8 +69,19 @@ def linear_act(x, weight, bias=None, act="linear", residual=None, alpha=None,
     once from 32 bits. On the GPU x is float32 or bfloat16; x, weight and
     residual may have strided rows.
     """
-    if act not in linear_activations:
+    spec = linear_activations.get(act)
+    if spec is None:
         raise ValueError(f"linear_act: unknown activation {act!r}")
+    if alpha is None:
+        alpha = spec[1]
+    if gain is None:
+        gain = spec[2]
+    if clamp is not None and clamp < 0:
+        clamp = None
+    if x.is_cuda:  # checks its arguments likewise
+        return native.require_ext().linear_act(
+            x, weight, bias, residual, spec[0], alpha, gain,
+            math.inf if clamp is None else clamp, weight_gain, bias_gain)
     if x.ndim < 1 or weight.ndim != 2 or weight.shape[1] != x.shape[-1]:
         raise ValueError(f"linear_act: x {tuple(x.shape)} and weight "
                          f"{tuple(weight.shape)} do not fit")
@@ -119,23 +100,5 @@ def linear_act(x, weight, bias=None, act="linear", residual=None, alpha=None,
         if residual.dtype != x.dtype or residual.device != x.device:
             raise ValueError(f"linear_act: residual is {residual.dtype} on "
                              f"{residual.device}, x {x.dtype} on {x.device}")
-    _, def_alpha, def_gain, _ = linear_activations[act]
-    alpha = float(def_alpha if alpha is None else alpha)
-    gain = float(def_gain if gain is None else gain)
-    clamp = None if clamp is None or clamp < 0 else float(clamp)
-    if not native.use_native(x):
-        return _eager_linear_act(x, weight, bias, residual, act, alpha, gain,
-                                 clamp, weight_gain, bias_gain)
-    if x.dtype not in _GPU_DTYPES:
-        raise ValueError(f"linear_act: expected float32 or bfloat16 on the "
-                         f"GPU, got {x.dtype}")
-    if torch.is_grad_enabled() and (
-            x.requires_grad or weight.requires_grad
-            or (bias is not None and bias.requires_grad)
-            or (residual is not None and residual.requires_grad)):
-        return _LinearAct.apply(x, weight, bias, residual, act, alpha, gain,
-                                clamp, float(weight_gain), float(bias_gain))
-    return native.require_ext().linear_act_fwd(
-        x, weight, bias, residual, linear_activations[act][0], alpha, gain,
-        math.inf if clamp is None else clamp, weight_gain, bias_gain,
-        False)[0]
+    return _eager_linear_act(x, weight, bias, residual, act, alpha, gain,
+                             clamp, weight_gain, bias_gain)
