@@ -255,6 +255,12 @@ Rows tile_rows(const Rows& r, int64_t n) {
   return p;
 }
 
+// room for the sums of k in parts
+OptTensor split_sums(int splits, int64_t m, int64_t n, const Tensor& like) {
+  if (splits <= 1) return {};
+  return torch::empty({splits, m, n}, like.options().dtype(torch::kFloat32));
+}
+
 template <typename T>
 gfa::EpilogueArgs<T> epilogue(const OptTensor& bias, const LinearParams& p) {
   gfa::EpilogueArgs<T> e{};
@@ -291,11 +297,15 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(const Tensor& x, const Tensor& w,
       e.res_stride = rr.stride;
     }
     e.z = mptr<float>(z);
+    const int splits = gfa::linear_splits(
+        xr.count, n, k, std::is_same_v<scalar_t, float>, false);
+    const OptTensor parts = split_sums(splits, xr.count, n, x);
+    e.partial = mptr<float>(parts);
     gfa::launch_linear_forward<scalar_t>(
         static_cast<scalar_t*>(y.data_ptr()), cptr<scalar_t>(xr.t),
         cptr<scalar_t>(wr.t),
         {xr.count, n, k, xr.stride, wr.stride, n, (float)p.weight_gain, k}, e,
-        cur_stream());
+        splits, cur_stream());
   });
   HIP_CHECK_LAST();
   return {y, z};
@@ -373,19 +383,22 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     }
     const float scale = (float)(p.weight_gain * slope);
     if (need_dx || need_dw) dr = tile_rows<scalar_t>(dr, n);
-    if (need_dx)
+    constexpr bool is_f32 = std::is_same_v<scalar_t, float>;
+    if (need_dx) {
+      const int splits = gfa::linear_splits(m, k, n, is_f32, false);
+      const OptTensor parts = split_sums(splits, m, k, x);
       gfa::launch_linear_dx<scalar_t>(
-          mptr<scalar_t>(dx), cptr<scalar_t>(dr.t), cptr<scalar_t>(wr.t),
-          {m, k, n, dr.stride, wr.stride, k, scale, n}, cur_stream());
+          mptr<scalar_t>(dx), mptr<float>(parts), cptr<scalar_t>(dr.t),
+          cptr<scalar_t>(wr.t),
+          {m, k, n, dr.stride, wr.stride, k, scale, n}, splits, cur_stream());
+    }
     if (need_dw) {
-      const int splits =
-          gfa::linear_splits(n, k, m, std::is_same_v<scalar_t, float>);
-      OptTensor parts;
-      if (splits > 1) parts = torch::empty({splits, n, k}, f32);
+      const int splits = gfa::linear_splits(n, k, m, is_f32, true);
+      const OptTensor parts = split_sums(splits, n, k, x);
       gfa::launch_linear_dw<scalar_t>(
           mptr<scalar_t>(dw), mptr<float>(parts), cptr<scalar_t>(dr.t),
           cptr<scalar_t>(xr.t),
-          {n, k, m, dr.stride, xr.stride, k, scale, m}, cur_stream());
+          {n, k, m, dr.stride, xr.stride, k, scale, m}, splits, cur_stream());
     }
   });
   HIP_CHECK_LAST();

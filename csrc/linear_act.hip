@@ -46,10 +46,8 @@ struct Operand {
     return s & (kGran - 1);
   }
 
-  // byte offset from the tile's corner for a lane of the wave's i-th piece
-  template <int WAVES>
-  GFA_DEV static int source(int wave, int i, int lane, int stride) {
-    const int idx = (i * WAVES + wave) * 64 + lane;
+  // byte offset from the tile's corner of what belongs at granule idx
+  GFA_DEV static int source(int idx, int stride) {
     const int r = idx / kGran, p = idx % kGran;
     return r * stride * ES + ((p ^ swizzle(r)) << 4);
   }
@@ -189,13 +187,6 @@ GFA_DEV void store8(bf16* p, const float* v, int left) {
   }
 }
 
-GFA_DEV auto buffer_at(const void* p, long bytes) {
-  const long most = 0x7ffffff0;
-  return __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<void*>(p), 0, (int)max(0l, min(bytes, most)),
-      0x00020000);
-}
-
 // waits until at most N of the wave's pieces are under way and its LDS reads
 // are done, then for the block's other waves
 template <int N>
@@ -205,6 +196,66 @@ GFA_DEV void wait_pieces() {
                : "memory");
 }
 
+GFA_DEV auto buffer_at(const void* p, long bytes) {
+  const long most = 0x7ffffff0;
+  return __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<void*>(p), 0, (int)max(0l, min(bytes, most)),
+      0x00020000);
+}
+
+// One operand's way into LDS: pieces of 1 KB, DEPTH k-tiles a stage, shared
+// out over the block's waves.
+template <typename T, int BX, bool COLS, int WAVES, int DEPTH>
+struct Loader {
+  using O = Operand<T, BX, COLS>;
+  static constexpr int ES = sizeof(T), BK = O::BK;
+  static constexpr int kTile = BX / 8;  // pieces of a k-tile
+  static constexpr int kPieces = kTile * DEPTH / WAVES;
+  static_assert(kTile * DEPTH % WAVES == 0, "whole pieces a wave");
+  const char* corner;
+  long bytes;  // from there to the operand's end, whose rows end with a
+               // whole granule
+  long step;   // bytes from one k-tile to the next
+  int kn, wave, lane;
+  int offset[kPieces];
+
+  // x0: first row (column) of the tile, X: all of them; kb, kn: part of k
+  GFA_DEV Loader(const T* p, long stride, long x0, long X, long kb, int kn_,
+                 int wave_, int lane_)
+      : kn(kn_), wave(wave_), lane(lane_) {
+    auto whole16 = [](long v) { return (v * ES + 15) & ~15l; };
+    corner = reinterpret_cast<const char*>(COLS ? p + kb * stride + x0
+                                                : p + x0 * stride + kb);
+    bytes = COLS ? (kn - 1) * stride * ES + whole16(X) - x0 * ES
+                 : (X - x0 - 1) * stride * ES + whole16(kn);
+    step = (COLS ? BK * stride : BK) * ES;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      offset[i] = O::source(piece(i) % kTile * 64 + lane, (int)stride);
+  }
+  GFA_DEV int piece(int i) const { return i * WAVES + wave; }
+
+  // Stage t of the operand. Past the end nothing is read and zeros arrive,
+  // so the counts of pieces under way stay what the waits expect.
+  GFA_DEV void fetch(char* lds, int t) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int q = t * DEPTH + piece(i) / kTile;
+      int off = offset[i];
+      if constexpr (!COLS) {
+        // rows: the last k-tile is cut off at the end of k
+        const int idx = piece(i) % kTile * 64 + lane;
+        const int k = ((idx & 7) ^ O::swizzle(idx >> 3)) * (16 / ES);
+        const int left = kn - q * BK;
+        if (left < BK && k >= left) off = 0x7ffffff8;
+      }
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          buffer_at(corner + q * step, bytes - q * step),
+          (LdsPtr)(lds + piece(i) * 1024), 16, off, 0, 0, 0);
+    }
+  }
+};
+
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool ACOLS,
           bool BCOLS, int EPI>
 __global__ __launch_bounds__(WM * WN * 64)
@@ -213,9 +264,8 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   using OA = Operand<T, BM, ACOLS>;
   using OB = Operand<T, BN, BCOLS>;
   using F = Frag<T>;
-  constexpr int ES = sizeof(T), BK = OA::BK, WAVES = WM * WN;
+  constexpr int BK = OA::BK, WAVES = WM * WN;
   constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  constexpr int PA = BM / 8 / WAVES, PB = BN / 8 / WAVES;
   constexpr int kStage = OA::kBytes + OB::kBytes;
   // the epilogue turns 32 rows of a wave at a time in LDS
   constexpr int EROW = TN * 4 + 16;
@@ -241,55 +291,13 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const long kb = (long)blockIdx.y * g.k_split;
   const int kn = (int)min(g.K - kb, g.k_split);
 
-  const char* pa = reinterpret_cast<const char*>(
-      ACOLS ? a + kb * g.lda + m0 : a + m0 * g.lda + kb);
-  const char* pb = reinterpret_cast<const char*>(
-      BCOLS ? b + kb * g.ldb + n0 : b + n0 * g.ldb + kb);
-  // bytes from the corner of the tile to the end of the operand, whose rows
-  // end with a whole granule
-  auto whole16 = [](long v) { return (v * ES + 15) & ~15l; };
-  const long la = ACOLS ? (kn - 1) * g.lda * ES + whole16(g.M) - m0 * ES
-                        : (g.M - m0 - 1) * g.lda * ES + whole16(kn);
-  const long lb = BCOLS ? (kn - 1) * g.ldb * ES + whole16(g.N) - n0 * ES
-                        : (g.N - n0 - 1) * g.ldb * ES + whole16(kn);
-  const long sa = (ACOLS ? BK * g.lda : BK) * ES;
-  const long sb = (BCOLS ? BK * g.ldb : BK) * ES;
-
-  int va[PA], vb[PB];
-#pragma unroll
-  for (int i = 0; i < PA; ++i)
-    va[i] = OA::template source<WAVES>(wave, i, lane, (int)g.lda);
-#pragma unroll
-  for (int i = 0; i < PB; ++i)
-    vb[i] = OB::template source<WAVES>(wave, i, lane, (int)g.ldb);
-  // rows: the lane's k within a k-tile, past which the last one is cut off
-  auto k_of = [&](int i) {
-    const int idx = (i * WAVES + wave) * 64 + lane;
-    return ((idx & 7) ^ ((idx >> 4) & 7)) * (16 / ES);
-  };
-
+  using LA = Loader<T, BM, ACOLS, WAVES, 1>;
+  using LB = Loader<T, BN, BCOLS, WAVES, 1>;
+  const LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
+  const LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
   auto fetch = [&](int t, int stage) {
-    char* base = lds + stage * kStage;
-    // past the last k-tile: nothing is read, zeros arrive, the counts of
-    // pieces under way stay what the waits expect
-    const auto ra = buffer_at(pa + t * sa, la - t * sa);
-    const auto rb = buffer_at(pb + t * sb, lb - t * sb);
-    const int left = kn - t * BK;
-#pragma unroll
-    for (int i = 0; i < PA; ++i) {
-      const int off = !ACOLS && left < BK && k_of(i) >= left ? 0x7ffffff8
-                                                             : va[i];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          ra, (LdsPtr)(base + (i * WAVES + wave) * 1024), 16, off, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      const int off = !BCOLS && left < BK && k_of(i) >= left ? 0x7ffffff8
-                                                             : vb[i];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rb, (LdsPtr)(base + OA::kBytes + (i * WAVES + wave) * 1024), 16,
-          off, 0, 0, 0);
-    }
+    load_a.fetch(lds + stage * kStage, t);
+    load_b.fetch(lds + stage * kStage + OA::kBytes, t);
   };
 
   const int wm = wave / WN * TM, wn = wave % WN * TN;
@@ -299,7 +307,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   for (int t = 0; t < STAGES - 1; ++t) fetch(t, t);
   int use = 0, fill = STAGES - 1;
   for (int t = 0; t < tiles; ++t) {
-    wait_pieces<(STAGES - 2) * (PA + PB)>();
+    wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
     if (STAGES > 2 || t + 1 < tiles) fetch(t + STAGES - 1, fill);
     const char* la_ = lds + use * kStage;
     const char* lb_ = la_ + OA::kBytes;
@@ -443,6 +451,161 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   }
 }
 
+// The epilogue of four sums of row m from column n on, the first `left` of
+// them within the matrix; they become what was written, 0 outside.
+template <typename T, int EPI>
+GFA_DEV void finish4(float (&o)[4], long m, long n, int left,
+                     const GemmArgs& g, const EpilogueArgs<T>& e, T* c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] *= g.alpha;
+  if constexpr (EPI == kForward || EPI == kSlope) {
+    if (e.bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left)
+          o[j] += e.bias_gain *
+                  (e.bias_f32 ? static_cast<const float*>(e.bias)[n + j]
+                              : to_f32(static_cast<const T*>(e.bias)[n + j]));
+    }
+    if (EPI == kForward && e.z)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < left) e.z[m * g.N + n + j] = o[j];
+    if (EPI == kForward)
+      act_values(o, e.act);
+    else
+      act_slopes(o, e.act);
+    const T* p = EPI == kForward ? e.residual : e.dy;
+    if (p) {
+      p += m * (EPI == kForward ? e.res_stride : e.dy_stride) + n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float r = j < left ? to_f32(p[j]) : 0.f;
+        o[j] = EPI == kForward ? o[j] + r : o[j] * r;
+      }
+    }
+  }
+  // dz has rows padded to eight, zero behind the last element
+  const long end = EPI == kSlope && left > 0 ? g.ldc - n : left;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= left) o[j] = 0.f;
+    if (j < end) put(c + m * g.ldc + n + j, o[j]);
+  }
+}
+
+// Products that tiles of 64x64 spread over too few CUs: 32x32 of C a block.
+// The four waves share out k instead of C (each takes every fourth step of
+// all 32x32), so a block's operands pass through LDS once and its time falls
+// with k alone; their sums meet in LDS. Where that still leaves CUs idle, k
+// is split over blocks too (kPartial).
+template <typename T, bool ACOLS, bool BCOLS, int EPI>
+__global__ __launch_bounds__(256)
+void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
+                  const T* __restrict__ a, const T* __restrict__ b) {
+  constexpr int B = 32, DEPTH = 2, STAGES = 4, WAVES = 4;
+  using OA = Operand<T, B, ACOLS>;
+  using F = Frag<T>;
+  constexpr int kHalf = OA::kBytes * DEPTH, kStage = 2 * kHalf;
+  constexpr int ROW = B * 4 + 16;  // bytes of a row of sums
+  __shared__ __attribute__((aligned(16))) char lds[STAGES * kStage];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tn = (int)((g.N + B - 1) / B);
+  const int mt = blockIdx.x / tn;
+  const long m0 = (long)mt * B, n0 = (long)(blockIdx.x % tn) * B;
+  const long kb = (long)blockIdx.y * g.k_split;
+  const int kn = (int)min(g.K - kb, g.k_split);
+
+  using LA = Loader<T, B, ACOLS, WAVES, DEPTH>;
+  using LB = Loader<T, B, BCOLS, WAVES, DEPTH>;
+  const LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
+  const LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
+  auto fetch = [&](int t, int stage) {
+    load_a.fetch(lds + stage * kStage, t);
+    load_b.fetch(lds + stage * kStage + kHalf, t);
+  };
+  f32x4 acc[2][2] = {};
+  const int tiles = (kn + DEPTH * OA::BK - 1) / (DEPTH * OA::BK);
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) fetch(t, t);
+  // a k-tile holds two steps, a stage four: one for each wave
+  const int tile_of = wave / 2 * OA::kBytes, step = wave % 2;
+  for (int t = 0; t < tiles; ++t) {
+    wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
+    fetch(t + STAGES - 1, (t + STAGES - 1) % STAGES);
+    const char* pa = lds + t % STAGES * kStage + tile_of;
+    const char* pb = pa + kHalf;
+    typename F::Type fa[2], fb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      fa[i] = F::template read<B, ACOLS>(pa, i * 16, step, lane);
+      fb[i] = F::template read<B, BCOLS>(pb, i * 16, step, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
+  }
+  wait_pieces<0>();  // the sums go where the pieces went
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<f32x4*>(lds + (wave * B + i * 16 + (lane & 15)) * ROW +
+                                (j * 16 + (lane >> 4) * 4) * 4) = acc[i][j];
+  __syncthreads();
+  // a thread: four neighbouring n of one m
+  const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
+  const long m = m0 + row, n = n0 + col;
+  f32x4 v = {};
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w)
+    v += *reinterpret_cast<f32x4*>(lds + (w * B + row) * ROW + col * 4);
+  float o[4] = {v[0], v[1], v[2], v[3]};
+  const int left = m < g.M ? (int)max(0l, min(4l, g.N - n)) : 0;
+  if constexpr (EPI == kPartial) {
+    float* p = e.partial + ((long)blockIdx.y * g.M + m) * g.N + n;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = o[j];
+    return;
+  }
+  finish4<T, EPI>(o, m, n, left, g, e, c);
+  if (EPI == kSlope && e.partial) {
+    __syncthreads();
+    *reinterpret_cast<f32x4*>(lds + row * ROW + col * 4) =
+        f32x4{o[0], o[1], o[2], o[3]};
+    __syncthreads();
+    if (threadIdx.x < B && n0 + threadIdx.x < g.N) {
+      float s = 0.f;
+      for (int r = 0; r < B; ++r)
+        s += *reinterpret_cast<float*>(lds + r * ROW + threadIdx.x * 4);
+      e.partial[(long)mt * g.N + n0 + threadIdx.x] = s;
+    }
+  }
+}
+
+// The epilogue over sums of k split over blocks; four n a thread.
+template <typename T, int EPI>
+__global__ __launch_bounds__(256)
+void linear_finish(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
+                   int splits) {
+  const long wide = (g.N + 3) / 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const long m = i / wide, n = i % wide * 4;
+  if (m >= g.M) return;
+  const int left = (int)min(4l, g.N - n);
+  const float* p = e.partial + m * g.N + n;
+  float o[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] += j < left ? p[s * g.M * g.N + j] : 0.f;
+  finish4<T, EPI>(o, m, n, left, g, e, c);
+}
+
 // C = alpha * sum of the splits: 256 elements a block, 32 threads of eight
 // side by side, blockDim / 32 of them for every so manieth split
 template <typename T>
@@ -503,99 +666,129 @@ void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
 
 namespace {
 
-struct Tile {
-  int bm, bn, stages;
-};
-
 static int LT = getenv("LT") ? atoi(getenv("LT")) : 0;
-Tile tile_for(long M, long N, int splits) {
+static int SPL = getenv("SPL") ? atoi(getenv("SPL")) : 256;
+static int SPK = getenv("SPK") ? atoi(getenv("SPK")) : 4;
+// The side of a tile: the largest that still gives the CUs a block each.
+// Large tiles read their operands less often, small ones spread a small
+// product wider.
+int tile_for(long M, long N, int splits) {
   auto blocks = [&](int b) {
     return ((M + b - 1) / b) * ((N + b - 1) / b) * splits;
   };
-  if (LT) return {LT / 10, LT / 10, LT % 10};
-  if (blocks(256) >= 256) return {256, 256, 2};
-  if (blocks(128) >= 192) return {128, 128, 2};
-  return {64, 64, 4};
+  if (LT) return LT;
+  if (blocks(256) >= 256) return 256;
+  if (blocks(128) >= 192) return 128;
+  if (blocks(64) >= 192) return 64;
+  return 32;
 }
 
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
-void launch_tile(T* c, const T* a, const T* b, const GemmArgs& g,
+void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
                  const EpilogueArgs<T>& e, int splits, hipStream_t s) {
-  const Tile t = tile_for(g.M, g.N, splits);
-  const long tiles = ceil_div(g.M, t.bm) * (long)ceil_div(g.N, t.bn);
+  const long tiles = ceil_div(g.M, tile) * (long)ceil_div(g.N, tile);
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8), splits);
-#define LAUNCH(B, WM, WN, ST)                                                 \
-  hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, ST, ACOLS, BCOLS, EPI>),   \
+#define LAUNCH(B, WM, WN)                                                     \
+  hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, 2, ACOLS, BCOLS, EPI>),    \
                      grid, dim3(WM * WN * 64), 0, s, g, e, c, a, b)
-  if (t.bm == 256)
-    LAUNCH(256, 2, 4, 2);
-  else if (t.bm == 128 && t.stages == 2)
-    LAUNCH(128, 2, 2, 2);
-  else if (t.bm == 128)
-    LAUNCH(128, 2, 2, 4);
-  else if (t.stages == 4)
-    LAUNCH(64, 2, 2, 4);
-  else if (t.stages == 2)
-    LAUNCH(64, 2, 2, 2);
+  if (tile == 256)
+    LAUNCH(256, 2, 4);
+  else if (tile == 128)
+    LAUNCH(128, 2, 2);
+  else if (tile == 64)
+    LAUNCH(64, 2, 2);
   else
-    LAUNCH(64, 2, 2, 8);
+    hipLaunchKernelGGL((linear_small<T, ACOLS, BCOLS, EPI>),
+                       dim3((unsigned)tiles, splits), dim3(256), 0, s, g, e, c,
+                       a, b);
 #undef LAUNCH
 }
 
 }  // namespace
 
 int linear_row_tiles(long M, long N) {
-  return ceil_div(M, tile_for(M, N, 1).bm);
+  return ceil_div(M, tile_for(M, N, 1));
 }
 
-// Splits of a long k where the tiles of C alone leave CUs idle: enough for
-// about two blocks of 128x128 a CU, at least 16 k-tiles each.
-int linear_splits(long M, long N, long K, bool f32) {
-  const long tiles = (long)ceil_div(M, 128) * ceil_div(N, 128);
-  const long depth = f32 ? 512 : 1024;
-  const long want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-  const long most = (K + depth - 1) / depth;
+// Blocks that share out k. Tiles of 32: until there are 256 blocks, each
+// with at least four stages of two k-tiles. dw, whose k is the rows: enough
+// for about two blocks of 128x128 a CU, at least 16 k-tiles each.
+int linear_splits(long M, long N, long K, bool f32, bool dw) {
+  const long bk = f32 ? 32 : 64;
+  if (dw && M * N > 128 * 128) {
+    const long tiles = (long)ceil_div(M, 128) * ceil_div(N, 128);
+    const long want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+    const long most = (K + 16 * bk - 1) / (16 * bk);
+    return (int)(want < most ? want : most);
+  }
+  if (tile_for(M, N, 1) != 32) return 1;
+  const long tiles = (long)ceil_div(M, 32) * ceil_div(N, 32);
+  const long want = (SPL + tiles - 1) / tiles;
+  const long most = (K + SPK * 2 * bk - 1) / (SPK * 2 * bk);
   return (int)(want < most ? want : most);
 }
 
+namespace {
+
+// C in one launch, or by splits of k and a launch that sums them
+template <typename T, bool ACOLS, bool BCOLS, int EPI>
+void launch_split(T* c, const T* a, const T* b, GemmArgs g,
+                  EpilogueArgs<T> e, int splits, hipStream_t s) {
+  if (splits > 1) {
+    const long bk = 128 / sizeof(T);
+    g.k_split = ((g.K + splits - 1) / splits + bk - 1) / bk * bk;
+    splits = (int)((g.K + g.k_split - 1) / g.k_split);
+  }
+  const int tile = tile_for(g.M, g.N, splits);
+  if (splits == 1) {
+    launch_tile<T, ACOLS, BCOLS, EPI>(tile, c, a, b, g, e, 1, s);
+    return;
+  }
+  launch_tile<T, ACOLS, BCOLS, kPartial>(tile, c, a, b, g, e, splits, s);
+  if (EPI == kPlain) {
+    const long count = g.M * g.N;
+    int groups = 1;
+    while (groups < 32 && groups * 4 < splits) groups *= 2;
+    hipLaunchKernelGGL(sum_splits<T>, dim3(ceil_div(count, 256)),
+                       dim3(32 * groups), 0, s, c, e.partial, splits, count,
+                       g.alpha);
+  } else {
+    hipLaunchKernelGGL((linear_finish<T, EPI>),
+                       dim3(ceil_div(g.M * ((g.N + 3) / 4), 256)), dim3(256),
+                       0, s, g, e, c, splits);
+  }
+}
+
+}  // namespace
+
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
-                           const EpilogueArgs<T>& e, hipStream_t s) {
-  launch_tile<T, false, false, kForward>(y, x, w, g, e, 1, s);
+                           const EpilogueArgs<T>& e, int splits,
+                           hipStream_t s) {
+  launch_split<T, false, false, kForward>(y, x, w, g, e, splits, s);
 }
 
 template <typename T>
 void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
                          const EpilogueArgs<T>& e, hipStream_t s) {
-  launch_tile<T, false, false, kSlope>(dz, x, w, g, e, 1, s);
+  launch_tile<T, false, false, kSlope>(tile_for(g.M, g.N, 1), dz, x, w, g, e,
+                                       1, s);
 }
 
 template <typename T>
-void launch_linear_dx(T* dx, const T* dz, const T* w, const GemmArgs& g,
-                      hipStream_t s) {
-  launch_tile<T, false, true, kPlain>(dx, dz, w, g, EpilogueArgs<T>{}, 1, s);
+void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
+                      const GemmArgs& g, int splits, hipStream_t s) {
+  EpilogueArgs<T> e{};
+  e.partial = partial;
+  launch_split<T, false, true, kPlain>(dx, dz, w, g, e, splits, s);
 }
 
 template <typename T>
 void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
-                      GemmArgs g, hipStream_t s) {
-  const int splits = linear_splits(g.M, g.N, g.K, sizeof(T) == 4);
+                      const GemmArgs& g, int splits, hipStream_t s) {
   EpilogueArgs<T> e{};
-  if (splits == 1) {
-    launch_tile<T, true, true, kPlain>(dw, dz, x, g, e, 1, s);
-    return;
-  }
-  const long bk = 128 / sizeof(T);
-  g.k_split = ((g.K + splits - 1) / splits + bk - 1) / bk * bk;
-  const int used = (int)((g.K + g.k_split - 1) / g.k_split);
   e.partial = partial;
-  launch_tile<T, true, true, kPartial>(dw, dz, x, g, e, used, s);
-  const long count = g.M * g.N;
-  int groups = 1;
-  while (groups < 32 && groups * 4 < used) groups *= 2;
-  hipLaunchKernelGGL(sum_splits<T>, dim3(ceil_div(count, 256)),
-                     dim3(32 * groups), 0, s, dw, partial, used, count,
-                     g.alpha);
+  launch_split<T, true, true, kPlain>(dw, dz, x, g, e, splits, s);
 }
 
 // ---- dz from a kept z, and sums over rows ----
@@ -697,15 +890,15 @@ void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
 #define INSTANTIATE(T)                                                       \
   template void launch_linear_forward<T>(T*, const T*, const T*,             \
                                          const GemmArgs&,                    \
-                                         const EpilogueArgs<T>&,             \
+                                         const EpilogueArgs<T>&, int,        \
                                          hipStream_t);                       \
   template void launch_linear_slope<T>(T*, const T*, const T*,               \
                                        const GemmArgs&,                      \
                                        const EpilogueArgs<T>&, hipStream_t); \
-  template void launch_linear_dx<T>(T*, const T*, const T*, const GemmArgs&, \
-                                    hipStream_t);                            \
+  template void launch_linear_dx<T>(T*, float*, const T*, const T*,          \
+                                    const GemmArgs&, int, hipStream_t);      \
   template void launch_linear_dw<T>(T*, float*, const T*, const T*,          \
-                                    GemmArgs, hipStream_t);                  \
+                                    const GemmArgs&, int, hipStream_t);      \
   template void launch_pad_rows<T>(T*, const T*, long, long, int, int,       \
                                    hipStream_t);                             \
   template void launch_linear_dz<T>(T*, long, float*, const T*, long,        \

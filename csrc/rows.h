@@ -145,12 +145,18 @@ struct EpilogueArgs {
   float* z;     // forward: [M, N] or null
   const T* dy;  // slope: [M, N] with rows of dy_stride
   long dy_stride;
-  float* partial;  // slope: sums over the rows of each row of tiles, or null
+  // slope: sums over the rows of each row of tiles, or null; with k in
+  // parts: their sums
+  float* partial;
 };
+// Into how many parts the launches below share k, given C's M x N: each but
+// linear_slope takes linear_splits(...), and needs partial (e.partial) of
+// that many M * N floats if it is over 1.
+int linear_splits(long M, long N, long K, bool f32, bool dw);
 // y = clamp(act(alpha x W^T + bias) * gain) + residual
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
-                           const EpilogueArgs<T>& e, hipStream_t);
+                           const EpilogueArgs<T>& e, int splits, hipStream_t);
 // dz = dy * slope(alpha x W^T + bias); linear_row_tiles sums of rows
 int linear_row_tiles(long M, long N);
 template <typename T>
@@ -158,14 +164,12 @@ void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
                          const EpilogueArgs<T>& e, hipStream_t);
 // dx[M, N] = alpha dz[M, K] W[K, N]
 template <typename T>
-void launch_linear_dx(T* dx, const T* dz, const T* w, const GemmArgs& g,
-                      hipStream_t);
-// dw[M, N] = alpha dz[K, M]^T x[K, N]; partial: linear_splits * M * N floats,
-// unused for one split
-int linear_splits(long M, long N, long K, bool f32);
+void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
+                      const GemmArgs& g, int splits, hipStream_t);
+// dw[M, N] = alpha dz[K, M]^T x[K, N]
 template <typename T>
 void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
-                      GemmArgs g, hipStream_t);
+                      const GemmArgs& g, int splits, hipStream_t);
 template <typename T>
 void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
                      int width, hipStream_t);
