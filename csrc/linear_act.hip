@@ -210,48 +210,54 @@ struct Loader {
   using O = Operand<T, BX, COLS>;
   static constexpr int ES = sizeof(T), BK = O::BK;
   static constexpr int kTile = BX / 8;  // pieces of a k-tile
-  static constexpr int kPieces = kTile * DEPTH / WAVES;
-  static_assert(kTile * DEPTH % WAVES == 0, "whole pieces a wave");
-  const char* corner;
-  long bytes;  // from there to the operand's end, whose rows end with a
-               // whole granule
-  long step;   // bytes from one k-tile to the next
-  int kn, wave, lane;
-  int offset[kPieces];
+  static constexpr int kPieces = kTile / WAVES * DEPTH;  // a wave's of a stage
+  static_assert(kTile % WAVES == 0, "whole pieces a wave");
+  static constexpr int kEach = kTile / WAVES;  // a wave's of a k-tile
+  const char* at;  // the corner of the next k-tile
+  long bytes;      // from there to the operand's end, whose rows end with a
+                   // whole granule
+  long step;       // from one k-tile to the next
+  int left;        // k from there on
+  int wave, lane;
+  int offset[kEach];
 
   // x0: first row (column) of the tile, X: all of them; kb, kn: part of k
-  GFA_DEV Loader(const T* p, long stride, long x0, long X, long kb, int kn_,
+  GFA_DEV Loader(const T* p, long stride, long x0, long X, long kb, int kn,
                  int wave_, int lane_)
-      : kn(kn_), wave(wave_), lane(lane_) {
+      : left(kn), wave(wave_), lane(lane_) {
     auto whole16 = [](long v) { return (v * ES + 15) & ~15l; };
-    corner = reinterpret_cast<const char*>(COLS ? p + kb * stride + x0
-                                                : p + x0 * stride + kb);
+    at = reinterpret_cast<const char*>(COLS ? p + kb * stride + x0
+                                            : p + x0 * stride + kb);
     bytes = COLS ? (kn - 1) * stride * ES + whole16(X) - x0 * ES
                  : (X - x0 - 1) * stride * ES + whole16(kn);
     step = (COLS ? BK * stride : BK) * ES;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      offset[i] = O::source(piece(i) % kTile * 64 + lane, (int)stride);
+    for (int i = 0; i < kEach; ++i)
+      offset[i] = O::source((i * WAVES + wave) * 64 + lane, (int)stride);
   }
-  GFA_DEV int piece(int i) const { return i * WAVES + wave; }
 
-  // Stage t of the operand. Past the end nothing is read and zeros arrive,
+  // The next DEPTH k-tiles. Past the end nothing is read and zeros arrive,
   // so the counts of pieces under way stay what the waits expect.
-  GFA_DEV void fetch(char* lds, int t) const {
+  GFA_DEV void fetch(char* lds) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int q = t * DEPTH + piece(i) / kTile;
-      int off = offset[i];
-      if constexpr (!COLS) {
-        // rows: the last k-tile is cut off at the end of k
-        const int idx = piece(i) % kTile * 64 + lane;
-        const int k = ((idx & 7) ^ O::swizzle(idx >> 3)) * (16 / ES);
-        const int left = kn - q * BK;
-        if (left < BK && k >= left) off = 0x7ffffff8;
+    for (int d = 0; d < DEPTH; ++d) {
+      const auto rsrc = buffer_at(at, bytes);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        int off = offset[i];
+        if constexpr (!COLS) {
+          // rows: the last k-tile is cut off at the end of k
+          const int idx = (i * WAVES + wave) * 64 + lane;
+          const int k = ((idx & 7) ^ O::swizzle(idx >> 3)) * (16 / ES);
+          if (left < BK && k >= left) off = 0x7ffffff8;
+        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc, (LdsPtr)(lds + (d * kTile + i * WAVES + wave) * 1024), 16,
+            off, 0, 0, 0);
       }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          buffer_at(corner + q * step, bytes - q * step),
-          (LdsPtr)(lds + piece(i) * 1024), 16, off, 0, 0, 0);
+      at += step;
+      bytes -= step;
+      left -= BK;
     }
   }
 };
@@ -293,22 +299,22 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 
   using LA = Loader<T, BM, ACOLS, WAVES, 1>;
   using LB = Loader<T, BN, BCOLS, WAVES, 1>;
-  const LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
-  const LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
-  auto fetch = [&](int t, int stage) {
-    load_a.fetch(lds + stage * kStage, t);
-    load_b.fetch(lds + stage * kStage + OA::kBytes, t);
+  LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
+  LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
+  auto fetch = [&](int stage) {
+    load_a.fetch(lds + stage * kStage);
+    load_b.fetch(lds + stage * kStage + OA::kBytes);
   };
 
   const int wm = wave / WN * TM, wn = wave % WN * TN;
   f32x4 acc[FM][FN] = {};
   const int tiles = (kn + BK - 1) / BK;
 #pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t) fetch(t, t);
+  for (int t = 0; t < STAGES - 1; ++t) fetch(t);
   int use = 0, fill = STAGES - 1;
   for (int t = 0; t < tiles; ++t) {
     wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
-    if (STAGES > 2 || t + 1 < tiles) fetch(t + STAGES - 1, fill);
+    if (STAGES > 2 || t + 1 < tiles) fetch(fill);
     const char* la_ = lds + use * kStage;
     const char* lb_ = la_ + OA::kBytes;
     use = use + 1 == STAGES ? 0 : use + 1;
@@ -519,21 +525,21 @@ void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 
   using LA = Loader<T, B, ACOLS, WAVES, DEPTH>;
   using LB = Loader<T, B, BCOLS, WAVES, DEPTH>;
-  const LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
-  const LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
-  auto fetch = [&](int t, int stage) {
-    load_a.fetch(lds + stage * kStage, t);
-    load_b.fetch(lds + stage * kStage + kHalf, t);
+  LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
+  LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
+  auto fetch = [&](int stage) {
+    load_a.fetch(lds + stage * kStage);
+    load_b.fetch(lds + stage * kStage + kHalf);
   };
   f32x4 acc[2][2] = {};
   const int tiles = (kn + DEPTH * OA::BK - 1) / (DEPTH * OA::BK);
 #pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t) fetch(t, t);
+  for (int t = 0; t < STAGES - 1; ++t) fetch(t);
   // a k-tile holds two steps, a stage four: one for each wave
   const int tile_of = wave / 2 * OA::kBytes, step = wave % 2;
   for (int t = 0; t < tiles; ++t) {
     wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
-    fetch(t + STAGES - 1, (t + STAGES - 1) % STAGES);
+    fetch((t + STAGES - 1) % STAGES);
     const char* pa = lds + t % STAGES * kStage + tile_of;
     const char* pb = pa + kHalf;
     typename F::Type fa[2], fb[2];
