@@ -298,7 +298,7 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(const Tensor& x, const Tensor& w,
     }
     e.z = mptr<float>(z);
     const int splits = gfa::linear_splits(
-        xr.count, n, k, std::is_same_v<scalar_t, float>, false);
+        xr.count, n, k, std::is_same_v<scalar_t, float>, gfa::kRows);
     const OptTensor parts = split_sums(splits, xr.count, n, x);
     e.partial = mptr<float>(parts);
     gfa::launch_linear_forward<scalar_t>(
@@ -385,7 +385,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     if (need_dx || need_dw) dr = tile_rows<scalar_t>(dr, n);
     constexpr bool is_f32 = std::is_same_v<scalar_t, float>;
     if (need_dx) {
-      const int splits = gfa::linear_splits(m, k, n, is_f32, false);
+      const int splits = gfa::linear_splits(m, k, n, is_f32, gfa::kInputs);
       const OptTensor parts = split_sums(splits, m, k, x);
       gfa::launch_linear_dx<scalar_t>(
           mptr<scalar_t>(dx), mptr<float>(parts), cptr<scalar_t>(dr.t),
@@ -393,7 +393,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
           {m, k, n, dr.stride, wr.stride, k, scale, n}, splits, cur_stream());
     }
     if (need_dw) {
-      const int splits = gfa::linear_splits(n, k, m, is_f32, true);
+      const int splits = gfa::linear_splits(n, k, m, is_f32, gfa::kWeights);
       const OptTensor parts = split_sums(splits, n, k, x);
       gfa::launch_linear_dw<scalar_t>(
           mptr<scalar_t>(dw), mptr<float>(parts), cptr<scalar_t>(dr.t),

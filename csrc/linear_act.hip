@@ -55,6 +55,13 @@ struct Operand {
 
 // fragments of 16 (m or n) x 128 bits of k: what one lane gives to the
 // matrix cores for a step of kStep
+template <typename T> struct Unaligned;
+template <> struct Unaligned<float> {
+  typedef float Vec __attribute__((ext_vector_type(4), aligned(4)));
+};
+template <> struct Unaligned<bf16> {
+  typedef short Vec __attribute__((ext_vector_type(8), aligned(2)));
+};
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
   static constexpr int kStep = 32;
@@ -348,6 +355,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const long n = n0 + wn + (lane % LPR) * 8;
   const int left = (int)max(0l, min(8l, g.N - n));
   const bool whole = n0 + wn + TN <= g.N;
+  const bool curved = e.act.act != kLinear || e.act.clamp < INFINITY;
   float bias[8] = {};
   if (EPI != kPlain && EPI != kPartial && e.bias && left) {
     if (e.bias_f32)
@@ -384,7 +392,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
             acc[h * 2 + i][j];
     __builtin_amdgcn_wave_barrier();
     char* at = mine + lane / LPR * EROW + (lane % LPR) * 32;
-    if (EPI == kForward || EPI == kSlope) {
+    if ((EPI == kForward && curved) || EPI == kSlope) {
 #pragma unroll 1
       for (int q = 0; q < ITER; ++q) {
         f32x4* p = reinterpret_cast<f32x4*>(at + q * RPI * EROW);
@@ -412,6 +420,8 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       for (int j = 0; j < 8; ++j) {
         o[j] = v[j / 4][j % 4];
         if (EPI == kPlain) o[j] *= g.alpha;
+        if (EPI == kForward && !curved)
+          o[j] = e.act.gain * (g.alpha * o[j] + bias[j]);
       }
       const long m = mh + q * RPI;
       if (m >= g.M) continue;
@@ -457,47 +467,210 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   }
 }
 
-// The epilogue of four sums of row m from column n on, the first `left` of
-// them within the matrix; they become what was written, 0 outside.
+// The epilogue of four neighbouring sums of row m, from column n on. What it
+// reads besides can be asked for before the sums are there.
 template <typename T, int EPI>
-GFA_DEV void finish4(float (&o)[4], long m, long n, int left,
-                     const GemmArgs& g, const EpilogueArgs<T>& e, T* c) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) o[j] *= g.alpha;
-  if constexpr (EPI == kForward || EPI == kSlope) {
-    if (e.bias) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left)
-          o[j] += e.bias_gain *
-                  (e.bias_f32 ? static_cast<const float*>(e.bias)[n + j]
-                              : to_f32(static_cast<const T*>(e.bias)[n + j]));
-    }
-    if (EPI == kForward && e.z)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < left) e.z[m * g.N + n + j] = o[j];
-    if (EPI == kForward)
-      act_values(o, e.act);
-    else
-      act_slopes(o, e.act);
-    const T* p = EPI == kForward ? e.residual : e.dy;
-    if (p) {
-      p += m * (EPI == kForward ? e.res_stride : e.dy_stride) + n;
+struct Finish4 {
+  long m, n;
+  int left;  // how many of the four lie within the matrix
+  float bias[4];
+  typename Raw<T>::type other[4];
+
+  GFA_DEV Finish4(long m_, long n_, const GemmArgs& g,
+                  const EpilogueArgs<T>& e)
+      : m(m_), n(n_), left(m_ < g.M ? (int)max(0l, min(4l, g.N - n_)) : 0) {
+    if constexpr (EPI == kForward || EPI == kSlope) {
+      const T* p = EPI == kForward ? e.residual : e.dy;
+      if (p) p += m * (EPI == kForward ? e.res_stride : e.dy_stride) + n;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float r = j < left ? to_f32(p[j]) : 0.f;
-        o[j] = EPI == kForward ? o[j] + r : o[j] * r;
+        bias[j] = 0.f;
+        other[j] = 0;
+        if (j < left) {
+          if (e.bias)
+            bias[j] = e.bias_gain *
+                      (e.bias_f32
+                           ? static_cast<const float*>(e.bias)[n + j]
+                           : to_f32(static_cast<const T*>(e.bias)[n + j]));
+          if (p) other[j] = reinterpret_cast<const typename Raw<T>::type*>(p)[j];
+        }
       }
     }
   }
-  // dz has rows padded to eight, zero behind the last element
-  const long end = EPI == kSlope && left > 0 ? g.ldc - n : left;
+
+  // the sums become what was written, 0 outside the matrix
+  GFA_DEV void write(float (&o)[4], const GemmArgs& g,
+                     const EpilogueArgs<T>& e, T* c) const {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (j >= left) o[j] = 0.f;
-    if (j < end) put(c + m * g.ldc + n + j, o[j]);
+    for (int j = 0; j < 4; ++j) o[j] *= g.alpha;
+    if constexpr (EPI == kForward || EPI == kSlope) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += bias[j];
+      if (EPI == kForward && e.z)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < left) e.z[m * g.N + n + j] = o[j];
+      if (EPI == kForward)
+        act_values(o, e.act);
+      else
+        act_slopes(o, e.act);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float r = raw_to_f32(other[j]);
+        o[j] = EPI == kForward ? o[j] + r : o[j] * r;
+      }
+    }
+    // dz has rows padded to eight, zero behind the last element
+    const long end = EPI == kSlope && left > 0 ? g.ldc - n : left;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j >= left) o[j] = 0.f;
+      if (j < end) put(c + m * g.ldc + n + j, o[j]);
+    }
   }
+};
+
+// The sums of a block's four waves over 16 FM x 16 FN of C meet in LDS and
+// go through the epilogue, four neighbouring n of one m a thread.
+template <typename T, int EPI, int FM, int FN>
+GFA_DEV void join_waves(const f32x4 (&acc)[FM][FN], char* lds, long n0, int mt,
+                        const Finish4<T, EPI>& finish, const GemmArgs& g,
+                        const EpilogueArgs<T>& e, T* c) {
+  constexpr int BM = 16 * FM, BN = 16 * FN, WAVES = 4;
+  constexpr int ROW = BN * 4 + 16;  // bytes
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      *reinterpret_cast<f32x4*>(lds + (wave * BM + i * 16 + (lane & 15)) * ROW +
+                                (j * 16 + (lane >> 4) * 4) * 4) = acc[i][j];
+  __syncthreads();
+  const int row = threadIdx.x / (BN / 4), col = threadIdx.x % (BN / 4) * 4;
+  float o[4] = {};
+  if (row < BM) {
+    f32x4 v = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      v += *reinterpret_cast<f32x4*>(lds + (w * BM + row) * ROW + col * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = v[j];
+    if constexpr (EPI == kPartial) {
+      float* p =
+          e.partial + ((long)blockIdx.y * g.M + finish.m) * g.N + finish.n;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < finish.left) p[j] = o[j];
+    } else {
+      finish.write(o, g, e, c);
+    }
+  }
+  if (EPI == kSlope && e.partial) {
+    __syncthreads();
+    if (row < BM)
+      *reinterpret_cast<f32x4*>(lds + row * ROW + col * 4) =
+          f32x4{o[0], o[1], o[2], o[3]};
+    __syncthreads();
+    if (threadIdx.x < BN && n0 + threadIdx.x < g.N) {
+      float s = 0.f;
+      for (int r = 0; r < BM; ++r)
+        s += *reinterpret_cast<float*>(lds + r * ROW + threadIdx.x * 4);
+      e.partial[(long)mt * g.N + n0 + threadIdx.x] = s;
+    }
+  }
+}
+
+// the part of C that join_waves gives a thread
+template <typename T, int EPI, int FM, int FN>
+GFA_DEV Finish4<T, EPI> thread_part(long m0, long n0, const GemmArgs& g,
+                                    const EpilogueArgs<T>& e) {
+  const int row = threadIdx.x / (FN * 4);
+  return {row < FM * 16 ? m0 + row : g.M, n0 + threadIdx.x % (FN * 4) * 4, g,
+          e};
+}
+
+// eight bf16 or four floats of a row at any alignment, as a fragment
+template <typename T>
+GFA_DEV typename Frag<T>::Type load16(const T* p) {
+  return *reinterpret_cast<const typename Unaligned<T>::Vec*>(p);
+}
+template <typename T>
+GFA_DEV typename Frag<T>::Type load16(const T* p, int left) {
+  typename Frag<T>::Type v{};
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(T); ++j)
+    if (j < left) v[j] = reinterpret_cast<const typename Raw<T>::type*>(p)[j];
+  return v;
+}
+
+// Products with at most 32 rows (rows times rows only): 16 FM x 16 of C a
+// block, so that the weights, each read once, come in over as many CUs as
+// there are; k is shared out over the block's four waves in chunks of 256
+// bytes. Fragments come straight from memory, two chunks a wave under way,
+// with no barrier before the waves meet; a row needs no alignment.
+template <typename T, int FM, int EPI>
+__global__ __launch_bounds__(256)
+void linear_direct(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
+                   const T* __restrict__ a, const T* __restrict__ b) {
+  constexpr int FN = 1, WAVES = 4, U = 4;
+  using F = Frag<T>;
+  constexpr int STEP = F::kStep, V = 16 / sizeof(T);
+  __shared__
+      __attribute__((aligned(16))) char lds[WAVES * FM * 16 * (64 + 16)];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long n0 = (long)blockIdx.x * 16;
+  const long kb = (long)blockIdx.y * g.k_split;
+  const int kn = (int)min(g.K - kb, g.k_split);
+  const auto finish = thread_part<T, EPI, FM, FN>(0, n0, g, e);
+
+  // rows past the last repeat it; their sums are not stored
+  const int lane_k = (lane >> 4) * V;
+  const T* pa[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+    pa[i] = a + min((long)(i * 16 + (lane & 15)), g.M - 1) * g.lda + kb + lane_k;
+  const T* pb = b + min(n0 + (lane & 15), g.N - 1) * g.ldb + kb + lane_k;
+  f32x4 acc[FM][FN] = {};
+  struct Chunk {
+    typename F::Type a[U][FM], b[U];
+  };
+  auto load = [&](Chunk& q, int chunk) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (chunk * U + u) * STEP;
+      q.b[u] = load16<T>(pb + k);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) q.a[u][i] = load16<T>(pa[i] + k);
+    }
+  };
+  auto mma = [&](const Chunk& q) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+        acc[i][0] = F::mma(q.b[u], q.a[u][i], acc[i][0]);
+  };
+  const int chunks = kn / (U * STEP);
+  Chunk q0, q1;
+  if (wave < chunks) load(q0, wave);
+  for (int q = wave; q < chunks; q += 2 * WAVES) {
+    const bool more = q + WAVES < chunks;
+    if (more) load(q1, q + WAVES);
+    mma(q0);
+    if (!more) break;
+    if (q + 2 * WAVES < chunks) load(q0, q + 2 * WAVES);
+    mma(q1);
+  }
+  // what is left of k, a step a wave, the last one cut off
+  for (int k = (chunks * U + wave) * STEP; k < kn; k += WAVES * STEP) {
+    const int left = kn - k - lane_k;
+    const auto fb = load16<T>(pb + k, left);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+      acc[i][0] = F::mma(fb, load16<T>(pa[i] + k, left), acc[i][0]);
+  }
+  join_waves<T, EPI, FM, FN>(acc, lds, n0, 0, finish, g, e, c);
 }
 
 // Products that tiles of 64x64 spread over too few CUs: 32x32 of C a block.
@@ -509,11 +682,10 @@ template <typename T, bool ACOLS, bool BCOLS, int EPI>
 __global__ __launch_bounds__(256)
 void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
                   const T* __restrict__ a, const T* __restrict__ b) {
-  constexpr int B = 32, DEPTH = 2, STAGES = 4, WAVES = 4;
+  constexpr int B = 32, DEPTH = 2, STAGES = 4, WAVES = 4, FM = 2, FN = 2;
   using OA = Operand<T, B, ACOLS>;
   using F = Frag<T>;
   constexpr int kHalf = OA::kBytes * DEPTH, kStage = 2 * kHalf;
-  constexpr int ROW = B * 4 + 16;  // bytes of a row of sums
   __shared__ __attribute__((aligned(16))) char lds[STAGES * kStage];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -522,6 +694,7 @@ void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const long m0 = (long)mt * B, n0 = (long)(blockIdx.x % tn) * B;
   const long kb = (long)blockIdx.y * g.k_split;
   const int kn = (int)min(g.K - kb, g.k_split);
+  const auto finish = thread_part<T, EPI, FM, FN>(m0, n0, g, e);
 
   using LA = Loader<T, B, ACOLS, WAVES, DEPTH>;
   using LB = Loader<T, B, BCOLS, WAVES, DEPTH>;
@@ -554,42 +727,7 @@ void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       for (int j = 0; j < 2; ++j) acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
   }
   wait_pieces<0>();  // the sums go where the pieces went
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      *reinterpret_cast<f32x4*>(lds + (wave * B + i * 16 + (lane & 15)) * ROW +
-                                (j * 16 + (lane >> 4) * 4) * 4) = acc[i][j];
-  __syncthreads();
-  // a thread: four neighbouring n of one m
-  const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
-  const long m = m0 + row, n = n0 + col;
-  f32x4 v = {};
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w)
-    v += *reinterpret_cast<f32x4*>(lds + (w * B + row) * ROW + col * 4);
-  float o[4] = {v[0], v[1], v[2], v[3]};
-  const int left = m < g.M ? (int)max(0l, min(4l, g.N - n)) : 0;
-  if constexpr (EPI == kPartial) {
-    float* p = e.partial + ((long)blockIdx.y * g.M + m) * g.N + n;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < left) p[j] = o[j];
-    return;
-  }
-  finish4<T, EPI>(o, m, n, left, g, e, c);
-  if (EPI == kSlope && e.partial) {
-    __syncthreads();
-    *reinterpret_cast<f32x4*>(lds + row * ROW + col * 4) =
-        f32x4{o[0], o[1], o[2], o[3]};
-    __syncthreads();
-    if (threadIdx.x < B && n0 + threadIdx.x < g.N) {
-      float s = 0.f;
-      for (int r = 0; r < B; ++r)
-        s += *reinterpret_cast<float*>(lds + r * ROW + threadIdx.x * 4);
-      e.partial[(long)mt * g.N + n0 + threadIdx.x] = s;
-    }
-  }
+  join_waves<T, EPI, FM, FN>(acc, lds, n0, mt, finish, g, e, c);
 }
 
 // The epilogue over sums of k split over blocks; four n a thread.
@@ -601,15 +739,15 @@ void linear_finish(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const long m = i / wide, n = i % wide * 4;
   if (m >= g.M) return;
-  const int left = (int)min(4l, g.N - n);
+  const Finish4<T, EPI> finish(m, n, g, e);
   const float* p = e.partial + m * g.N + n;
   float o[4] = {};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < splits; ++s)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      o[j] += j < left ? p[s * g.M * g.N + j] : 0.f;
-  finish4<T, EPI>(o, m, n, left, g, e, c);
+      o[j] += j < finish.left ? p[s * g.M * g.N + j] : 0.f;
+  finish.write(o, g, e, c);
 }
 
 // C = alpha * sum of the splits: 256 elements a block, 32 threads of eight
@@ -673,8 +811,6 @@ void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
 namespace {
 
 static int LT = getenv("LT") ? atoi(getenv("LT")) : 0;
-static int SPL = getenv("SPL") ? atoi(getenv("SPL")) : 256;
-static int SPK = getenv("SPK") ? atoi(getenv("SPK")) : 4;
 // The side of a tile: the largest that still gives the CUs a block each.
 // Large tiles read their operands less often, small ones spread a small
 // product wider.
@@ -692,6 +828,18 @@ int tile_for(long M, long N, int splits) {
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
 void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
                  const EpilogueArgs<T>& e, int splits, hipStream_t s) {
+  if constexpr (!ACOLS && !BCOLS) {
+    if (g.M <= 32) {
+      const dim3 grid((unsigned)ceil_div(g.N, 16), splits);
+      if (g.M <= 16)
+        hipLaunchKernelGGL((linear_direct<T, 1, EPI>), grid, dim3(256), 0, s,
+                           g, e, c, a, b);
+      else
+        hipLaunchKernelGGL((linear_direct<T, 2, EPI>), grid, dim3(256), 0, s,
+                           g, e, c, a, b);
+      return;
+    }
+  }
   const long tiles = ceil_div(g.M, tile) * (long)ceil_div(g.N, tile);
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8), splits);
 #define LAUNCH(B, WM, WN)                                                     \
@@ -716,21 +864,30 @@ int linear_row_tiles(long M, long N) {
   return ceil_div(M, tile_for(M, N, 1));
 }
 
-// Blocks that share out k. Tiles of 32: until there are 256 blocks, each
-// with at least four stages of two k-tiles. dw, whose k is the rows: enough
-// for about two blocks of 128x128 a CU, at least 16 k-tiles each.
-int linear_splits(long M, long N, long K, bool f32, bool dw) {
+// Blocks that share out k. dw, whose k is the rows: enough for about two
+// blocks of 128x128 a CU, at least 16 k-tiles each. The others: until there
+// are 256 blocks, with at least 32 k-tiles each, as the launch that sums
+// them takes about as long as those (17x512x512 float: 5.5 us in one part,
+// 7.0 us in two; 32x8192x512: 45 us in one, 13 us in eight).
+int linear_splits(long M, long N, long K, bool f32, LinearKind kind) {
   const long bk = f32 ? 32 : 64;
-  if (dw && M * N > 128 * 128) {
+  long want, depth;
+  if (kind == kWeights) {
     const long tiles = (long)ceil_div(M, 128) * ceil_div(N, 128);
-    const long want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-    const long most = (K + 16 * bk - 1) / (16 * bk);
-    return (int)(want < most ? want : most);
+    want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+    depth = 16 * bk;
+  } else {
+    long blocks;
+    if (kind == kRows && M <= 32)
+      blocks = ceil_div(N, 16);
+    else if (tile_for(M, N, 1) == 32)
+      blocks = (long)ceil_div(M, 32) * ceil_div(N, 32);
+    else
+      return 1;
+    want = (256 + blocks - 1) / blocks;
+    depth = 32 * bk;
   }
-  if (tile_for(M, N, 1) != 32) return 1;
-  const long tiles = (long)ceil_div(M, 32) * ceil_div(N, 32);
-  const long want = (SPL + tiles - 1) / tiles;
-  const long most = (K + SPK * 2 * bk - 1) / (SPK * 2 * bk);
+  const long most = (K + depth - 1) / depth;
   return (int)(want < most ? want : most);
 }
 

@@ -24,7 +24,54 @@ struct ActParams {
   float alpha, gain, clamp;  // clamp: infinity for none
 };
 
-// f(v[j]) for eight values behind one switch over the activation.
+// ---- activations ----
+// On the hardware's exponential and reciprocal (one unit in the last place
+// each): the library's erf and tanh are several times as many instructions,
+// and a product of few multiplications an element is bounded by them.
+GFA_DEV float fast_exp(float x) {
+  return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+GFA_DEV float sigmoid(float z) {
+  return __builtin_amdgcn_rcpf(1.f + fast_exp(-z));
+}
+
+// Phi(z), the normal distribution's integral, and exp(-z^2 / 2). The upper
+// tail Q(u) = exp(-u^2 / 2) P(1 / (1 + 0.27 u)) with a polynomial P fitted
+// to it for u in 0..14 (largest relative error 2.4e-8): no difference of
+// nearly equal numbers on the negative side.
+GFA_DEV float normal_cdf(float z, float& bell) {
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.27f * fabsf(z));
+  bell = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  float p = 0.028915234201599187f;
+  p = p * t - 0.12625508802828958f;
+  p = p * t + 0.169291076679552f;
+  p = p * t - 0.06862064123099605f;
+  p = p * t + 0.10739922529842338f;
+  p = p * t + 0.07224036705627161f;
+  p = p * t + 0.10175914852646588f;
+  p = p * t + 0.10755050830418758f;
+  p = p * t + 0.1077201809422401f;
+  p *= t * bell;
+  return z < 0.f ? p : 1.f - p;
+}
+
+// tanh(z), and 1 - tanh(z)^2 = 4 r (1 - r) with r = 1 / (1 + exp(2 |z|)).
+// Below 0.6 by a polynomial in z^2 (relative error 2.5e-9), where 1 - 2 r
+// would lose digits.
+GFA_DEV float tanh_of(float z, float& slope) {
+  const float r = __builtin_amdgcn_rcpf(1.f + fast_exp(2.f * fabsf(z)));
+  slope = 4.f * r * (1.f - r);
+  const float s = z * z;
+  float p = -0.005852152574643519f;
+  p = p * s + 0.020753615804063843f;
+  p = p * s - 0.053768701016077794f;
+  p = p * s + 0.13331688918204498f;
+  p = p * s - 0.3333328325571884f;
+  p = p * s + 0.9999999975108838f;
+  return s < 0.36f ? z * p : copysignf(1.f - 2.f * r, z);
+}
+
+// f(v[j]) for all values behind one switch over the activation.
 // Comparisons are written so that a NaN takes the branch that keeps it.
 template <int N>
 GFA_DEV void act_values(float (&z)[N], const ActParams& p) {
@@ -32,22 +79,24 @@ GFA_DEV void act_values(float (&z)[N], const ActParams& p) {
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = f(z[j]);
   };
+  float unused;
   switch (p.act) {
     case kRelu: each([](float z) { return z <= 0.f ? 0.f : z; }); break;
     case kLrelu:
       each([&](float z) { return z <= 0.f ? p.alpha * z : z; });
       break;
-    case kTanh: each([](float z) { return tanhf(z); }); break;
-    case kSigmoid: each([](float z) { return 1.f / (1.f + expf(-z)); }); break;
+    case kTanh: each([&](float z) { return tanh_of(z, unused); }); break;
+    case kSigmoid: each([](float z) { return sigmoid(z); }); break;
     case kGelu:
-      each([](float z) { return 0.5f * z * (1.f + erff(z * 0.70710678f)); });
+      each([&](float z) { return z * normal_cdf(z, unused); });
       break;
-    case kSilu: each([](float z) { return z / (1.f + expf(-z)); }); break;
+    case kSilu: each([](float z) { return z * sigmoid(z); }); break;
   }
-  each([&](float a) {
-    a *= p.gain;
-    return a > p.clamp ? p.clamp : a < -p.clamp ? -p.clamp : a;
-  });
+  if (p.gain != 1.f) each([&](float a) { return a * p.gain; });
+  if (p.clamp < INFINITY)
+    each([&](float a) {
+      return a > p.clamp ? p.clamp : a < -p.clamp ? -p.clamp : a;
+    });
 }
 
 // d y / d z at z, zero where the clamp holds
@@ -55,11 +104,20 @@ template <int N>
 GFA_DEV void act_slopes(float (&z)[N], const ActParams& p) {
   // f: activation and slope
   auto each = [&](auto f) {
+    if (p.clamp < INFINITY) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      float a, s;
-      f(z[j], a, s);
-      z[j] = fabsf(a * p.gain) >= p.clamp ? 0.f : s * p.gain;
+      for (int j = 0; j < N; ++j) {
+        float a, s;
+        f(z[j], a, s);
+        z[j] = fabsf(a * p.gain) >= p.clamp ? 0.f : s * p.gain;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float a, s;
+        f(z[j], a, s);
+        z[j] = s * p.gain;
+      }
     }
   };
   switch (p.act) {
@@ -77,24 +135,23 @@ GFA_DEV void act_slopes(float (&z)[N], const ActParams& p) {
       });
       break;
     case kTanh:
-      each([](float z, float& a, float& s) {
-        a = tanhf(z), s = 1.f - a * a;
-      });
+      each([](float z, float& a, float& s) { a = tanh_of(z, s); });
       break;
     case kSigmoid:
       each([](float z, float& a, float& s) {
-        a = 1.f / (1.f + expf(-z)), s = a * (1.f - a);
+        a = sigmoid(z), s = a * (1.f - a);
       });
       break;
     case kGelu:
       each([](float z, float& a, float& s) {
-        const float cdf = 0.5f * (1.f + erff(z * 0.70710678f));
-        a = z * cdf, s = cdf + z * 0.39894228f * expf(-0.5f * z * z);
+        float bell;
+        const float cdf = normal_cdf(z, bell);
+        a = z * cdf, s = cdf + z * 0.39894228f * bell;
       });
       break;
     case kSilu:
       each([](float z, float& a, float& s) {
-        const float g = 1.f / (1.f + expf(-z));
+        const float g = sigmoid(z);
         a = z * g, s = g * (1.f + z * (1.f - g));
       });
       break;
@@ -152,7 +209,8 @@ struct EpilogueArgs {
 // Into how many parts the launches below share k, given C's M x N: each but
 // linear_slope takes linear_splits(...), and needs partial (e.partial) of
 // that many M * N floats if it is over 1.
-int linear_splits(long M, long N, long K, bool f32, bool dw);
+enum LinearKind { kRows, kInputs, kWeights };  // forward, dx, dw
+int linear_splits(long M, long N, long K, bool f32, LinearKind kind);
 // y = clamp(act(alpha x W^T + bias) * gain) + residual
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
