@@ -289,19 +289,21 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  // Tiles: an XCD's blocks (every eighth) take neighbouring tiles, in
-  // groups of 4 rows of tiles, so that they share operands in its L2.
+  // Work: an XCD's blocks (every eighth) take neighbouring tiles of one part
+  // of k, in groups of 4 rows of tiles, so that they share operands in its
+  // L2 (all tiles of a part, where there are few).
   const int tm = (int)((g.M + BM - 1) / BM), tn = (int)((g.N + BN - 1) / BN);
-  const int total = tm * tn, per = (total + 7) / 8;
-  const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || tile >= total) return;
+  const int parts = (int)((g.K + g.k_split - 1) / g.k_split);
+  const int total = tm * tn * parts, per = (total + 7) / 8;
+  const int work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || work >= total) return;
+  const int part = work / (tm * tn), tile = work - part * tm * tn;
   const int group = tile / (4 * tn), in_group = tile - group * 4 * tn;
   const int rows = min(4, tm - group * 4);
   const int mt = group * 4 + in_group % rows;
   const long m0 = (long)mt * BM;
   const long n0 = (long)(in_group / rows) * BN;
-  // the block's part of k
-  const long kb = (long)blockIdx.y * g.k_split;
+  const long kb = part * g.k_split;
   const int kn = (int)min(g.K - kb, g.k_split);
 
   using LA = Loader<T, BM, ACOLS, WAVES, 1>;
@@ -440,7 +442,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       if constexpr (EPI == kSlope) {
         if (left) store8(c + m * g.ldc + n, o, 8);
       } else if constexpr (EPI == kPartial)
-        store8(e.partial + ((long)blockIdx.y * g.M + m) * g.N + n, o, left);
+        store8(e.partial + (part * g.M + m) * g.N + n, o, left);
       else
         store8(c + m * g.ldc + n, o, left);
     }
@@ -810,18 +812,19 @@ void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
 
 namespace {
 
-static int LT = getenv("LT") ? atoi(getenv("LT")) : 0;
-// The side of a tile: the largest that still gives the CUs a block each.
-// Large tiles read their operands less often, small ones spread a small
-// product wider.
+// The side of a tile: the largest that still gives the CUs a block each and
+// is not mostly padding. Large tiles read their operands less often
+// (8192x4096x4096 bf16: 266 us with 256, 314 with 128, 439 with 64), small
+// ones spread a small product wider (524288x128x128: 120 us with 256, 65 with
+// 128).
 int tile_for(long M, long N, int splits) {
   auto blocks = [&](int b) {
     return ((M + b - 1) / b) * ((N + b - 1) / b) * splits;
   };
-  if (LT) return LT;
-  if (blocks(256) >= 256) return 256;
-  if (blocks(128) >= 192) return 128;
-  if (blocks(64) >= 192) return 64;
+  const long side = M < N ? M : N;
+  if (side > 128 && blocks(256) >= 256) return 256;
+  if (side > 64 && blocks(128) >= 192) return 128;
+  if (side > 32 && blocks(64) >= 192) return 64;
   return 32;
 }
 
@@ -841,7 +844,7 @@ void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
     }
   }
   const long tiles = ceil_div(g.M, tile) * (long)ceil_div(g.N, tile);
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), splits);
+  const dim3 grid((unsigned)((tiles * splits + 7) / 8 * 8));
 #define LAUNCH(B, WM, WN)                                                     \
   hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, 2, ACOLS, BCOLS, EPI>),    \
                      grid, dim3(WM * WN * 64), 0, s, g, e, c, a, b)
@@ -873,7 +876,9 @@ int linear_splits(long M, long N, long K, bool f32, LinearKind kind) {
   const long bk = f32 ? 32 : 64;
   long want, depth;
   if (kind == kWeights) {
-    const long tiles = (long)ceil_div(M, 128) * ceil_div(N, 128);
+    const long side = M < N ? M : N;
+    const int t = side > 64 ? 128 : side > 32 ? 64 : 32;
+    const long tiles = (long)ceil_div(M, t) * ceil_div(N, t);
     want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
     depth = 16 * bk;
   } else {
