@@ -1,6 +1,8 @@
 // Torch bindings of the row operators: layer_norm and linear_act.
 #include <torch/extension.h>
 
+#include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -54,15 +56,37 @@ void check_param(const OptTensor& p, const Tensor& x, int64_t n,
             " or float32, got ", p->scalar_type());
 }
 
+// torch::empty without the way through the dispatcher, which costs more than
+// the allocation
+Tensor new_tensor(torch::IntArrayRef shape, torch::ScalarType dtype,
+                  const Tensor& like) {
+  return Tensor(at::detail::empty_cuda(shape, dtype, like.device(),
+                                       std::nullopt));
+}
+
+// Room for a launch's intermediate values, on the current stream as tensors
+// are: given back to the allocator at the end of its scope, reused only by
+// what comes later on that stream.
+struct Room {
+  c10::DataPtr data;
+  template <typename T>
+  T* get(int64_t count) {
+    if (count == 0) return nullptr;
+    data = c10::hip::HIPCachingAllocator::get()->allocate(count * sizeof(T));
+    return static_cast<T*>(data.get());
+  }
+};
+
 // A tensor [..., n] as rows of n contiguous elements at one stride
 struct Rows {
   Tensor t;  // what is read: the tensor itself or a contiguous copy
   int64_t count, stride;
+  const void* at;
 };
 
 Rows rows_of(const Tensor& t) {
   const int64_t n = t.size(-1);
-  Rows r{t, 1, n};
+  Rows r{t, 1, n, t.data_ptr()};
   bool ok = t.stride(-1) == 1 || n == 1;
   bool first = true;
   for (int64_t d = t.dim() - 2; d >= 0; --d) {
@@ -80,8 +104,14 @@ Rows rows_of(const Tensor& t) {
   if (!ok) {
     r.t = t.contiguous();
     r.stride = n;
+    r.at = r.t.data_ptr();
   }
   return r;
+}
+
+template <typename T>
+const T* rptr(const Rows& r) {
+  return static_cast<const T*>(r.at);
 }
 
 template <typename T>
@@ -144,17 +174,17 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_fwd(
   const OptTensor wc = w ? OptTensor(w->contiguous()) : w;
   const OptTensor bc = b ? OptTensor(b->contiguous()) : b;
   const Rows xr = rows_of(x);
-  Tensor y = torch::empty(x.sizes(), x.options());
+  Tensor y = new_tensor(x.sizes(), x.scalar_type(), x);
   OptTensor mean, rstd;
   if (save) {
-    mean = torch::empty({xr.count}, x.options().dtype(torch::kFloat32));
-    rstd = torch::empty({xr.count}, x.options().dtype(torch::kFloat32));
+    mean = new_tensor({xr.count}, torch::kFloat32, x);
+    rstd = new_tensor({xr.count}, torch::kFloat32, x);
   }
   if (xr.count > 0) {
     DISPATCH_TP(x, p32, {
       gfa::launch_layer_norm_fwd<T, P>(
           static_cast<T*>(y.data_ptr()), mptr<float>(mean), mptr<float>(rstd),
-          cptr<T>(xr.t), xr.stride, cptr<P>(wc), cptr<P>(bc), xr.count, n,
+          rptr<T>(xr), xr.stride, cptr<P>(wc), cptr<P>(bc), xr.count, n,
           (float)eps, cur_stream());
     });
     HIP_CHECK_LAST();
@@ -174,27 +204,24 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
   c10::hip::HIPGuard guard(x.get_device());
   const OptTensor wc = w ? OptTensor(w->contiguous()) : w;
   const Rows xr = rows_of(x), dr = rows_of(dy);
-  const auto f32 = x.options().dtype(torch::kFloat32);
-  const auto popt = p32 ? f32 : x.options();
-  OptTensor dx, dw, db, partial;
-  if (need_dx) dx = torch::empty(x.sizes(), x.options());
+  const auto ptype = p32 ? torch::kFloat32 : x.scalar_type();
+  OptTensor dx, dw, db;
+  Room partial;
+  if (need_dx) dx = new_tensor(x.sizes(), x.scalar_type(), x);
+  if (need_dw) dw = new_tensor({n}, ptype, x);
+  if (need_db) db = new_tensor({n}, ptype, x);
   if (xr.count == 0) {
-    if (need_dw) dw = torch::zeros({n}, popt);
-    if (need_db) db = torch::zeros({n}, popt);
+    if (need_dw) dw->zero_();
+    if (need_db) db->zero_();
     return {dx, dw, db};
   }
-  if (need_dw) dw = torch::empty({n}, popt);
-  if (need_db) db = torch::empty({n}, popt);
-  if (need_dw || need_db)
-    partial = torch::empty({2, gfa::layer_norm_bwd_groups(
-                                   xr.count, n,
-                                   x.scalar_type() == torch::kFloat32),
-                            n},
-                           f32);
+  const int64_t groups = gfa::layer_norm_bwd_groups(
+      xr.count, n, x.scalar_type() == torch::kFloat32);
+  float* sums = partial.get<float>(need_dw || need_db ? 2 * groups * n : 0);
   DISPATCH_TP(x, p32, {
     gfa::launch_layer_norm_bwd<T, P>(
-        mptr<T>(dx), mptr<P>(dw), mptr<P>(db), mptr<float>(partial),
-        cptr<T>(dr.t), dr.stride, cptr<T>(xr.t), xr.stride, cptr<P>(wc),
+        mptr<T>(dx), mptr<P>(dw), mptr<P>(db), sums,
+        rptr<T>(dr), dr.stride, rptr<T>(xr), xr.stride, cptr<P>(wc),
         cptr<float>(mean), cptr<float>(rstd), xr.count, n, cur_stream());
   });
   HIP_CHECK_LAST();
@@ -241,24 +268,33 @@ std::vector<int64_t> out_shape(const Tensor& x, int64_t n) {
 }
 
 // The tiles read rows of 16-byte granules: rows elsewhere, or of another
-// width, are copied to padded ones (zeros behind the last element).
+// width, are copied to padded ones (zeros behind the last element). up to two
+// tensors in one launch.
 template <typename T>
-Rows tile_rows(const Rows& r, int64_t n) {
-  const int64_t v = 16 / sizeof(T);
-  const int64_t width = (n + 7) / 8 * 8;
-  if (n % v == 0 && r.stride % v == 0 && r.stride < (1 << 20) &&
-      reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0)
-    return r;
-  Rows p{torch::empty({r.count, width}, r.t.options()), r.count, width};
-  gfa::launch_pad_rows<T>(static_cast<T*>(p.t.data_ptr()), cptr<T>(r.t),
-                          r.stride, r.count, (int)n, (int)width, cur_stream());
-  return p;
-}
+struct TileRows {
+  Room room;
+  gfa::PadArgs<T> pad{};
 
-// room for the sums of k in parts
-OptTensor split_sums(int splits, int64_t m, int64_t n, const Tensor& like) {
-  if (splits <= 1) return {};
-  return torch::empty({splits, m, n}, like.options().dtype(torch::kFloat32));
+  void add(Rows& r, int64_t n) {
+    const int64_t v = 16 / sizeof(T);
+    if (n % v == 0 && r.stride % v == 0 && r.stride < (1 << 20) &&
+        reinterpret_cast<uintptr_t>(r.at) % 16 == 0)
+      return;
+    const int64_t width = (n + 7) / 8 * 8;
+    T* dst = room.get<T>(r.count * width);
+    pad = {dst, static_cast<const T*>(r.at), r.stride, r.count, (int)n,
+           (int)width};
+    r.stride = width;
+    r.at = dst;
+  }
+};
+
+template <typename T>
+void pad(const TileRows<T>& a, const TileRows<T>& b = {}) {
+  if (a.pad.dst)
+    gfa::launch_pad_rows<T>(a.pad, b.pad, cur_stream());
+  else if (b.pad.dst)
+    gfa::launch_pad_rows<T>(b.pad, a.pad, cur_stream());
 }
 
 template <typename T>
@@ -282,30 +318,36 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(const Tensor& x, const Tensor& w,
   const auto shape = out_shape(x, n);
   c10::hip::HIPGuard guard(x.get_device());
   const OptTensor bc = bias ? OptTensor(bias->contiguous()) : bias;
-  Tensor y = torch::empty(shape, x.options());
+  Tensor y = new_tensor(shape, x.scalar_type(), x);
   OptTensor z;
-  if (save_z) z = torch::empty(shape, x.options().dtype(torch::kFloat32));
+  if (save_z) z = new_tensor(shape, torch::kFloat32, x);
   if (y.numel() == 0) return {y, z};
   DISPATCH_FT(x.scalar_type(), {
-    const Rows xr = tile_rows<scalar_t>(rows_of(x), k);
-    const Rows wr = tile_rows<scalar_t>(rows_of(w), k);
+    Rows xr = rows_of(x), wr = rows_of(w);
+    const int64_t m = xr.count;
+    TileRows<scalar_t> px, pw;
+    if (!gfa::linear_reads_any_rows(m)) {
+      px.add(xr, k);
+      pw.add(wr, k);
+      pad(px, pw);
+    }
     auto e = epilogue<scalar_t>(bc, p);
     Rows rr;
     if (residual) {
       rr = rows_of(*residual);
-      e.residual = cptr<scalar_t>(rr.t);
+      e.residual = rptr<scalar_t>(rr);
       e.res_stride = rr.stride;
     }
     e.z = mptr<float>(z);
     const int splits = gfa::linear_splits(
-        xr.count, n, k, std::is_same_v<scalar_t, float>, gfa::kRows);
-    const OptTensor parts = split_sums(splits, xr.count, n, x);
-    e.partial = mptr<float>(parts);
+        m, n, k, std::is_same_v<scalar_t, float>, gfa::kRows);
+    Room parts;
+    e.partial = parts.get<float>(splits > 1 ? splits * m * n : 0);
     gfa::launch_linear_forward<scalar_t>(
-        static_cast<scalar_t*>(y.data_ptr()), cptr<scalar_t>(xr.t),
-        cptr<scalar_t>(wr.t),
-        {xr.count, n, k, xr.stride, wr.stride, n, (float)p.weight_gain, k}, e,
-        splits, cur_stream());
+        static_cast<scalar_t*>(y.data_ptr()), rptr<scalar_t>(xr),
+        rptr<scalar_t>(wr),
+        {m, n, k, xr.stride, wr.stride, n, (float)p.weight_gain, k}, e, splits,
+        cur_stream());
   });
   HIP_CHECK_LAST();
   return {y, z};
@@ -322,83 +364,110 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
   c10::hip::HIPGuard guard(x.get_device());
   const int64_t m = dy.numel() / n;
   OptTensor dx, dw, db;
-  if (need_dx) dx = torch::empty(x.sizes(), x.options());
+  if (need_dx) dx = new_tensor(x.sizes(), x.scalar_type(), x);
   if (m == 0) {
     if (need_dw) dw = torch::zeros(w.sizes(), w.options());
     if (need_db) db = torch::zeros({n}, bias->options());
     return {dx, dw, db};
   }
-  if (need_dw) dw = torch::empty(w.sizes(), w.options());
-  if (need_db) db = torch::empty({n}, bias->options());
+  if (need_dw) dw = new_tensor(w.sizes(), w.scalar_type(), x);
+  if (need_db) db = new_tensor({n}, bias->scalar_type(), x);
   if (!need_dx && !need_dw && !need_db) return {dx, dw, db};
   const OptTensor bc = bias ? OptTensor(bias->contiguous()) : bias;
-  const auto f32 = x.options().dtype(torch::kFloat32);
   // a slope that is the same everywhere goes into the products: dz is dy
-  const bool curved = p.curved();
+  const bool curved = p.curved(), again = curved && !z;
   const double slope = curved ? 1.0 : p.gain;
+  const bool small = gfa::linear_backward_is_small(m, n, k);
   DISPATCH_FT(x.scalar_type(), {
-    const Rows xr = tile_rows<scalar_t>(rows_of(x), k);
-    const Rows wr = tile_rows<scalar_t>(rows_of(w), k);
-    Rows dr = rows_of(dy);
+    constexpr bool is_f32 = std::is_same_v<scalar_t, float>;
+    Rows xr = rows_of(x), wr = rows_of(w), dr = rows_of(dy);
+    TileRows<scalar_t> px, pw, pd;
+    const bool any = gfa::linear_reads_any_rows(m);
+    if (need_dw || (again && !any)) px.add(xr, k);
+    if (need_dx || (again && !any)) pw.add(wr, k);
+    pad(px, pw);
     auto e = epilogue<scalar_t>(bc, p);
-    OptTensor partial;
+    Room dz_room, partial_room, dx_parts, dw_parts;
+    float* partial = nullptr;
     int groups = 0;
-    if (curved && !z) {
-      // z again, from the product that made it
-      const int64_t width = (n + 7) / 8 * 8;
-      Rows dz{torch::empty({m, width}, x.options()), m, width};
-      e.dy = cptr<scalar_t>(dr.t);
-      e.dy_stride = dr.stride;
-      groups = gfa::linear_row_tiles(m, n);
-      if (need_db) partial = torch::empty({groups, n}, f32);
-      e.partial = mptr<float>(partial);
-      gfa::launch_linear_slope<scalar_t>(
-          static_cast<scalar_t*>(dz.t.data_ptr()), cptr<scalar_t>(xr.t),
-          cptr<scalar_t>(wr.t),
-          {m, n, k, xr.stride, wr.stride, width, (float)p.weight_gain, k}, e,
-          cur_stream());
-      dr = dz;
-    } else if (curved || need_db) {
-      const int64_t width = (n + 7) / 8 * 8;
-      Rows dz{Tensor(), m, width};
-      if (curved) dz.t = torch::empty({m, width}, x.options());
-      groups = gfa::linear_dz_groups(m, (int)n);
-      if (need_db) partial = torch::empty({groups, n}, f32);
-      gfa::launch_linear_dz<scalar_t>(
-          curved ? static_cast<scalar_t*>(dz.t.data_ptr()) : nullptr, width,
-          mptr<float>(partial), cptr<scalar_t>(dr.t), dr.stride,
-          curved ? mptr<float>(z) : nullptr, e.act, m, (int)n, cur_stream());
-      if (curved) dr = dz;
-    }
-    if (need_db) {
-      const float scale = (float)(p.bias_gain * slope);
-      if (bias->scalar_type() == torch::kFloat32)
-        gfa::launch_sum_groups<float>(mptr<float>(db), nullptr,
-                                      partial->data_ptr<float>(), groups,
-                                      (int)n, scale, cur_stream());
-      else
-        gfa::launch_sum_groups<gfa::bf16>(mptr<gfa::bf16>(db), nullptr,
-                                          partial->data_ptr<float>(), groups,
-                                          (int)n, scale, cur_stream());
+    if (curved) {
+      const int64_t width = (n + 7) / 8 * 8;  // zeros behind n
+      scalar_t* dz = dz_room.get<scalar_t>(m * width);
+      groups = again ? gfa::linear_row_tiles(m, n)
+                     : gfa::linear_dz_groups(m, (int)n);
+      partial = partial_room.get<float>(need_db ? groups * n : 0);
+      if (again) {
+        // z again, from the product that made it
+        e.dy = rptr<scalar_t>(dr);
+        e.dy_stride = dr.stride;
+        e.partial = partial;
+        gfa::launch_linear_slope<scalar_t>(
+            dz, rptr<scalar_t>(xr), rptr<scalar_t>(wr),
+            {m, n, k, xr.stride, wr.stride, width, (float)p.weight_gain, k}, e,
+            cur_stream());
+      } else {
+        gfa::launch_linear_dz<scalar_t>(dz, width, partial, rptr<scalar_t>(dr),
+                                        dr.stride, mptr<float>(z), e.act, m,
+                                        (int)n, cur_stream());
+      }
+      dr.at = dz;
+      dr.stride = width;
+    } else {
+      if (need_db && !small) {
+        groups = gfa::linear_dz_groups(m, (int)n);
+        partial = partial_room.get<float>(groups * n);
+        gfa::launch_linear_dz<scalar_t>(nullptr, 0, partial,
+                                        rptr<scalar_t>(dr), dr.stride, nullptr,
+                                        e.act, m, (int)n, cur_stream());
+      }
+      if (need_dx || need_dw) {
+        pd.add(dr, n);
+        pad(pd);
+      }
     }
     const float scale = (float)(p.weight_gain * slope);
-    if (need_dx || need_dw) dr = tile_rows<scalar_t>(dr, n);
-    constexpr bool is_f32 = std::is_same_v<scalar_t, float>;
-    if (need_dx) {
-      const int splits = gfa::linear_splits(m, k, n, is_f32, gfa::kInputs);
-      const OptTensor parts = split_sums(splits, m, k, x);
-      gfa::launch_linear_dx<scalar_t>(
-          mptr<scalar_t>(dx), mptr<float>(parts), cptr<scalar_t>(dr.t),
-          cptr<scalar_t>(wr.t),
-          {m, k, n, dr.stride, wr.stride, k, scale, n}, splits, cur_stream());
-    }
-    if (need_dw) {
-      const int splits = gfa::linear_splits(n, k, m, is_f32, gfa::kWeights);
-      const OptTensor parts = split_sums(splits, n, k, x);
-      gfa::launch_linear_dw<scalar_t>(
-          mptr<scalar_t>(dw), mptr<float>(parts), cptr<scalar_t>(dr.t),
-          cptr<scalar_t>(xr.t),
-          {n, k, m, dr.stride, xr.stride, k, scale, m}, splits, cur_stream());
+    const float db_scale = (float)(p.bias_gain * slope);
+    const bool db_f32 = need_db && bias->scalar_type() == torch::kFloat32;
+    const gfa::GemmArgs gx{m, k, n, dr.stride, wr.stride, k, scale, n};
+    const gfa::GemmArgs gw{n, k, m, dr.stride, xr.stride, k, scale, m};
+    if (small) {
+      gfa::SmallBackward<scalar_t> s{};
+      s.dw = gw;
+      s.dx = gx;
+      s.dw_out = mptr<scalar_t>(dw);
+      s.dx_out = mptr<scalar_t>(dx);
+      s.db_out = db ? db->data_ptr() : nullptr;
+      s.db_f32 = db_f32;
+      s.dz = rptr<scalar_t>(dr);
+      s.x = rptr<scalar_t>(xr);
+      s.w = rptr<scalar_t>(wr);
+      s.partial = partial;
+      s.groups = groups;
+      s.n = (int)n;
+      s.db_scale = db_scale;
+      gfa::launch_linear_backward_small<scalar_t>(s, cur_stream());
+    } else {
+      if (db_f32)
+        gfa::launch_sum_groups<float>(mptr<float>(db), nullptr, partial,
+                                      groups, (int)n, db_scale, cur_stream());
+      else if (need_db)
+        gfa::launch_sum_groups<gfa::bf16>(mptr<gfa::bf16>(db), nullptr,
+                                          partial, groups, (int)n, db_scale,
+                                          cur_stream());
+      if (need_dx) {
+        const int splits = gfa::linear_splits(m, k, n, is_f32, gfa::kInputs);
+        gfa::launch_linear_dx<scalar_t>(
+            mptr<scalar_t>(dx),
+            dx_parts.get<float>(splits > 1 ? splits * m * k : 0),
+            rptr<scalar_t>(dr), rptr<scalar_t>(wr), gx, splits, cur_stream());
+      }
+      if (need_dw) {
+        const int splits = gfa::linear_splits(n, k, m, is_f32, gfa::kWeights);
+        gfa::launch_linear_dw<scalar_t>(
+            mptr<scalar_t>(dw),
+            dw_parts.get<float>(splits > 1 ? splits * n * k : 0),
+            rptr<scalar_t>(dr), rptr<scalar_t>(xr), gw, splits, cur_stream());
+      }
     }
   });
   HIP_CHECK_LAST();

@@ -680,20 +680,21 @@ void linear_direct(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 // all 32x32), so a block's operands pass through LDS once and its time falls
 // with k alone; their sums meet in LDS. Where that still leaves CUs idle, k
 // is split over blocks too (kPartial).
+constexpr int kSmallLds = 4 * 2 * 2 * 32 * 128;  // stages, operands, depth
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
-__global__ __launch_bounds__(256)
-void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
-                  const T* __restrict__ a, const T* __restrict__ b) {
+GFA_DEV void small_block(char* lds, int block, const GemmArgs& g,
+                         const EpilogueArgs<T>& e, T* c, const T* a,
+                         const T* b) {
   constexpr int B = 32, DEPTH = 2, STAGES = 4, WAVES = 4, FM = 2, FN = 2;
   using OA = Operand<T, B, ACOLS>;
   using F = Frag<T>;
   constexpr int kHalf = OA::kBytes * DEPTH, kStage = 2 * kHalf;
-  __shared__ __attribute__((aligned(16))) char lds[STAGES * kStage];
+  static_assert(STAGES * kStage == kSmallLds, "what the callers give");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tn = (int)((g.N + B - 1) / B);
-  const int mt = blockIdx.x / tn;
-  const long m0 = (long)mt * B, n0 = (long)(blockIdx.x % tn) * B;
+  const int mt = block / tn;
+  const long m0 = (long)mt * B, n0 = (long)(block % tn) * B;
   const long kb = (long)blockIdx.y * g.k_split;
   const int kn = (int)min(g.K - kb, g.k_split);
   const auto finish = thread_part<T, EPI, FM, FN>(m0, n0, g, e);
@@ -730,6 +731,67 @@ void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   }
   wait_pieces<0>();  // the sums go where the pieces went
   join_waves<T, EPI, FM, FN>(acc, lds, n0, mt, finish, g, e, c);
+}
+
+template <typename T, bool ACOLS, bool BCOLS, int EPI>
+__global__ __launch_bounds__(256)
+void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
+                  const T* __restrict__ a, const T* __restrict__ b) {
+  __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
+  small_block<T, ACOLS, BCOLS, EPI>(lds, blockIdx.x, g, e, c, a, b);
+}
+
+// out[i] = scale * sum_r src[r][i] for eight columns from n0 on
+template <typename S>
+GFA_DEV void sum_columns(char* lds, const S* src, long stride, long rows,
+                         int n, int n0, float scale, void* out, bool out_f32) {
+  const int c = threadIdx.x & 7, q = threadIdx.x >> 3, i = n0 + c;
+  float* red = reinterpret_cast<float*>(lds);
+  float s = 0.f;
+  if (i < n) {
+#pragma unroll 8
+    for (long r = q; r < rows; r += 32) s += to_f32(src[r * stride + i]);
+  }
+  red[c * 33 + q] = s;
+  __syncthreads();
+  if (threadIdx.x < 8 && i < n) {
+    s = 0.f;
+    for (int k = 0; k < 32; ++k) s += red[c * 33 + k];
+    s *= scale;
+    if (out_f32)
+      static_cast<float*>(out)[i] = s;
+    else
+      put(static_cast<bf16*>(out) + i, s);
+  }
+}
+
+// A small layer's whole backward after dz: blocks of dw, of dx and of db
+// side by side. One launch for three costs the host less, and neither
+// product alone fills the card.
+template <typename T>
+__global__ __launch_bounds__(256)
+void linear_backward_small(SmallBackward<T> p) {
+  __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
+  const EpilogueArgs<T> none{};
+  int block = blockIdx.x;
+  if (block < p.dw_blocks) {
+    small_block<T, true, true, kPlain>(lds, block, p.dw, none, p.dw_out, p.dz,
+                                       p.x);
+    return;
+  }
+  block -= p.dw_blocks;
+  if (block < p.dx_blocks) {
+    small_block<T, false, true, kPlain>(lds, block, p.dx, none, p.dx_out, p.dz,
+                                        p.w);
+    return;
+  }
+  block -= p.dx_blocks;
+  if (p.partial)
+    sum_columns(lds, p.partial, p.n, p.groups, p.n, block * 8, p.db_scale,
+                p.db_out, p.db_f32);
+  else
+    sum_columns(lds, p.dz, p.dw.lda, p.dw.K, p.n, block * 8, p.db_scale,
+                p.db_out, p.db_f32);
 }
 
 // The epilogue over sums of k split over blocks; four n a thread.
@@ -789,25 +851,31 @@ void sum_splits(T* __restrict__ c, const float* __restrict__ partial,
 // dst[r][0..width) = src[r][0..n), zero behind: 16-byte rows for the tiles
 template <typename T>
 __global__ __launch_bounds__(256)
-void pad_rows(T* __restrict__ dst, const T* __restrict__ src, long stride,
-              long rows, int n, int width) {
-  const long count = rows * (width / 8);
+void pad_rows(PadArgs<T> p0, PadArgs<T> p1) {
+  const PadArgs<T>& p = blockIdx.y ? p1 : p0;
+  const int wide = p.width / 8;
+  const long count = p.rows * wide;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < count;
        i += (long)gridDim.x * 256) {
-    const long r = i / (width / 8);
-    const int col = (int)(i % (width / 8)) * 8;
+    const long r = i / wide;
+    const int col = (int)(i - r * wide) * 8;
     float v[8];
-    load8(v, src + r * stride + col, min(8, n - col));
-    store8(dst + r * width + col, v, 8);
+    load8(v, p.src + r * p.stride + col, min(8, p.n - col));
+    store8(p.dst + r * p.width + col, v, 8);
   }
 }
 
+// one tensor or two
 template <typename T>
-void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
-                     int width, hipStream_t s) {
-  const long blocks = (rows * (width / 8) + 255) / 256;
-  hipLaunchKernelGGL(pad_rows<T>, dim3((unsigned)(blocks < 4096 ? blocks : 4096)),
-                     dim3(256), 0, s, dst, src, stride, rows, n, width);
+void launch_pad_rows(const PadArgs<T>& p0, const PadArgs<T>& p1,
+                     hipStream_t s) {
+  auto work = [](const PadArgs<T>& p) {
+    return p.dst ? (p.rows * (p.width / 8) + 255) / 256 : 0l;
+  };
+  const long most = work(p0) > work(p1) ? work(p0) : work(p1);
+  hipLaunchKernelGGL(pad_rows<T>,
+                     dim3((unsigned)(most < 4096 ? most : 4096), p1.dst ? 2 : 1),
+                     dim3(256), 0, s, p0, p1);
 }
 
 namespace {
@@ -832,7 +900,7 @@ template <typename T, bool ACOLS, bool BCOLS, int EPI>
 void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
                  const EpilogueArgs<T>& e, int splits, hipStream_t s) {
   if constexpr (!ACOLS && !BCOLS) {
-    if (g.M <= 32) {
+    if (linear_reads_any_rows(g.M)) {
       const dim3 grid((unsigned)ceil_div(g.N, 16), splits);
       if (g.M <= 16)
         hipLaunchKernelGGL((linear_direct<T, 1, EPI>), grid, dim3(256), 0, s,
@@ -863,8 +931,11 @@ void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
 
 }  // namespace
 
+// linear_direct's rows
+bool linear_reads_any_rows(long M) { return M <= 32; }
+
 int linear_row_tiles(long M, long N) {
-  return ceil_div(M, tile_for(M, N, 1));
+  return linear_reads_any_rows(M) ? 1 : ceil_div(M, tile_for(M, N, 1));
 }
 
 // Blocks that share out k. dw, whose k is the rows: enough for about two
@@ -882,11 +953,14 @@ int linear_splits(long M, long N, long K, bool f32, LinearKind kind) {
     want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
     depth = 16 * bk;
   } else {
+    const int tile = tile_for(M, N, 1);
     long blocks;
-    if (kind == kRows && M <= 32)
+    if (kind == kRows && linear_reads_any_rows(M))
       blocks = ceil_div(N, 16);
-    else if (tile_for(M, N, 1) == 32)
+    else if (tile == 32)
       blocks = (long)ceil_div(M, 32) * ceil_div(N, 32);
+    else if (tile == 64)  // fewer, larger tiles in parts
+      blocks = (long)ceil_div(M, 128) * ceil_div(N, 128);
     else
       return 1;
     want = (256 + blocks - 1) / blocks;
@@ -1055,7 +1129,31 @@ void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
                      act, rows, n, wide);
 }
 
+// One launch where both products' tiles of 32 fit the card a few times over
+// and neither k is long.
+bool linear_backward_is_small(long m, long n, long k) {
+  auto tiles = [](long a, long b) {
+    return (long)ceil_div(a, 32) * ceil_div(b, 32);
+  };
+  return m <= 1024 && n <= 2048 && tiles(m, k) <= 768 && tiles(n, k) <= 1024;
+}
+
+template <typename T>
+void launch_linear_backward_small(SmallBackward<T> p, hipStream_t s) {
+  auto tiles = [](const GemmArgs& g) {
+    return ceil_div(g.M, 32) * ceil_div(g.N, 32);
+  };
+  p.dw_blocks = p.dw_out ? tiles(p.dw) : 0;
+  p.dx_blocks = p.dx_out ? tiles(p.dx) : 0;
+  const int db_blocks = p.db_out ? ceil_div(p.n, 8) : 0;
+  hipLaunchKernelGGL(linear_backward_small<T>,
+                     dim3(p.dw_blocks + p.dx_blocks + db_blocks), dim3(256), 0,
+                     s, p);
+}
+
 #define INSTANTIATE(T)                                                       \
+  template void launch_linear_backward_small<T>(SmallBackward<T>,            \
+                                                hipStream_t);                \
   template void launch_linear_forward<T>(T*, const T*, const T*,             \
                                          const GemmArgs&,                    \
                                          const EpilogueArgs<T>&, int,        \
@@ -1067,7 +1165,7 @@ void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
                                     const GemmArgs&, int, hipStream_t);      \
   template void launch_linear_dw<T>(T*, float*, const T*, const T*,          \
                                     const GemmArgs&, int, hipStream_t);      \
-  template void launch_pad_rows<T>(T*, const T*, long, long, int, int,       \
+  template void launch_pad_rows<T>(const PadArgs<T>&, const PadArgs<T>&,     \
                                    hipStream_t);                             \
   template void launch_linear_dz<T>(T*, long, float*, const T*, long,        \
                                     const float*, const ActParams&, long,    \

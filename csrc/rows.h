@@ -211,6 +211,8 @@ struct EpilogueArgs {
 // that many M * N floats if it is over 1.
 enum LinearKind { kRows, kInputs, kWeights };  // forward, dx, dw
 int linear_splits(long M, long N, long K, bool f32, LinearKind kind);
+// whether forward and slope of M rows read x and W at any alignment
+bool linear_reads_any_rows(long M);
 // y = clamp(act(alpha x W^T + bias) * gain) + residual
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
@@ -228,9 +230,35 @@ void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
 template <typename T>
 void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
                       const GemmArgs& g, int splits, hipStream_t);
+// dw, dx and db (each null if not wanted) of a small layer in one launch
 template <typename T>
-void launch_pad_rows(T* dst, const T* src, long stride, long rows, int n,
-                     int width, hipStream_t);
+struct SmallBackward {
+  GemmArgs dw, dx;
+  T *dw_out, *dx_out;
+  void* db_out;
+  bool db_f32;
+  const T *dz, *x, *w;
+  // db: db_scale times the sums of the groups of partial, or of dz's rows
+  const float* partial;
+  int groups, n;
+  float db_scale;
+  int dw_blocks, dx_blocks;
+};
+bool linear_backward_is_small(long m, long n, long k);
+template <typename T>
+void launch_linear_backward_small(SmallBackward<T> p, hipStream_t);
+
+// dst [rows][width] = src [rows][n] at a stride, zero behind n; dst may be
+// null. width is a multiple of 8.
+template <typename T>
+struct PadArgs {
+  T* dst;
+  const T* src;
+  long stride, rows;
+  int n, width;
+};
+template <typename T>
+void launch_pad_rows(const PadArgs<T>& p0, const PadArgs<T>& p1, hipStream_t);
 
 // dz = dy * slope(z) (z and dz null: dz = dy) and, unless partial is null,
 // partial[g][n] = sums of dz over the rows of group g
