@@ -339,14 +339,14 @@ std::tuple<Tensor, OptTensor> linear_act_fwd(const Tensor& x, const Tensor& w,
       e.res_stride = rr.stride;
     }
     e.z = mptr<float>(z);
-    const int splits = gfa::linear_splits(
+    const auto plan = gfa::linear_plan(
         m, n, k, std::is_same_v<scalar_t, float>, gfa::kRows);
     Room parts;
-    e.partial = parts.get<float>(splits > 1 ? splits * m * n : 0);
+    e.partial = parts.get<float>(plan.splits > 1 ? plan.splits * m * n : 0);
     gfa::launch_linear_forward<scalar_t>(
         static_cast<scalar_t*>(y.data_ptr()), rptr<scalar_t>(xr),
         rptr<scalar_t>(wr),
-        {m, n, k, xr.stride, wr.stride, n, (float)p.weight_gain, k}, e, splits,
+        {m, n, k, xr.stride, wr.stride, n, (float)p.weight_gain, k}, e, plan,
         cur_stream());
   });
   HIP_CHECK_LAST();
@@ -393,7 +393,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     if (curved) {
       const int64_t width = (n + 7) / 8 * 8;  // zeros behind n
       scalar_t* dz = dz_room.get<scalar_t>(m * width);
-      groups = again ? gfa::linear_row_tiles(m, n)
+      const auto plan = gfa::linear_plan(m, n, k, is_f32, gfa::kSlopes);
+      groups = again ? gfa::linear_row_tiles(plan, m)
                      : gfa::linear_dz_groups(m, (int)n);
       partial = partial_room.get<float>(need_db ? groups * n : 0);
       if (again) {
@@ -404,7 +405,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
         gfa::launch_linear_slope<scalar_t>(
             dz, rptr<scalar_t>(xr), rptr<scalar_t>(wr),
             {m, n, k, xr.stride, wr.stride, width, (float)p.weight_gain, k}, e,
-            cur_stream());
+            plan, cur_stream());
       } else {
         gfa::launch_linear_dz<scalar_t>(dz, width, partial, rptr<scalar_t>(dr),
                                         dr.stride, mptr<float>(z), e.act, m,
@@ -455,18 +456,18 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
                                           partial, groups, (int)n, db_scale,
                                           cur_stream());
       if (need_dx) {
-        const int splits = gfa::linear_splits(m, k, n, is_f32, gfa::kInputs);
+        const auto plan = gfa::linear_plan(m, k, n, is_f32, gfa::kInputs);
         gfa::launch_linear_dx<scalar_t>(
             mptr<scalar_t>(dx),
-            dx_parts.get<float>(splits > 1 ? splits * m * k : 0),
-            rptr<scalar_t>(dr), rptr<scalar_t>(wr), gx, splits, cur_stream());
+            dx_parts.get<float>(plan.splits > 1 ? plan.splits * m * k : 0),
+            rptr<scalar_t>(dr), rptr<scalar_t>(wr), gx, plan, cur_stream());
       }
       if (need_dw) {
-        const int splits = gfa::linear_splits(n, k, m, is_f32, gfa::kWeights);
+        const auto plan = gfa::linear_plan(n, k, m, is_f32, gfa::kWeights);
         gfa::launch_linear_dw<scalar_t>(
             mptr<scalar_t>(dw),
-            dw_parts.get<float>(splits > 1 ? splits * n * k : 0),
-            rptr<scalar_t>(dr), rptr<scalar_t>(xr), gw, splits, cur_stream());
+            dw_parts.get<float>(plan.splits > 1 ? plan.splits * n * k : 0),
+            rptr<scalar_t>(dr), rptr<scalar_t>(xr), gw, plan, cur_stream());
       }
     }
   });

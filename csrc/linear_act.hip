@@ -880,27 +880,30 @@ void launch_pad_rows(const PadArgs<T>& p0, const PadArgs<T>& p1,
 
 namespace {
 
-// The side of a tile: the largest that still gives the CUs a block each and
-// is not mostly padding. Large tiles read their operands less often
-// (8192x4096x4096 bf16: 266 us with 256, 314 with 128, 439 with 64), small
-// ones spread a small product wider (524288x128x128: 120 us with 256, 65 with
-// 128).
-int tile_for(long M, long N, int splits) {
-  auto blocks = [&](int b) {
-    return ((M + b - 1) / b) * ((N + b - 1) / b) * splits;
-  };
-  const long side = M < N ? M : N;
-  if (side > 128 && blocks(256) >= 256) return 256;
-  if (side > 64 && blocks(128) >= 192) return 128;
-  if (side > 32 && blocks(64) >= 192) return 64;
-  return 32;
-}
+// Microseconds that a CU spends on one k-tile of a block, alone on it or with
+// others, and on the rest of a block's work. Measured: 8192x4096x4096 bf16
+// takes 262, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 980,
+// 1021 and 1089 us; 524288x128x128 bf16, half of whose tiles of 256 would be
+// padding, 120 us with those and 48 us with 128. Of 21 shapes and up to 40
+// ways to cut each, in both types, what the figures choose is within 5% of
+// the quickest in 37 cases and within 20% in the others.
+struct TileCost {
+  int side;
+  double alone, shared, rest;
+};
+const TileCost kTileCosts[2][5] = {
+    // bf16
+    {{256, 2.0, 2.0, 8}, {128, 0.95, 0.61, 2}, {64, 0.40, 0.214, 1},
+     {32, 0.2, 0.12, 0.5}, {16, 0.06, 0.05, 0.5}},
+    // float
+    {{256, 7.6, 7.6, 8}, {128, 2.15, 2.0, 2}, {64, 0.65, 0.53, 1},
+     {32, 0.24, 0.21, 0.5}, {16, 0.165, 0.15, 0.5}}};
 
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
 void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
                  const EpilogueArgs<T>& e, int splits, hipStream_t s) {
   if constexpr (!ACOLS && !BCOLS) {
-    if (linear_reads_any_rows(g.M)) {
+    if (tile == 16) {
       const dim3 grid((unsigned)ceil_div(g.N, 16), splits);
       if (g.M <= 16)
         hipLaunchKernelGGL((linear_direct<T, 1, EPI>), grid, dim3(256), 0, s,
@@ -934,40 +937,37 @@ void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
 // linear_direct's rows
 bool linear_reads_any_rows(long M) { return M <= 32; }
 
-int linear_row_tiles(long M, long N) {
-  return linear_reads_any_rows(M) ? 1 : ceil_div(M, tile_for(M, N, 1));
+// The tile and the number of parts of k for which the busiest CU is done
+// first: rounds of blocks over 256 CUs, each of so many k-tiles, and for
+// parts a launch more that reads their sums again.
+LinearPlan linear_plan(long M, long N, long K, bool f32, LinearKind kind) {
+  const long ktiles = (K + (f32 ? 31 : 63)) / (f32 ? 32 : 64);
+  LinearPlan best{};
+  double least = 1e30;
+  for (const TileCost& t : kTileCosts[f32]) {
+    const bool direct = t.side == 16;
+    if (direct != (kind <= kSlopes && linear_reads_any_rows(M))) continue;
+    const long blocks =
+        direct ? (N + 15) / 16
+               : ((M + t.side - 1) / t.side) * ((N + t.side - 1) / t.side);
+    for (long s = 1; s <= 1024; s += (s + 3) / 4) {
+      const long each = (ktiles + s - 1) / s;
+      if (s > 1 && (kind == kSlopes || each < 8)) break;
+      const long rounds = (blocks * s + 255) / 256;
+      double cost = rounds == 1 ? each * t.alone + t.rest
+                                : rounds * (each * t.shared + t.rest);
+      if (s > 1) cost += 3 + 2e-6 * s * M * N;
+      if (cost < least) {
+        least = cost;
+        best = {t.side, (int)s};
+      }
+    }
+  }
+  return best;
 }
 
-// Blocks that share out k. dw, whose k is the rows: enough for about two
-// blocks of 128x128 a CU, at least 16 k-tiles each. The others: until there
-// are 256 blocks, with at least 32 k-tiles each, as the launch that sums
-// them takes about as long as those (17x512x512 float: 5.5 us in one part,
-// 7.0 us in two; 32x8192x512: 45 us in one, 13 us in eight).
-int linear_splits(long M, long N, long K, bool f32, LinearKind kind) {
-  const long bk = f32 ? 32 : 64;
-  long want, depth;
-  if (kind == kWeights) {
-    const long side = M < N ? M : N;
-    const int t = side > 64 ? 128 : side > 32 ? 64 : 32;
-    const long tiles = (long)ceil_div(M, t) * ceil_div(N, t);
-    want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-    depth = 16 * bk;
-  } else {
-    const int tile = tile_for(M, N, 1);
-    long blocks;
-    if (kind == kRows && linear_reads_any_rows(M))
-      blocks = ceil_div(N, 16);
-    else if (tile == 32)
-      blocks = (long)ceil_div(M, 32) * ceil_div(N, 32);
-    else if (tile == 64)  // fewer, larger tiles in parts
-      blocks = (long)ceil_div(M, 128) * ceil_div(N, 128);
-    else
-      return 1;
-    want = (256 + blocks - 1) / blocks;
-    depth = 32 * bk;
-  }
-  const long most = (K + depth - 1) / depth;
-  return (int)(want < most ? want : most);
+int linear_row_tiles(const LinearPlan& p, long M) {
+  return p.tile == 16 ? 1 : ceil_div(M, p.tile);
 }
 
 namespace {
@@ -975,13 +975,14 @@ namespace {
 // C in one launch, or by splits of k and a launch that sums them
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
 void launch_split(T* c, const T* a, const T* b, GemmArgs g,
-                  EpilogueArgs<T> e, int splits, hipStream_t s) {
+                  EpilogueArgs<T> e, const LinearPlan& p, hipStream_t s) {
+  int splits = p.splits;
   if (splits > 1) {
     const long bk = 128 / sizeof(T);
     g.k_split = ((g.K + splits - 1) / splits + bk - 1) / bk * bk;
     splits = (int)((g.K + g.k_split - 1) / g.k_split);
   }
-  const int tile = tile_for(g.M, g.N, splits);
+  const int tile = p.tile;
   if (splits == 1) {
     launch_tile<T, ACOLS, BCOLS, EPI>(tile, c, a, b, g, e, 1, s);
     return;
@@ -1005,32 +1006,32 @@ void launch_split(T* c, const T* a, const T* b, GemmArgs g,
 
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
-                           const EpilogueArgs<T>& e, int splits,
+                           const EpilogueArgs<T>& e, const LinearPlan& p,
                            hipStream_t s) {
-  launch_split<T, false, false, kForward>(y, x, w, g, e, splits, s);
+  launch_split<T, false, false, kForward>(y, x, w, g, e, p, s);
 }
 
 template <typename T>
 void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
-                         const EpilogueArgs<T>& e, hipStream_t s) {
-  launch_tile<T, false, false, kSlope>(tile_for(g.M, g.N, 1), dz, x, w, g, e,
-                                       1, s);
+                         const EpilogueArgs<T>& e, const LinearPlan& p,
+                         hipStream_t s) {
+  launch_tile<T, false, false, kSlope>(p.tile, dz, x, w, g, e, 1, s);
 }
 
 template <typename T>
 void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
-                      const GemmArgs& g, int splits, hipStream_t s) {
+                      const GemmArgs& g, const LinearPlan& p, hipStream_t s) {
   EpilogueArgs<T> e{};
   e.partial = partial;
-  launch_split<T, false, true, kPlain>(dx, dz, w, g, e, splits, s);
+  launch_split<T, false, true, kPlain>(dx, dz, w, g, e, p, s);
 }
 
 template <typename T>
 void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
-                      const GemmArgs& g, int splits, hipStream_t s) {
+                      const GemmArgs& g, const LinearPlan& p, hipStream_t s) {
   EpilogueArgs<T> e{};
   e.partial = partial;
-  launch_split<T, true, true, kPlain>(dw, dz, x, g, e, splits, s);
+  launch_split<T, true, true, kPlain>(dw, dz, x, g, e, p, s);
 }
 
 // ---- dz from a kept z, and sums over rows ----
@@ -1156,15 +1157,18 @@ void launch_linear_backward_small(SmallBackward<T> p, hipStream_t s) {
                                                 hipStream_t);                \
   template void launch_linear_forward<T>(T*, const T*, const T*,             \
                                          const GemmArgs&,                    \
-                                         const EpilogueArgs<T>&, int,        \
-                                         hipStream_t);                       \
+                                         const EpilogueArgs<T>&,             \
+                                         const LinearPlan&, hipStream_t);    \
   template void launch_linear_slope<T>(T*, const T*, const T*,               \
                                        const GemmArgs&,                      \
-                                       const EpilogueArgs<T>&, hipStream_t); \
+                                       const EpilogueArgs<T>&,               \
+                                       const LinearPlan&, hipStream_t);      \
   template void launch_linear_dx<T>(T*, float*, const T*, const T*,          \
-                                    const GemmArgs&, int, hipStream_t);      \
+                                    const GemmArgs&, const LinearPlan&,      \
+                                    hipStream_t);                            \
   template void launch_linear_dw<T>(T*, float*, const T*, const T*,          \
-                                    const GemmArgs&, int, hipStream_t);      \
+                                    const GemmArgs&, const LinearPlan&,      \
+                                    hipStream_t);                            \
   template void launch_pad_rows<T>(const PadArgs<T>&, const PadArgs<T>&,     \
                                    hipStream_t);                             \
   template void launch_linear_dz<T>(T*, long, float*, const T*, long,        \

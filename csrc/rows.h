@@ -206,30 +206,34 @@ struct EpilogueArgs {
   // parts: their sums
   float* partial;
 };
-// Into how many parts the launches below share k, given C's M x N: each but
-// linear_slope takes linear_splits(...), and needs partial (e.partial) of
-// that many M * N floats if it is over 1.
-enum LinearKind { kRows, kInputs, kWeights };  // forward, dx, dw
-int linear_splits(long M, long N, long K, bool f32, LinearKind kind);
+// How C's M x N are cut up for the launches below: the side of a tile, and
+// into how many parts k is shared. For more than one, partial (e.partial)
+// holds that many M * N floats.
+struct LinearPlan {
+  int tile, splits;
+};
+enum LinearKind { kRows, kSlopes, kInputs, kWeights };
+LinearPlan linear_plan(long M, long N, long K, bool f32, LinearKind kind);
 // whether forward and slope of M rows read x and W at any alignment
 bool linear_reads_any_rows(long M);
 // y = clamp(act(alpha x W^T + bias) * gain) + residual
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
-                           const EpilogueArgs<T>& e, int splits, hipStream_t);
+                           const EpilogueArgs<T>& e, const LinearPlan&, hipStream_t);
 // dz = dy * slope(alpha x W^T + bias); linear_row_tiles sums of rows
-int linear_row_tiles(long M, long N);
+int linear_row_tiles(const LinearPlan&, long M);
 template <typename T>
 void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
-                         const EpilogueArgs<T>& e, hipStream_t);
+                         const EpilogueArgs<T>& e, const LinearPlan&,
+                         hipStream_t);
 // dx[M, N] = alpha dz[M, K] W[K, N]
 template <typename T>
 void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
-                      const GemmArgs& g, int splits, hipStream_t);
+                      const GemmArgs& g, const LinearPlan&, hipStream_t);
 // dw[M, N] = alpha dz[K, M]^T x[K, N]
 template <typename T>
 void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
-                      const GemmArgs& g, int splits, hipStream_t);
+                      const GemmArgs& g, const LinearPlan&, hipStream_t);
 // dw, dx and db (each null if not wanted) of a small layer in one launch
 template <typename T>
 struct SmallBackward {
