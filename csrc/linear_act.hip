@@ -8,7 +8,9 @@
 // Every product is one C[m, n] = sum_k A[m, k] B[n, k] over operands that are
 // contiguous along k ("rows") or along m or n ("columns"). Sums in float on
 // the matrix cores; what leaves a kernel is rounded to T once.
+#include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "rows.h"
 
@@ -20,9 +22,9 @@ using LdsPtr = __attribute__((address_space(3))) void*;
 // ---- tiles ----
 // A block computes BM x BN of C with WM x WN waves. Both operands of a k-tile
 // go from memory to LDS without passing through registers, 1 KB a wave and
-// instruction; a k-tile is 128 bytes deep (64 bf16, 32 float) and STAGES of
-// them are in LDS, one being used while the others are filled, with one
-// barrier a k-tile. Reads outside the operands return zero (the bounds are those of
+// instruction; a k-tile is 128 bytes deep (64 bf16, 32 float) and two of them
+// are in LDS, one being used while the other is filled, with one barrier a
+// k-tile. Reads outside the operands return zero (the bounds are those of
 // the buffer descriptor), so any M, N, K take this path as long as rows are
 // 16-byte aligned.
 //
@@ -64,7 +66,7 @@ template <> struct Unaligned<bf16> {
 };
 template <typename T> struct Frag;
 template <> struct Frag<bf16> {
-  static constexpr int kStep = 32;
+  static constexpr int kStep = 32, kMfmas = 1, kColReads = 2;
   using Type = s16x8;
   template <int BX, bool COLS>
   GFA_DEV static Type read(const char* lds, int row0, int step, int lane) {
@@ -98,7 +100,8 @@ template <> struct Frag<bf16> {
   }
 };
 template <> struct Frag<float> {
-  static constexpr int kStep = 16;  // k = 4 * (lane / 16) + j in step j of 4
+  // k = 4 * (lane / 16) + j in step j of 4
+  static constexpr int kStep = 16, kMfmas = 4, kColReads = 4;
   using Type = f32x4;
   template <int BX, bool COLS>
   GFA_DEV static Type read(const char* lds, int row0, int step, int lane) {
@@ -269,8 +272,20 @@ struct Loader {
   }
 };
 
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool ACOLS,
-          bool BCOLS, int EPI>
+// One step's instructions in the order written in linear_tile: for each row
+// of fragments its products, then the LDS reads for the next step.
+template <int FM, int FN, int MFMAS, int READS_A, int READS_B, int... I>
+GFA_DEV void order(std::integer_sequence<int, I...>) {
+  constexpr int kMfma = 0x8, kLdsRead = 0x100;
+  ((__builtin_amdgcn_sched_group_barrier(kMfma, FN * MFMAS, 0),
+    __builtin_amdgcn_sched_group_barrier(
+        kLdsRead,
+        ((I + 1) * FN / FM - I * FN / FM) * READS_B + READS_A, 0)),
+   ...);
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool ACOLS, bool BCOLS,
+          int EPI>
 __global__ __launch_bounds__(WM * WN * 64)
 void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
                  const T* __restrict__ a, const T* __restrict__ b) {
@@ -283,7 +298,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   // the epilogue turns 32 rows of a wave at a time in LDS
   constexpr int EROW = TN * 4 + 16;
   constexpr int kEpi = WAVES * 32 * EROW;
-  constexpr int kLds = STAGES * kStage > kEpi ? STAGES * kStage : kEpi;
+  constexpr int kLds = 2 * kStage > kEpi ? 2 * kStage : kEpi;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
 
   const int lane = threadIdx.x & 63;
@@ -318,31 +333,71 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   const int wm = wave / WN * TM, wn = wave % WN * TN;
   f32x4 acc[FM][FN] = {};
   const int tiles = (kn + BK - 1) / BK;
+  // n along the rows of the result, so that a lane holds four neighbours:
+  // b is the left operand.
+  struct Frags {
+    typename F::Type a[FM], b[FN];
+  };
+  auto read_a = [&](Frags& f, int stage, int step, int i) {
+    f.a[i] = F::template read<BM, ACOLS>(lds + stage * kStage, wm + i * 16,
+                                         step, lane);
+  };
+  auto read_b = [&](Frags& f, int stage, int step, int j) {
+    f.b[j] = F::template read<BN, BCOLS>(lds + stage * kStage + OA::kBytes,
+                                         wn + j * 16, step, lane);
+  };
+  if constexpr (BM == 256) {
+    // One block a CU: while one of a k-tile's two steps is multiplied, the
+    // fragments of the next are read, a row's as soon as the row before it is
+    // done with, and the k-tile after next is fetched into the half that was
+    // read last (8192x4096x4096 bf16: 247 us, 263 us as below).
+    auto multiply = [&](const Frags& f, Frags& next, int stage, int step) {
 #pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t) fetch(t);
-  int use = 0, fill = STAGES - 1;
-  for (int t = 0; t < tiles; ++t) {
-    wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
-    if (STAGES > 2 || t + 1 < tiles) fetch(fill);
-    const char* la_ = lds + use * kStage;
-    const char* lb_ = la_ + OA::kBytes;
-    use = use + 1 == STAGES ? 0 : use + 1;
-    fill = fill + 1 == STAGES ? 0 : fill + 1;
+      for (int i = 0; i < FM; ++i) {
+  #pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
 #pragma unroll
-    for (int s = 0; s < BK / F::kStep; ++s) {
-      typename F::Type fa[FM], fb[FN];
+        for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
+          read_b(next, stage, step, j);
+        read_a(next, stage, step, i);
+      }
+      order<FM, FN, F::kMfmas, ACOLS ? F::kColReads : 1,
+            BCOLS ? F::kColReads : 1>(std::make_integer_sequence<int, FM>{});
+    };
+    fetch(0);
+    fetch(1);
+    wait_pieces<LA::kPieces + LB::kPieces>();
+    Frags f0, f1;
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-        fb[j] = F::template read<BN, BCOLS>(lb_, wn + j * 16, s, lane);
+    for (int j = 0; j < FN; ++j) read_b(f0, 0, 0, j);
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-        fa[i] = F::template read<BM, ACOLS>(la_, wm + i * 16, s, lane);
-      // n along the rows of the result: a lane holds four neighbours
+    for (int i = 0; i < FM; ++i) read_a(f0, 0, 0, i);
+    for (int t = 0; t < tiles; ++t) {
+      multiply(f0, f1, t & 1, 1);
+      wait_pieces<0>();
+      fetch(t & 1);
+      multiply(f1, f0, (t + 1) & 1, 0);
+    }
+  } else {
+    // Several blocks a CU fill each other's gaps, and a simple order leaves
+    // them the registers (dw of 65536x512x2048: 176 us, 250 us as above).
+    fetch(0);
+    for (int t = 0; t < tiles; ++t) {
+      wait_pieces<0>();
+      if (t + 1 < tiles) fetch((t + 1) & 1);
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int s = 0; s < 2; ++s) {
+        Frags f;
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
+        for (int j = 0; j < FN; ++j) read_b(f, t & 1, s, j);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) read_a(f, t & 1, s, i);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
+      }
     }
   }
   wait_pieces<0>();  // the epilogue writes where the pieces go
@@ -882,7 +937,7 @@ namespace {
 
 // Microseconds that a CU spends on one k-tile of a block, alone on it or with
 // others, and on the rest of a block's work. Measured: 8192x4096x4096 bf16
-// takes 262, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 980,
+// takes 247, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 955,
 // 1021 and 1089 us; 524288x128x128 bf16, half of whose tiles of 256 would be
 // padding, 120 us with those and 48 us with 128. Of 21 shapes and up to 40
 // ways to cut each, in both types, what the figures choose is within 5% of
@@ -893,10 +948,10 @@ struct TileCost {
 };
 const TileCost kTileCosts[2][5] = {
     // bf16
-    {{256, 2.0, 2.0, 8}, {128, 0.95, 0.61, 2}, {64, 0.40, 0.214, 1},
+    {{256, 1.9, 1.9, 8}, {128, 0.95, 0.61, 2}, {64, 0.40, 0.214, 1},
      {32, 0.2, 0.12, 0.5}, {16, 0.06, 0.05, 0.5}},
     // float
-    {{256, 7.6, 7.6, 8}, {128, 2.15, 2.0, 2}, {64, 0.65, 0.53, 1},
+    {{256, 7.4, 7.4, 8}, {128, 2.15, 2.0, 2}, {64, 0.65, 0.53, 1},
      {32, 0.24, 0.21, 0.5}, {16, 0.165, 0.15, 0.5}}};
 
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
@@ -917,7 +972,7 @@ void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
   const long tiles = ceil_div(g.M, tile) * (long)ceil_div(g.N, tile);
   const dim3 grid((unsigned)((tiles * splits + 7) / 8 * 8));
 #define LAUNCH(B, WM, WN)                                                     \
-  hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, 2, ACOLS, BCOLS, EPI>),    \
+  hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, ACOLS, BCOLS, EPI>),       \
                      grid, dim3(WM * WN * 64), 0, s, g, e, c, a, b)
   if (tile == 256)
     LAUNCH(256, 2, 4);
@@ -950,12 +1005,15 @@ LinearPlan linear_plan(long M, long N, long K, bool f32, LinearKind kind) {
     const long blocks =
         direct ? (N + 15) / 16
                : ((M + t.side - 1) / t.side) * ((N + t.side - 1) / t.side);
-    for (long s = 1; s <= 1024; s += (s + 3) / 4) {
+    // one part, or as many as fill so many rounds, of 8 k-tiles at least
+    for (int fill = 0; fill <= 8; ++fill) {
+      const long s = fill ? std::min(256 * fill / blocks, ktiles / 8) : 1;
+      if (fill && (s < 2 || kind == kSlopes)) continue;
       const long each = (ktiles + s - 1) / s;
-      if (s > 1 && (kind == kSlopes || each < 8)) break;
       const long rounds = (blocks * s + 255) / 256;
       double cost = rounds == 1 ? each * t.alone + t.rest
                                 : rounds * (each * t.shared + t.rest);
+      if (kind == kWeights && t.side == 256 && !f32) cost *= 1.15;
       if (s > 1) cost += 3 + 2e-6 * s * M * N;
       if (cost < least) {
         least = cost;

@@ -34,6 +34,8 @@ from ..ops import (
     bipartite_attention,
     conv2d_gradfix,
     downsample2d,
+    layer_norm,
+    linear_act,
     linear_nobias,
     linear_transposed,
     minibatch_stddev,
@@ -65,7 +67,13 @@ class FullyConnected(nn.Module):
         self.weight_gain = lr_mul / math.sqrt(in_features)
         self.bias_gain = lr_mul
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
+        """act(x W^T + b), plus the residual in the product's epilogue."""
+        if residual is not None:
+            return linear_act(x, self.weight.to(x.dtype), self.bias,
+                              act=self.act, residual=residual,
+                              weight_gain=self.weight_gain,
+                              bias_gain=self.bias_gain)
         w = (self.weight * self.weight_gain).to(x.dtype)
         b = self.bias
         if b is not None:
@@ -74,6 +82,19 @@ class FullyConnected(nn.Module):
         # hipBLASLt's direct tall-K GEMM runs ~25 TF/s, the split ~250+
         y = linear_nobias(x, w)
         return _fc_bias_act(y, b, self.act)
+
+
+class LayerNorm(nn.Module):
+    """Normalization of a token over its channels, learned scale and shift."""
+
+    def __init__(self, features, eps=1e-5):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(features))
+        self.bias = nn.Parameter(torch.zeros(features))
+        self.eps = eps
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
 
 
 def _fc_transposed(fc, u):
@@ -291,8 +312,16 @@ class BipartiteLayer(nn.Module):
 
 
 class MappingNetwork(nn.Module):
+    """Per-component MLP from z to w.
+
+    residual: every layer after the first is a pre-norm residual one,
+    x + act(W layer_norm(x) + b), so that deeper mappings keep their
+    gradients; off, the layers follow each other plainly.
+    """
+
     def __init__(self, z_dim=512, w_dim=512, num_components=16, num_ws=14,
-                 num_layers=8, lr_mul=0.01, w_avg_beta=0.995, label_dim=0):
+                 num_layers=8, lr_mul=0.01, w_avg_beta=0.995, label_dim=0,
+                 residual=False):
         super().__init__()
         self.z_dim, self.w_dim = z_dim, w_dim
         self.num_components = num_components  # k (attention latents)
@@ -311,6 +340,9 @@ class MappingNetwork(nn.Module):
             layers.append(FullyConnected(dims[i], dims[i + 1], act="lrelu",
                                          lr_mul=lr_mul))
         self.layers = nn.ModuleList(layers)
+        self.norms = nn.ModuleList(
+            LayerNorm(w_dim) for _ in range(num_layers - 1)) \
+            if residual else None
         self.register_buffer("w_avg", torch.zeros(self.num_latents, w_dim))
 
     def forward(self, z, label=None, truncation_psi=1.0,
@@ -324,8 +356,13 @@ class MappingNetwork(nn.Module):
             y = pixel_norm(self.label_embed(label.to(torch.float32)), dim=-1)
             x = torch.cat([x, y.unsqueeze(1).expand(-1, self.num_latents,
                                                     -1)], dim=-1)
-        for layer in self.layers:
-            x = layer(x)
+        if self.norms is None:
+            for layer in self.layers:
+                x = layer(x)
+        else:
+            x = self.layers[0](x)
+            for norm, layer in zip(self.norms, self.layers[1:]):
+                x = layer(norm(x), residual=x)
         if update_w_avg:
             with torch.no_grad():
                 self.w_avg.copy_(
@@ -509,7 +546,7 @@ class Generator(nn.Module):
                  attn_resolutions=None, use_pos=True, channel_base=32768,
                  channel_max=512, bf16_res_count=16, mapping_layers=8,
                  mapping_lr_mul=0.01, w_avg_beta=0.995, conv_clamp=256.0,
-                 style_mixing_prob=0.9, label_dim=0):
+                 style_mixing_prob=0.9, label_dim=0, mapping_residual=False):
         super().__init__()
         self.z_dim = z_dim
         self.w_dim = w_dim
@@ -527,7 +564,7 @@ class Generator(nn.Module):
             bf16_res_count=bf16_res_count, mapping_layers=mapping_layers,
             mapping_lr_mul=mapping_lr_mul, w_avg_beta=w_avg_beta,
             conv_clamp=conv_clamp, style_mixing_prob=style_mixing_prob,
-            label_dim=label_dim)
+            label_dim=label_dim, mapping_residual=mapping_residual)
         self.synthesis = SynthesisNetwork(
             w_dim=w_dim, img_resolution=img_resolution,
             img_channels=img_channels, num_components=num_components,
@@ -539,7 +576,7 @@ class Generator(nn.Module):
             z_dim=z_dim, w_dim=w_dim, num_components=num_components,
             num_ws=self.synthesis.num_ws, num_layers=mapping_layers,
             lr_mul=mapping_lr_mul, w_avg_beta=w_avg_beta,
-            label_dim=label_dim)
+            label_dim=label_dim, residual=mapping_residual)
 
     @property
     def num_latents(self):

@@ -733,3 +733,67 @@ def test_captured_and_replayed(dev, m):
             torch.cuda.synchronize()
             for a, b in zip(outs[k], want):
                 assert torch.equal(a, b)
+
+
+# ---------------- in the mapping network ----------------
+def mapping(residual, layers=4, dim=64):
+    from gansformer_amd.models.networks import MappingNetwork
+    torch.manual_seed(5)
+    net = MappingNetwork(z_dim=dim, w_dim=dim, num_components=4, num_ws=3,
+                         num_layers=layers, residual=residual)
+    if residual:
+        with torch.no_grad():
+            for norm in net.norms:
+                norm.weight.add_(0.2 * torch.randn_like(norm.weight))
+                norm.bias.add_(0.2 * torch.randn_like(norm.bias))
+    return net
+
+
+def test_residual_mapping_is_the_formula():
+    net, z = mapping(True), randn(3, 5, 64, seed=7)
+    x = z * (z.square().mean(-1, keepdim=True) + 1e-8).rsqrt()
+    x = net.layers[0](x)
+    for norm, fc in zip(net.norms, list(net.layers)[1:]):
+        h = torch.nn.functional.layer_norm(x, (64,), norm.weight, norm.bias,
+                                           1e-5)
+        x = x + math.sqrt(2) * torch.nn.functional.leaky_relu(
+            h @ (fc.weight * fc.weight_gain).t() + fc.bias * fc.bias_gain, 0.2)
+    assert torch.allclose(net(z)[:, 0], x, rtol=1e-4, atol=1e-4)
+
+
+def test_plain_mapping_has_no_norms():
+    keys = set(mapping(False).state_dict())
+    assert not any("norm" in k for k in keys)
+    assert keys < set(mapping(True).state_dict())
+
+
+def test_generator_with_residual_mapping():
+    from gansformer_amd.models.networks import Generator
+    G = Generator(z_dim=32, w_dim=32, img_resolution=16, num_components=4,
+                  channel_base=256, channel_max=32, bf16_res_count=0,
+                  mapping_layers=3, mapping_residual=True)
+    assert G.init_kwargs["mapping_residual"]
+    img = G(G.sample_z(2))
+    grads = torch.autograd.grad(img.square().mean(),
+                                list(G.mapping.norms.parameters()))
+    assert all(torch.isfinite(g).all() and g.any() for g in grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 40])
+def test_residual_mapping_matches_the_cpu(dev, batch):
+    """float32 on both sides. A layer's product of 64 terms, its norm over
+    64 and its epilogue are each off by at most 2 * 96 u of the norm of what
+    they work on, on either side, and four layers add up; the backward pass
+    is as deep again, with sums over the 5 * batch rows."""
+    net, z = mapping(True), randn(batch, 5, 64, seed=7)
+    dy = randn(batch, 3, 5, 64, seed=8)
+
+    def grads(m, z, dy):
+        w = m(z)
+        return [w.detach(), *torch.autograd.grad(w, list(m.parameters()), dy)]
+    want = grads(net, z, dy)
+    got = grads(net.to(dev), z.to(dev), dy.to(dev))
+    for g, r in zip(got, want):
+        tol = 4 * 2 * 2 * 2 * max(96, 5 * batch) * U
+        assert (g.cpu() - r).norm() <= tol * r.norm()

@@ -35,6 +35,7 @@ def build_configs(args):
         integration=args.integration, use_pos=not args.no_pos,
         channel_base=args.fmap_base, channel_max=args.fmap_max,
         bf16_res_count=args.bf16_res, mapping_layers=args.mapping_layers,
+        mapping_residual=args.mapping_residual,
         style_mixing_prob=args.style_mixing)
     if args.attn_resolutions:
         G_args.attn_resolutions = [int(r) for r in parse_comma_list(args.attn_resolutions)]
@@ -94,6 +95,8 @@ def main(argv=None):
     p.add_argument("--fmap-base", type=int, default=32768)
     p.add_argument("--fmap-max", type=int, default=512)
     p.add_argument("--mapping-layers", type=int, default=8)
+    p.add_argument("--mapping-residual", action="store_true",
+                   help="pre-norm residual layers in the mapping network")
     p.add_argument("--mbstd-group", type=int, default=4)
     p.add_argument("--bf16-res", type=int, default=16,
                    help="number of top resolutions computed in bf16")
