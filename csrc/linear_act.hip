@@ -295,9 +295,10 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   constexpr int BK = OA::BK, WAVES = WM * WN;
   constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr int kStage = OA::kBytes + OB::kBytes;
-  // the epilogue turns 32 rows of a wave at a time in LDS
+  // the epilogue turns so many rows of a wave at a time in LDS
+  constexpr int ROWS = 32;
   constexpr int EROW = TN * 4 + 16;
-  constexpr int kEpi = WAVES * 32 * EROW;
+  constexpr int kEpi = WAVES * ROWS * EROW;
   constexpr int kLds = 2 * kStage > kEpi ? 2 * kStage : kEpi;
   __shared__ __attribute__((aligned(16))) char lds[kLds];
 
@@ -403,16 +404,17 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   wait_pieces<0>();  // the epilogue writes where the pieces go
 
   // ---- epilogue ----
-  // Each wave passes 32 rows at a time through LDS of its own, from the
+  // Each wave passes ROWS rows at a time through LDS of its own, from the
   // matrix cores' layout to eight neighbouring n a lane: full lines to and
-  // from memory, and the activation once in a loop instead of unrolled over
-  // all accumulators.
-  constexpr int LPR = TN / 8, RPI = 64 / LPR, ITER = 32 / RPI;
-  char* mine = lds + wave * 32 * EROW;
+  // from memory, and a loop for the activation, whose code unrolled over all
+  // accumulators would not stay in the instruction cache.
+  constexpr int LPR = TN / 8, RPI = 64 / LPR, ITER = ROWS / RPI;
+  char* mine = lds + wave * ROWS * EROW;
   const long n = n0 + wn + (lane % LPR) * 8;
   const int left = (int)max(0l, min(8l, g.N - n));
   const bool whole = n0 + wn + TN <= g.N;
-  const bool curved = e.act.act != kLinear || e.act.clamp < INFINITY;
+  const bool curved =
+      EPI == kSlope || e.act.act != kLinear || e.act.clamp < INFINITY;
   float bias[8] = {};
   if (EPI != kPlain && EPI != kPartial && e.bias && left) {
     if (e.bias_f32)
@@ -422,14 +424,16 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 #pragma unroll
     for (int j = 0; j < 8; ++j) bias[j] *= e.bias_gain;
   }
+  const T* op = EPI == kForward ? e.residual : EPI == kSlope ? e.dy : nullptr;
+  const long os = EPI == kForward ? e.res_stride : e.dy_stride;
   float sums[8] = {};
 #pragma unroll
-  for (int h = 0; h < FM / 2; ++h) {
-    const long mh = m0 + wm + h * 32 + lane / LPR;
-    // on its way while the activation is computed
+  for (int h = 0; h < TM / ROWS; ++h) {
+    const long mh = m0 + wm + h * ROWS + lane / LPR;
+    char* at = mine + lane / LPR * EROW + (lane % LPR) * 32;
+    // Residual or dy: all asked for before the first store, which would hold
+    // up what waits for a load behind it. Rows past the last repeat it.
     Eight<T> other[ITER];
-    const T* op = EPI == kForward ? e.residual : EPI == kSlope ? e.dy : nullptr;
-    const long os = EPI == kForward ? e.res_stride : e.dy_stride;
     if (op && whole) {
 #pragma unroll
       for (int q = 0; q < ITER; ++q)
@@ -441,65 +445,68 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < ROWS / 16; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j)
         *reinterpret_cast<f32x4*>(mine + (i * 16 + (lane & 15)) * EROW +
                                   (j * 16 + (lane >> 4) * 4) * 4) =
-            acc[h * 2 + i][j];
+            acc[h * (ROWS / 16) + i][j];
     __builtin_amdgcn_wave_barrier();
-    char* at = mine + lane / LPR * EROW + (lane % LPR) * 32;
-    if ((EPI == kForward && curved) || EPI == kSlope) {
+    auto read = [&](float (&z)[8], int q) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(at + q * RPI * EROW);
+      const f32x4 v[2] = {p[0], p[1]};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] = v[j / 4][j % 4];
+    };
+    if ((EPI == kForward || EPI == kSlope) && curved) {
+      // the activation, stored at once or back to meet the operands
 #pragma unroll 1
       for (int q = 0; q < ITER; ++q) {
-        f32x4* p = reinterpret_cast<f32x4*>(at + q * RPI * EROW);
-        f32x4 v[2] = {p[0], p[1]};
-        float z[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          z[j] = g.alpha * v[j / 4][j % 4] + bias[j];
         const long m = mh + q * RPI;
-        if (EPI == kForward && e.z && m < g.M) store8(e.z + m * g.N + n, z, left);
+        float z[8];
+        read(z, q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = g.alpha * z[j] + bias[j];
+        if (EPI == kForward && e.z && m < g.M)
+          store8(e.z + m * g.N + n, z, left);
         if (EPI == kForward)
           act_values(z, e.act);
         else
           act_slopes(z, e.act);
-        p[0] = f32x4{z[0], z[1], z[2], z[3]};
-        p[1] = f32x4{z[4], z[5], z[6], z[7]};
+        if (op) {
+          f32x4* p = reinterpret_cast<f32x4*>(at + q * RPI * EROW);
+          p[0] = f32x4{z[0], z[1], z[2], z[3]};
+          p[1] = f32x4{z[4], z[5], z[6], z[7]};
+        } else if (m < g.M) {
+          store8(c + m * g.ldc + n, z, left);
+        }
       }
+      if (!op) continue;
     }
 #pragma unroll
     for (int q = 0; q < ITER; ++q) {
-      const f32x4* p = reinterpret_cast<const f32x4*>(at + q * RPI * EROW);
-      const f32x4 v[2] = {p[0], p[1]};
-      float o[8];
+      const long m = mh + q * RPI;
+      float z[8];
+      read(z, q);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        o[j] = v[j / 4][j % 4];
-        if (EPI == kPlain) o[j] *= g.alpha;
+        if (EPI == kPlain) z[j] *= g.alpha;
         if (EPI == kForward && !curved)
-          o[j] = e.act.gain * (g.alpha * o[j] + bias[j]);
+          z[j] = e.act.gain * (g.alpha * z[j] + bias[j]);
+        if (EPI == kForward && op) z[j] += other[q][j];
+        if (EPI == kSlope) z[j] *= other[q][j];
       }
-      const long m = mh + q * RPI;
       if (m >= g.M) continue;
-      if (EPI == kForward && op) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] += other[q][j];
-      }
-      if (EPI == kSlope) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          o[j] *= other[q][j];
-          sums[j] += o[j];
-        }
-      }
-      // dz has padded rows, zero behind the last element
       if constexpr (EPI == kSlope) {
-        if (left) store8(c + m * g.ldc + n, o, 8);
-      } else if constexpr (EPI == kPartial)
-        store8(e.partial + (part * g.M + m) * g.N + n, o, left);
-      else
-        store8(c + m * g.ldc + n, o, left);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[j] += z[j];
+        // dz has padded rows, zero behind the last element
+        if (left) store8(c + m * g.ldc + n, z, 8);
+      } else if constexpr (EPI == kPartial) {
+        store8(e.partial + (part * g.M + m) * g.N + n, z, left);
+      } else {
+        store8(c + m * g.ldc + n, z, left);
+      }
     }
   }
   if (EPI == kSlope && e.partial) {
