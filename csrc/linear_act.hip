@@ -876,38 +876,48 @@ void linear_finish(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   finish.write(o, g, e, c);
 }
 
-// C = alpha * sum of the splits: 256 elements a block, 32 threads of eight
-// side by side, blockDim / 32 of them for every so manieth split
+// C = alpha * sum of the parts of k: eight elements a thread, the threads of
+// a block side by side or, for many parts, `groups` of them one above the
+// other, each for every so manieth part.
 template <typename T>
-__global__ __launch_bounds__(1024)
+__global__ __launch_bounds__(256)
 void sum_splits(T* __restrict__ c, const float* __restrict__ partial,
-                int splits, long count, float alpha) {
-  __shared__ float red[32][257];
-  const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const int groups = blockDim.x >> 5;
-  const long i0 = (long)blockIdx.x * 256, i = i0 + lane * 8;
+                int splits, long count, float alpha, int groups) {
+  __shared__ __attribute__((aligned(16))) float red[256 * 8];
+  const int wide = 256 / groups;
+  const int col = threadIdx.x % wide, q = threadIdx.x / wide;
+  const long i = ((long)blockIdx.x * wide + col) * 8;
   const int left = (int)max(0l, min(8l, count - i));
   float s[8] = {};
-  if (left) {
+  if (left == 8) {
 #pragma unroll 4
     for (int k = q; k < splits; k += groups) {
       Eight<float> v;
-      if (left == 8)
-        v.load(partial + k * count + i);
-      else
-        v.load(partial + k * count + i, left);
+      v.load(partial + k * count + i);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
     }
+  } else if (left) {
+    for (int k = q; k < splits; k += groups)
+      for (int j = 0; j < 8; ++j)
+        if (j < left) s[j] += partial[k * count + i + j];
+  }
+  if (groups > 1) {
+    f32x4* mine = reinterpret_cast<f32x4*>(red + threadIdx.x * 8);
+    mine[0] = f32x4{s[0], s[1], s[2], s[3]};
+    mine[1] = f32x4{s[4], s[5], s[6], s[7]};
+    __syncthreads();
+    if (q) return;
+    for (int g = 1; g < groups; ++g) {
+      const f32x4* v =
+          reinterpret_cast<const f32x4*>(red + (g * wide + col) * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j / 4][j % 4];
+    }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) red[q][lane * 8 + j] = s[j];
-  __syncthreads();
-  for (int k = threadIdx.x; k < 256 && i0 + k < count; k += blockDim.x) {
-    float v = 0.f;
-    for (int g = 0; g < groups; ++g) v += red[g][k];
-    put(c + i0 + k, alpha * v);
-  }
+  for (int j = 0; j < 8; ++j) s[j] *= alpha;
+  if (left) store8(c + i, s, left);
 }
 
 // dst[r][0..width) = src[r][0..n), zero behind: 16-byte rows for the tiles
@@ -1055,11 +1065,13 @@ void launch_split(T* c, const T* a, const T* b, GemmArgs g,
   launch_tile<T, ACOLS, BCOLS, kPartial>(tile, c, a, b, g, e, splits, s);
   if (EPI == kPlain) {
     const long count = g.M * g.N;
+    // a thread for every four parts, as long as there are threads to fill
     int groups = 1;
-    while (groups < 32 && groups * 4 < splits) groups *= 2;
-    hipLaunchKernelGGL(sum_splits<T>, dim3(ceil_div(count, 256)),
-                       dim3(32 * groups), 0, s, c, e.partial, splits, count,
-                       g.alpha);
+    while (groups < 64 && groups * 4 < splits && count / 8 * groups < 1 << 19)
+      groups *= 2;
+    hipLaunchKernelGGL(sum_splits<T>,
+                       dim3(ceil_div(count, 2048 / groups)), dim3(256), 0, s,
+                       c, e.partial, splits, count, g.alpha, groups);
   } else {
     hipLaunchKernelGGL((linear_finish<T, EPI>),
                        dim3(ceil_div(g.M * ((g.N + 3) / 4), 256)), dim3(256),
