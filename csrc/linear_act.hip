@@ -585,7 +585,7 @@ struct Finish4 {
       }
     }
     // dz has rows padded to eight, zero behind the last element
-    const long end = EPI == kSlope && left > 0 ? g.ldc - n : left;
+    const int end = EPI == kSlope ? (m < g.M ? (int)(g.ldc - n) : 0) : left;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j >= left) o[j] = 0.f;

@@ -460,15 +460,19 @@ def linear_inputs(dev, m, k, n, dtype, btype=F32):
             randn(m, n, device=dev, dtype=dtype, seed=3))
 
 
-def linear_grads(c, dev, dy=None):
+def linear_grads(c, dev, dy=None, poisoned=False):
     leaves = [t.detach().requires_grad_() for t in (c.x, c.w, c.b, c.res)
               if t is not None]
     it = iter(leaves)
     args = [next(it) if t is not None else None
             for t in (c.x, c.w, c.b, c.res)]
+    if poisoned:
+        poison(dev)
     y = linear_act(args[0], args[1], args[2], residual=args[3], **c.kw)
     c.check_forward(y.detach())
     dy = c.dy(torch.Generator(device=dev).manual_seed(9)) if dy is None else dy
+    if poisoned:
+        poison(dev)
     got = iter(torch.autograd.grad(y, leaves, dy))
     dx, dw = next(got), next(got)
     db = next(got) if c.b is not None else None
@@ -610,6 +614,42 @@ def test_linear_act_far_rows(dev):
     dx, dw = torch.autograd.grad(y, (x, w), dy)
     assert not dx[:-100].any()
     c.check_backward(dy[-100:], dx[-100:], dw)
+
+
+def poison(dev):
+    """Leaves NaN in the memory that the next tensors are made of."""
+    torch.cuda.synchronize()
+    sizes = [512 << i for i in range(11)] + [1 << 21, 1 << 23, 1 << 25]
+    held = [torch.full((size // 2,), math.nan, device=dev, dtype=BF16)
+            for size in sizes for _ in range(24 if size < 1 << 20 else 4)]
+    del held
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [3, 20, 41, 600, 2500])
+@pytest.mark.parametrize("n", [1, 3, 33, 50, 52, 113, 118, 127])
+@pytest.mark.parametrize("k", [49, 72, 1600])
+def test_linear_act_leaves_nothing_unwritten(dev, dtype, m, n, k):
+    """What lies behind the ends of rows in intermediate values does not
+    matter: widths of every rest modulo 8, over memory full of NaN."""
+    x, w, b, res = linear_inputs(dev, m, k, n, dtype)
+    linear_grads(Linear(x, w, b, res, "silu", wg=1 / math.sqrt(k)), dev,
+                 poisoned=True)
+    linear_grads(Linear(x, w, b, None, "linear", wg=1 / math.sqrt(k)), dev,
+                 poisoned=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [5, 64, 100, 1021, 2049, 20011])
+def test_layer_norm_leaves_nothing_unwritten(dev, n):
+    for rows in (1, 50, 700):
+        x, w, b, dy = ln_inputs(dev, rows, n, BF16)
+        poison(dev)
+        y = layer_norm(x, w, b)
+        poison(dev)
+        check_ln(x, w, b, dy,
+                 (y.detach(), *torch.autograd.grad(y, (x, w, b), dy)))
 
 
 # ---------------- together ----------------
