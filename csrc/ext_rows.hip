@@ -377,7 +377,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
   // a slope that is the same everywhere goes into the products: dz is dy
   const bool curved = p.curved(), again = curved && !z;
   const double slope = curved ? 1.0 : p.gain;
-  const bool small = gfa::linear_backward_is_small(m, n, k);
+  const bool small = gfa::linear_backward_is_small(
+      m, n, k, x.scalar_type() == torch::kFloat32);
   DISPATCH_FT(x.scalar_type(), {
     constexpr bool is_f32 = std::is_same_v<scalar_t, float>;
     Rows xr = rows_of(x), wr = rows_of(w), dr = rows_of(dy);
@@ -392,7 +393,10 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     int groups = 0;
     if (curved) {
       const int64_t width = (n + 7) / 8 * 8;  // zeros behind n
-      scalar_t* dz = dz_room.get<scalar_t>(m * width);
+      // few rows: also what rounding dz to bf16 took
+      const bool low = !is_f32 && any && small;
+      scalar_t* dz = dz_room.get<scalar_t>(m * width * (low ? 2 : 1));
+      if (low) e.dz_low = dz + m * width;
       const auto plan = gfa::linear_plan(m, n, k, is_f32, gfa::kSlopes);
       groups = again ? gfa::linear_row_tiles(plan, m)
                      : gfa::linear_dz_groups(m, (int)n);
@@ -407,9 +411,10 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
             {m, n, k, xr.stride, wr.stride, width, (float)p.weight_gain, k}, e,
             plan, cur_stream());
       } else {
-        gfa::launch_linear_dz<scalar_t>(dz, width, partial, rptr<scalar_t>(dr),
-                                        dr.stride, mptr<float>(z), e.act, m,
-                                        (int)n, cur_stream());
+        gfa::launch_linear_dz<scalar_t>(dz, e.dz_low, width, partial,
+                                        rptr<scalar_t>(dr), dr.stride,
+                                        mptr<float>(z), e.act, m, (int)n,
+                                        cur_stream());
       }
       dr.at = dz;
       dr.stride = width;
@@ -417,7 +422,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
       if (need_db && !small) {
         groups = gfa::linear_dz_groups(m, (int)n);
         partial = partial_room.get<float>(groups * n);
-        gfa::launch_linear_dz<scalar_t>(nullptr, 0, partial,
+        gfa::launch_linear_dz<scalar_t>(nullptr, nullptr, 0, partial,
                                         rptr<scalar_t>(dr), dr.stride, nullptr,
                                         e.act, m, (int)n, cur_stream());
       }
@@ -440,6 +445,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
       s.db_out = db ? db->data_ptr() : nullptr;
       s.db_f32 = db_f32;
       s.dz = rptr<scalar_t>(dr);
+      s.dz_low = e.dz_low;
       s.x = rptr<scalar_t>(xr);
       s.w = rptr<scalar_t>(wr);
       s.partial = partial;

@@ -589,7 +589,12 @@ struct Finish4 {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j >= left) o[j] = 0.f;
-      if (j < end) put(c + m * g.ldc + n + j, o[j]);
+      if (j < end) {
+        const auto raw = round_raw<T>(o[j]);
+        *reinterpret_cast<typename Raw<T>::type*>(c + m * g.ldc + n + j) = raw;
+        if (EPI == kSlope && e.dz_low)
+          put(e.dz_low + m * g.ldc + n + j, o[j] - raw_to_f32(raw));
+      }
     }
   }
 };
@@ -746,7 +751,7 @@ constexpr int kSmallLds = 4 * 2 * 2 * 32 * 128;  // stages, operands, depth
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
 GFA_DEV void small_block(char* lds, int block, const GemmArgs& g,
                          const EpilogueArgs<T>& e, T* c, const T* a,
-                         const T* b) {
+                         const T* b, const T* a_low = nullptr) {
   constexpr int B = 32, DEPTH = 2, STAGES = 4, WAVES = 4, FM = 2, FN = 2;
   using OA = Operand<T, B, ACOLS>;
   using F = Frag<T>;
@@ -763,35 +768,38 @@ GFA_DEV void small_block(char* lds, int block, const GemmArgs& g,
 
   using LA = Loader<T, B, ACOLS, WAVES, DEPTH>;
   using LB = Loader<T, B, BCOLS, WAVES, DEPTH>;
-  LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
-  LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
-  auto fetch = [&](int stage) {
-    load_a.fetch(lds + stage * kStage);
-    load_b.fetch(lds + stage * kStage + kHalf);
-  };
   f32x4 acc[2][2] = {};
   const int tiles = (kn + DEPTH * OA::BK - 1) / (DEPTH * OA::BK);
-#pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t) fetch(t);
   // a k-tile holds two steps, a stage four: one for each wave
   const int tile_of = wave / 2 * OA::kBytes, step = wave % 2;
-  for (int t = 0; t < tiles; ++t) {
-    wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
-    fetch((t + STAGES - 1) % STAGES);
-    const char* pa = lds + t % STAGES * kStage + tile_of;
-    const char* pb = pa + kHalf;
-    typename F::Type fa[2], fb[2];
+  for (const T* left = a; left; left = left == a ? a_low : nullptr) {
+    LA load_a(left, g.lda, m0, g.M, kb, kn, wave, lane);
+    LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
+    auto fetch = [&](int stage) {
+      load_a.fetch(lds + stage * kStage);
+      load_b.fetch(lds + stage * kStage + kHalf);
+    };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fa[i] = F::template read<B, ACOLS>(pa, i * 16, step, lane);
-      fb[i] = F::template read<B, BCOLS>(pb, i * 16, step, lane);
+    for (int t = 0; t < STAGES - 1; ++t) fetch(t);
+    for (int t = 0; t < tiles; ++t) {
+      wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
+      fetch((t + STAGES - 1) % STAGES);
+      const char* pa = lds + t % STAGES * kStage + tile_of;
+      const char* pb = pa + kHalf;
+      typename F::Type fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[i] = F::template read<B, ACOLS>(pa, i * 16, step, lane);
+        fb[i] = F::template read<B, BCOLS>(pb, i * 16, step, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
+    wait_pieces<0>();  // the next operand, or the sums, go where pieces went
   }
-  wait_pieces<0>();  // the sums go where the pieces went
   join_waves<T, EPI, FM, FN>(acc, lds, n0, mt, finish, g, e, c);
 }
 
@@ -838,13 +846,13 @@ void linear_backward_small(SmallBackward<T> p) {
   int block = blockIdx.x;
   if (block < p.dw_blocks) {
     small_block<T, true, true, kPlain>(lds, block, p.dw, none, p.dw_out, p.dz,
-                                       p.x);
+                                       p.x, p.dz_low);
     return;
   }
   block -= p.dw_blocks;
   if (block < p.dx_blocks) {
     small_block<T, false, true, kPlain>(lds, block, p.dx, none, p.dx_out, p.dz,
-                                        p.w);
+                                        p.w, p.dz_low);
     return;
   }
   block -= p.dx_blocks;
@@ -1116,8 +1124,8 @@ void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
 // by side, 256 / wide rows at a time, four of them under way.
 template <typename T>
 __global__ __launch_bounds__(256)
-void linear_dz_kernel(T* __restrict__ dz, long dz_stride,
-                      float* __restrict__ partial, const T* __restrict__ dy,
+void linear_dz_kernel(T* __restrict__ dz, T* __restrict__ low,
+                      long dz_stride, float* __restrict__ partial, const T* __restrict__ dy,
                       long dy_stride, const float* __restrict__ z,
                       ActParams act, long rows, int n, int wide) {
   constexpr int U = 4;
@@ -1161,6 +1169,13 @@ void linear_dz_kernel(T* __restrict__ dz, long dz_stride,
         for (int j = 0; j < 8; ++j) v[j] *= s[j];
         // padded rows, zero behind the last element
         store8(dz + (r + u * step) * dz_stride + i, v, 8);
+        if (low) {
+          float rest[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            rest[j] = v[j] - raw_to_f32(round_raw<T>(v[j]));
+          store8(low + (r + u * step) * dz_stride + i, rest, 8);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] += v[j];  // before their rounding
@@ -1197,22 +1212,25 @@ int linear_dz_groups(long rows, int n) {
 }
 
 template <typename T>
-void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
+void launch_linear_dz(T* dz, T* low, long dz_stride, float* partial,
+                      const T* dy,
                       long dy_stride, const float* z, const ActParams& act,
                       long rows, int n, hipStream_t s) {
   const int wide = dz_wide(n);
   hipLaunchKernelGGL(linear_dz_kernel<T>,
                      dim3(ceil_div(n, wide * 8), linear_dz_groups(rows, n)),
-                     dim3(256), 0, s, dz, dz_stride, partial, dy, dy_stride, z,
+                     dim3(256), 0, s, dz, low, dz_stride, partial, dy, dy_stride, z,
                      act, rows, n, wide);
 }
 
 // One launch where both products' tiles of 32 fit the card a few times over
-// and neither k is long.
-bool linear_backward_is_small(long m, long n, long k) {
+// and neither k is long. A few rows of bf16 go there from further off, for
+// the part of dz that rounding takes.
+bool linear_backward_is_small(long m, long n, long k, bool f32) {
   auto tiles = [](long a, long b) {
     return (long)ceil_div(a, 32) * ceil_div(b, 32);
   };
+  if (!f32 && linear_reads_any_rows(m)) return n <= 4096 && tiles(n, k) <= 4096;
   return m <= 1024 && n <= 2048 && tiles(m, k) <= 768 && tiles(n, k) <= 1024;
 }
 
@@ -1248,7 +1266,7 @@ void launch_linear_backward_small(SmallBackward<T> p, hipStream_t s) {
                                     hipStream_t);                            \
   template void launch_pad_rows<T>(const PadArgs<T>&, const PadArgs<T>&,     \
                                    hipStream_t);                             \
-  template void launch_linear_dz<T>(T*, long, float*, const T*, long,        \
+  template void launch_linear_dz<T>(T*, T*, long, float*, const T*, long,    \
                                     const float*, const ActParams&, long,    \
                                     int, hipStream_t);
 INSTANTIATE(float)

@@ -202,6 +202,7 @@ struct EpilogueArgs {
   const T* residual;  // forward: [M, N] with rows of res_stride, or null
   long res_stride;
   float* z;     // forward: [M, N] or null
+  T* dz_low;    // slope: what rounding took from dz, or null
   const T* dy;  // slope: [M, N] with rows of dy_stride
   long dy_stride;
   // slope: sums over the rows of each row of tiles, or null; with k in
@@ -243,14 +244,17 @@ struct SmallBackward {
   T *dw_out, *dx_out;
   void* db_out;
   bool db_f32;
-  const T *dz, *x, *w;
+  // dz and, unless null, what rounding took from it: the rounding errors of
+  // a few rows do not average out
+  const T *dz, *dz_low;
+  const T *x, *w;
   // db: db_scale times the sums of the groups of partial, or of dz's rows
   const float* partial;
   int groups, n;
   float db_scale;
   int dw_blocks, dx_blocks;
 };
-bool linear_backward_is_small(long m, long n, long k);
+bool linear_backward_is_small(long m, long n, long k, bool f32);
 template <typename T>
 void launch_linear_backward_small(SmallBackward<T> p, hipStream_t);
 
@@ -266,11 +270,13 @@ struct PadArgs {
 template <typename T>
 void launch_pad_rows(const PadArgs<T>& p0, const PadArgs<T>& p1, hipStream_t);
 
-// dz = dy * slope(z) (z and dz null: dz = dy) and, unless partial is null,
+// dz = dy * slope(z) (z and dz null: dz = dy), low (or null) what rounding
+// took from it, and, unless partial is null,
 // partial[g][n] = sums of dz over the rows of group g
 int linear_dz_groups(long rows, int n);
 template <typename T>
-void launch_linear_dz(T* dz, long dz_stride, float* partial, const T* dy,
+void launch_linear_dz(T* dz, T* low, long dz_stride, float* partial,
+                      const T* dy,
                       long dy_stride, const float* z, const ActParams& act,
                       long rows, int n, hipStream_t s);
 
