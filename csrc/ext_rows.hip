@@ -165,7 +165,8 @@ void check_layer_norm(const Tensor& x, const OptTensor& w,
             ": weight is ", w->scalar_type(), ", bias ", b->scalar_type());
 }
 
-std::tuple<Tensor, OptTensor, OptTensor> layer_norm_fwd(
+// y and, if they are to be kept, the means and the 1 / deviations [2, rows]
+std::tuple<Tensor, OptTensor> layer_norm_fwd(
     const Tensor& x, const OptTensor& w, const OptTensor& b, double eps,
     bool save) {
   const int n = (int)x.size(-1);
@@ -175,27 +176,26 @@ std::tuple<Tensor, OptTensor, OptTensor> layer_norm_fwd(
   const OptTensor bc = b ? OptTensor(b->contiguous()) : b;
   const Rows xr = rows_of(x);
   Tensor y = new_tensor(x.sizes(), x.scalar_type(), x);
-  OptTensor mean, rstd;
+  OptTensor stats;
   if (save) {
-    mean = new_tensor({xr.count}, torch::kFloat32, x);
-    rstd = new_tensor({xr.count}, torch::kFloat32, x);
+    stats = new_tensor({2, xr.count}, torch::kFloat32, x);
   }
   if (xr.count > 0) {
     DISPATCH_TP(x, p32, {
       gfa::launch_layer_norm_fwd<T, P>(
-          static_cast<T*>(y.data_ptr()), mptr<float>(mean), mptr<float>(rstd),
+          static_cast<T*>(y.data_ptr()), mptr<float>(stats),
+          save ? mptr<float>(stats) + xr.count : nullptr,
           rptr<T>(xr), xr.stride, cptr<P>(wc), cptr<P>(bc), xr.count, n,
           (float)eps, cur_stream());
     });
     HIP_CHECK_LAST();
   }
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
 std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
     const Tensor& dy, const Tensor& x, const OptTensor& w, const OptTensor& b,
-    const Tensor& mean, const Tensor& rstd, bool need_dx, bool need_dw,
-    bool need_db) {
+    const Tensor& stats, bool need_dx, bool need_dw, bool need_db) {
   TORCH_CHECK(dy.device() == x.device() && dy.sizes() == x.sizes() &&
                   dy.scalar_type() == x.scalar_type(),
               "layer_norm: dy does not fit x");
@@ -215,14 +215,17 @@ std::tuple<OptTensor, OptTensor, OptTensor> layer_norm_bwd(
     if (need_db) db->zero_();
     return {dx, dw, db};
   }
-  const int64_t groups = gfa::layer_norm_bwd_groups(
-      xr.count, n, x.scalar_type() == torch::kFloat32);
-  float* sums = partial.get<float>(need_dw || need_db ? 2 * groups * n : 0);
+  const bool f32 = x.scalar_type() == torch::kFloat32;
+  const bool by_sums = (need_dw || need_db) &&
+                       gfa::layer_norm_bwd_sums(xr.count, n, f32);
+  const int64_t groups = gfa::layer_norm_bwd_groups(xr.count, n, f32);
+  float* sums = partial.get<float>(by_sums ? 2 * groups * n : 0);
   DISPATCH_TP(x, p32, {
     gfa::launch_layer_norm_bwd<T, P>(
         mptr<T>(dx), mptr<P>(dw), mptr<P>(db), sums,
         rptr<T>(dr), dr.stride, rptr<T>(xr), xr.stride, cptr<P>(wc),
-        cptr<float>(mean), cptr<float>(rstd), xr.count, n, cur_stream());
+        cptr<float>(stats), cptr<float>(stats) + xr.count, xr.count, n,
+        cur_stream());
   });
   HIP_CHECK_LAST();
   return {dx, dw, db};
@@ -535,8 +538,8 @@ Tensor composed_layer_norm(const variable_list& in, double eps) {
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x,
                         const OptTensor& w, const OptTensor& b, double eps) {
-    auto [y, mean, rstd] = layer_norm_fwd(x, w, b, eps, true);
-    ctx->save_for_backward({x, plain(w), plain(b), *mean, *rstd});
+    auto [y, stats] = layer_norm_fwd(x, w, b, eps, true);
+    ctx->save_for_backward({x, plain(w), plain(b), *stats});
     ctx->saved_data["eps"] = eps;
     return y;
   }
@@ -553,7 +556,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       return out;
     }
     const auto [dx, dw, db] =
-        layer_norm_bwd(dy[0], s[0], opt(s[1]), opt(s[2]), s[3], s[4], need[0],
+        layer_norm_bwd(dy[0], s[0], opt(s[1]), opt(s[2]), s[3], need[0],
                        need[1], need[2]);
     return {plain(dx), plain(dw), plain(db), Tensor()};
   }

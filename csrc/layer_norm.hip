@@ -200,12 +200,46 @@ void layer_norm_fwd_rows(T* __restrict__ y, float* __restrict__ mean,
   }
 }
 
+// dw and db of eight columns from n0 on, all rows, by a block of its own
+template <typename T, typename P, int THREADS>
+GFA_DEV void layer_norm_columns(P* dw, P* db, const T* dy, long dy_stride,
+                                const T* x, long x_stride, const float* mean,
+                                const float* rstd, long rows, int n, int n0) {
+  constexpr int Q = THREADS / 8;
+  __shared__ float red[2][8][Q + 1];
+  const int c = threadIdx.x & 7, q = threadIdx.x >> 3, i = n0 + c;
+  float sw = 0.f, sb = 0.f;
+  if (i < n) {
+#pragma unroll 4
+    for (long r = q; r < rows; r += Q) {
+      const float d = to_f32(dy[r * dy_stride + i]);
+      sw += d * (to_f32(x[r * x_stride + i]) - mean[r]) * rstd[r];
+      sb += d;
+    }
+  }
+  red[0][c][q] = sw;
+  red[1][c][q] = sb;
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    const int k = threadIdx.x >> 3;
+    P* out = k ? db : dw;
+    if (!out || i >= n) return;
+    float s = 0.f;
+    for (int g = 0; g < Q; ++g) s += red[k][c][g];
+    put(out + i, s);
+  }
+}
+
 // One pass over x and dy: dx, and the block's sums over its rows of dy * xn
 // and dy for the parameters, held in registers until the rows are through.
+// Where the rows are few, blocks behind the first row_blocks make dw and db
+// instead, from x and dy again: one launch where the sums of blocks take two.
 template <typename T, typename P, int WAVES, int V, int E, bool TAIL>
 __global__ __launch_bounds__(WAVES == 16 ? 1024 : 256)
 void layer_norm_bwd_rows(T* __restrict__ dx, float* __restrict__ partial,
-                         const T* __restrict__ dy, long dy_stride,
+                         P* __restrict__ dw, P* __restrict__ db,
+                         int row_blocks, const T* __restrict__ dy,
+                         long dy_stride,
                          const T* __restrict__ x, long x_stride,
                          const P* __restrict__ w,
                          const float* __restrict__ mean,
@@ -214,6 +248,12 @@ void layer_norm_bwd_rows(T* __restrict__ dx, float* __restrict__ partial,
   constexpr int kThreads = WAVES == 16 ? 1024 : 256;
   // a row ahead, except where its registers would spill
   constexpr bool kAhead = WAVES < 16 || E < 16;
+  if ((int)blockIdx.x >= row_blocks) {
+    layer_norm_columns<T, P, kThreads>(dw, db, dy, dy_stride, x, x_stride,
+                                       mean, rstd, rows, n,
+                                       (blockIdx.x - row_blocks) * 8);
+    return;
+  }
   __shared__ float red[WAVES > 1 ? 4 * WAVES : 1];
   // sums of the waves of a block, where they hold the same columns
   __shared__ float sums[WAVES == 1 ? kThreads * E : 1];
@@ -226,7 +266,7 @@ void layer_norm_bwd_rows(T* __restrict__ dx, float* __restrict__ partial,
   lane.params(wv, w, 1.f);
 #pragma unroll
   for (int e = 0; e < E; ++e) aw[e] = ab[e] = 0.f;
-  const long step = (long)gridDim.x * per_block;
+  const long step = (long)row_blocks * per_block;
   typename Raw<T>::type next_x[E], next_d[E];
   float next_mu, next_rs;
   auto load = [&](long r) {
@@ -273,7 +313,7 @@ void layer_norm_bwd_rows(T* __restrict__ dx, float* __restrict__ partial,
   }
   if (!partial) return;
   float* pw = partial + (long)blockIdx.x * n;
-  float* pb = partial + ((long)gridDim.x + blockIdx.x) * n;
+  float* pb = partial + ((long)row_blocks + blockIdx.x) * n;
   if constexpr (WAVES > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
@@ -529,6 +569,11 @@ int layer_norm_bwd_groups(long rows, int n, bool f32) {
   return (int)(blocks < most ? blocks : most);
 }
 
+// Rows that dw and db take again instead of leaving sums of blocks.
+bool layer_norm_bwd_sums(long rows, int n, bool f32) {
+  return rows > 1024 || !(f32 ? row_plan<float>(n) : row_plan<bf16>(n)).waves;
+}
+
 template <typename T, typename P>
 void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
                            long dy_stride, const T* x, long x_stride,
@@ -536,12 +581,15 @@ void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
                            long rows, int n, hipStream_t s) {
   const RowPlan p = row_plan<T>(n);
   const int groups = layer_norm_bwd_groups(rows, n, sizeof(T) == 4);
+  const bool columns = !partial && (dw || db);
   if (p.waves) {
+    const int blocks = (dx || partial ? groups : 0);
+    const int grid = blocks + (columns ? ceil_div(n, 8) : 0);
     with_plan<T, false>(p, [&](auto waves, auto v, auto e, auto tail) {
       hipLaunchKernelGGL(
-          (layer_norm_bwd_rows<T, P, waves(), v(), e(), tail()>), dim3(groups),
-          dim3(waves() == 16 ? 1024 : 256), 0, s, dx, partial, dy, dy_stride,
-          x, x_stride, w, mean, rstd, rows, n, p.lanes);
+          (layer_norm_bwd_rows<T, P, waves(), v(), e(), tail()>), dim3(grid),
+          dim3(waves() == 16 ? 1024 : 256), 0, s, dx, partial, dw, db, blocks,
+          dy, dy_stride, x, x_stride, w, mean, rstd, rows, n, p.lanes);
     });
   } else {
     if (dx) {
@@ -556,7 +604,7 @@ void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
                          partial, dy, dy_stride, x, x_stride, mean, rstd,
                          rows, n);
   }
-  if (dw || db)
+  if (partial)
     launch_sum_groups<P>(dw, db, partial, groups, n, 1.f, s);
 }
 

@@ -171,7 +171,9 @@ template <typename T, typename P>
 void launch_layer_norm_fwd(T* y, float* mean, float* rstd, const T* x,
                            long x_stride, const P* w, const P* b, long rows,
                            int n, float eps, hipStream_t);
-// partial: [2][groups][n] floats; dx, dw, db null if not wanted
+// dx, dw, db null if not wanted. partial: [2][groups][n] floats, where dw and
+// db go by sums of blocks and one is wanted; else null.
+bool layer_norm_bwd_sums(long rows, int n, bool f32);
 int layer_norm_bwd_groups(long rows, int n, bool f32);
 template <typename T, typename P>
 void launch_layer_norm_bwd(T* dx, P* dw, P* db, float* partial, const T* dy,
