@@ -243,6 +243,8 @@ void check_linear(const Tensor& x, const Tensor& w, const OptTensor& bias,
             w.sizes());
   CHECK_ARG(w.size(0) < (1 << 20) && w.size(1) < (1 << 20), op,
             ": weight of ", w.sizes(), ": sizes below 2^20 are served");
+  CHECK_ARG(x.numel() / x.size(-1) < (1l << 30), op, ": x ", x.sizes(),
+            ": fewer than 2^30 rows are served");
   check_device(w, x, op, "weight");
   CHECK_ARG(w.scalar_type() == x.scalar_type(), op, ": weight is ",
             w.scalar_type(), ", x ", x.scalar_type());
@@ -489,7 +491,9 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+OptTensor opt(const Tensor& t) {
+  return t.defined() ? OptTensor(t) : OptTensor();
+}
 Tensor plain(const OptTensor& t) { return t ? *t : Tensor(); }
 bool wants_grad(const OptTensor& t) { return t && t->requires_grad(); }
 

@@ -569,9 +569,11 @@ int layer_norm_bwd_groups(long rows, int n, bool f32) {
   return (int)(blocks < most ? blocks : most);
 }
 
-// Rows that dw and db take again instead of leaving sums of blocks.
+// Whether dw and db go by sums of blocks: not where x and dy are so small that
+// reading them again, eight columns a block, is less than a launch.
 bool layer_norm_bwd_sums(long rows, int n, bool f32) {
-  return rows > 1024 || !(f32 ? row_plan<float>(n) : row_plan<bf16>(n)).waves;
+  const RowPlan p = f32 ? row_plan<float>(n) : row_plan<bf16>(n);
+  return rows > 1024 || rows * n > 1 << 21 || !p.waves;
 }
 
 template <typename T, typename P>

@@ -224,7 +224,8 @@ bool linear_reads_any_rows(long M);
 // y = clamp(act(alpha x W^T + bias) * gain) + residual
 template <typename T>
 void launch_linear_forward(T* y, const T* x, const T* w, const GemmArgs& g,
-                           const EpilogueArgs<T>& e, const LinearPlan&, hipStream_t);
+                           const EpilogueArgs<T>& e, const LinearPlan&,
+                           hipStream_t);
 // dz = dy * slope(alpha x W^T + bias); linear_row_tiles sums of rows
 int linear_row_tiles(const LinearPlan&, long M);
 template <typename T>

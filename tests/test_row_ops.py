@@ -96,7 +96,8 @@ def act_parts(z, act):
     if act == "relu":
         return z.clamp_min(0), (z > 0).double()
     if act == "lrelu":
-        return torch.where(z > 0, z, 0.2 * z), torch.where(z > 0, 1.0, 0.2).to(z)
+        return (torch.where(z > 0, z, 0.2 * z),
+                torch.where(z > 0, 1.0, 0.2).to(z))
     if act == "tanh":
         return z.tanh(), 1 - z.tanh() ** 2
     if act == "sigmoid":
