@@ -28,9 +28,14 @@ using LdsPtr = __attribute__((address_space(3))) void*;
 // the buffer descriptor), so any M, N, K take this path as long as rows are
 // 16-byte aligned.
 //
+// What bounds it: float the matrix cores (busy 94% of the time at 4096^3, 146
+// TFLOP/s); bf16 8192x4096x4096 keeps them busy 61% (1136 TFLOP/s; a copy of
+// the operands and the result would take 32 us); a short k leaves a tile's
+// 128 KB of results, 9 us of its 23 us at k = 512.
+//
 // LDS layout. Rows: [m][128 bytes], 16-byte granule g of row r at g ^ (r/2
 // mod 8), so that the 16 rows a fragment read touches spread over all 64
-// banks. Columns: [k][BX], granules of row k exchanged likewise; bf16
+// banks (conflicts: 2% of the LDS's busy cycles). Columns: [k][BX], granules of row k exchanged likewise; bf16
 // fragments come out of it through the transposing LDS read.
 template <typename T, int BX, bool COLS>
 struct Operand {
@@ -272,15 +277,19 @@ struct Loader {
   }
 };
 
-// One step's instructions in the order written in linear_tile: for each row
-// of fragments its products, then the LDS reads for the next step.
-template <int FM, int FN, int MFMAS, int READS_A, int READS_B, int... I>
+// One step's instructions in the order that linear_tile wants: for each row of
+// fragments its products, then the LDS reads for the next step and its share
+// of the PIECES fetched (dx of 8192x4096x4096 bf16: 265 us, 283 us with all
+// pieces asked for at once).
+template <int FM, int FN, int MFMAS, int READS_A, int READS_B, int PIECES,
+          int... I>
 GFA_DEV void order(std::integer_sequence<int, I...>) {
-  constexpr int kMfma = 0x8, kLdsRead = 0x100;
+  constexpr int kMfma = 0x8, kVmemRead = 0x20, kLdsRead = 0x100;
   ((__builtin_amdgcn_sched_group_barrier(kMfma, FN * MFMAS, 0),
     __builtin_amdgcn_sched_group_barrier(
         kLdsRead,
-        ((I + 1) * FN / FM - I * FN / FM) * READS_B + READS_A, 0)),
+        ((I + 1) * FN / FM - I * FN / FM) * READS_B + READS_A, 0),
+    __builtin_amdgcn_sched_group_barrier(kVmemRead, PIECES / FM, 0)),
    ...);
 }
 
@@ -351,8 +360,9 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     // One block a CU: while one of a k-tile's two steps is multiplied, the
     // fragments of the next are read, a row's as soon as the row before it is
     // done with, and the k-tile after next is fetched into the half that was
-    // read last (8192x4096x4096 bf16: 247 us, 263 us as below).
-    auto multiply = [&](const Frags& f, Frags& next, int stage, int step) {
+    // read last (8192x4096x4096 bf16: 242 us, 263 us as below).
+    auto multiply = [&](const Frags& f, Frags& next, int stage, int step,
+                        auto pieces) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -364,8 +374,10 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
         read_a(next, stage, step, i);
       }
       order<FM, FN, F::kMfmas, ACOLS ? F::kColReads : 1,
-            BCOLS ? F::kColReads : 1>(std::make_integer_sequence<int, FM>{});
+            BCOLS ? F::kColReads : 1, pieces()>(
+          std::make_integer_sequence<int, FM>{});
     };
+    constexpr int kPieces = LA::kPieces + LB::kPieces;
     fetch(0);
     fetch(1);
     wait_pieces<LA::kPieces + LB::kPieces>();
@@ -375,10 +387,11 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 #pragma unroll
     for (int i = 0; i < FM; ++i) read_a(f0, 0, 0, i);
     for (int t = 0; t < tiles; ++t) {
-      multiply(f0, f1, t & 1, 1);
+      multiply(f0, f1, t & 1, 1, std::integral_constant<int, 0>{});
       wait_pieces<0>();
       fetch(t & 1);
-      multiply(f1, f0, (t + 1) & 1, 0);
+      multiply(f1, f0, (t + 1) & 1, 0,
+               std::integral_constant<int, kPieces>{});
     }
   } else {
     // Several blocks a CU fill each other's gaps, and a simple order leaves
@@ -971,7 +984,7 @@ namespace {
 
 // Microseconds that a CU spends on one k-tile of a block, alone on it or with
 // others, and on the rest of a block's work. Measured: 8192x4096x4096 bf16
-// takes 247, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 955,
+// takes 242, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 940,
 // 1021 and 1089 us; 524288x128x128 bf16, half of whose tiles of 256 would be
 // padding, 120 us with those and 48 us with 128. Of 21 shapes and up to 40
 // ways to cut each, in both types, what the figures choose is within 5% of
