@@ -251,36 +251,41 @@ struct Loader {
       offset[i] = O::source((i * WAVES + wave) * 64 + lane, (int)stride);
   }
 
-  // The next DEPTH k-tiles. Past the end nothing is read and zeros arrive,
-  // so the counts of pieces under way stay what the waits expect.
+  // A piece of the next k-tile, the i-th of this wave. Past the end nothing is
+  // read and zeros arrive, so the counts of pieces under way stay what the
+  // waits expect.
+  GFA_DEV void piece(char* lds, int i) const {
+    int off = offset[i];
+    if constexpr (!COLS) {
+      // rows: the last k-tile is cut off at the end of k
+      const int idx = (i * WAVES + wave) * 64 + lane;
+      const int k = ((idx & 7) ^ O::swizzle(idx >> 3)) * (16 / ES);
+      if (left < BK && k >= left) off = 0x7ffffff8;
+    }
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        buffer_at(at, bytes), (LdsPtr)(lds + (i * WAVES + wave) * 1024), 16,
+        off, 0, 0, 0);
+  }
+  GFA_DEV void advance() {
+    at += step;
+    bytes -= step;
+    left -= BK;
+  }
+
+  // the next DEPTH k-tiles
   GFA_DEV void fetch(char* lds) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const auto rsrc = buffer_at(at, bytes);
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        int off = offset[i];
-        if constexpr (!COLS) {
-          // rows: the last k-tile is cut off at the end of k
-          const int idx = (i * WAVES + wave) * 64 + lane;
-          const int k = ((idx & 7) ^ O::swizzle(idx >> 3)) * (16 / ES);
-          if (left < BK && k >= left) off = 0x7ffffff8;
-        }
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsrc, (LdsPtr)(lds + (d * kTile + i * WAVES + wave) * 1024), 16,
-            off, 0, 0, 0);
-      }
-      at += step;
-      bytes -= step;
-      left -= BK;
+      for (int i = 0; i < kEach; ++i) piece(lds + d * kTile * 1024, i);
+      advance();
     }
   }
 };
 
 // One step's instructions in the order that linear_tile wants: for each row of
 // fragments its products, then the LDS reads for the next step and its share
-// of the PIECES fetched (dx of 8192x4096x4096 bf16: 265 us, 283 us with all
-// pieces asked for at once).
+// of the PIECES fetched.
 template <int FM, int FN, int MFMAS, int READS_A, int READS_B, int PIECES,
           int... I>
 GFA_DEV void order(std::integer_sequence<int, I...>) {
@@ -340,6 +345,13 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     load_b.fetch(lds + stage * kStage + OA::kBytes);
   };
 
+  auto piece = [&](char* to, int p) {
+    if (p < LA::kEach)
+      load_a.piece(to, p);
+    else
+      load_b.piece(to + OA::kBytes, p - LA::kEach);
+  };
+
   const int wm = wave / WN * TM, wn = wave % WN * TN;
   f32x4 acc[FM][FN] = {};
   const int tiles = (kn + BK - 1) / BK;
@@ -348,21 +360,23 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   struct Frags {
     typename F::Type a[FM], b[FN];
   };
-  auto read_a = [&](Frags& f, int stage, int step, int i) {
-    f.a[i] = F::template read<BM, ACOLS>(lds + stage * kStage, wm + i * 16,
-                                         step, lane);
+  auto read_a = [&](Frags& f, const char* from, int step, int i) {
+    f.a[i] = F::template read<BM, ACOLS>(from, wm + i * 16, step, lane);
   };
-  auto read_b = [&](Frags& f, int stage, int step, int j) {
-    f.b[j] = F::template read<BN, BCOLS>(lds + stage * kStage + OA::kBytes,
-                                         wn + j * 16, step, lane);
+  auto read_b = [&](Frags& f, const char* from, int step, int j) {
+    f.b[j] = F::template read<BN, BCOLS>(from + OA::kBytes, wn + j * 16, step,
+                                         lane);
   };
   if constexpr (BM == 256) {
     // One block a CU: while one of a k-tile's two steps is multiplied, the
     // fragments of the next are read, a row's as soon as the row before it is
     // done with, and the k-tile after next is fetched into the half that was
-    // read last (8192x4096x4096 bf16: 242 us, 263 us as below).
-    auto multiply = [&](const Frags& f, Frags& next, int stage, int step,
-                        auto pieces) {
+    // read last (8192x4096x4096 bf16: 234 us, 263 us as below).
+    constexpr int kPieces = LA::kPieces + LB::kPieces;
+    Frags f0, f1;
+    // next: the step's fragments in `from`; pieces go to `to`
+    auto multiply = [&](const Frags& f, Frags& next, const char* from,
+                        int step, char* to, auto pieces) {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -370,49 +384,72 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
           acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
 #pragma unroll
         for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
-          read_b(next, stage, step, j);
-        read_a(next, stage, step, i);
+          read_b(next, from, step, j);
+        read_a(next, from, step, i);
+        if (pieces())
+#pragma unroll
+          for (int p = i * kPieces / FM; p < (i + 1) * kPieces / FM; ++p)
+            piece(to, p);
       }
       order<FM, FN, F::kMfmas, ACOLS ? F::kColReads : 1,
             BCOLS ? F::kColReads : 1, pieces()>(
           std::make_integer_sequence<int, FM>{});
     };
-    constexpr int kPieces = LA::kPieces + LB::kPieces;
+    // A k-tile's second step and the next one's first. Where the compiler
+    // cannot tell that no piece goes to where fragments are read, it lets
+    // transposed reads wait for all pieces under way (8192x4096x4096 bf16: dx
+    // 235 us, 267 us so; dw 216 us, 245 us so).
+    auto both = [&](const char* __restrict__ from, char* __restrict__ to) {
+      multiply(f1, f0, from, 0, to, std::integral_constant<int, kPieces>{});
+      load_a.advance();
+      load_b.advance();
+      multiply(f0, f1, from, 1, nullptr, std::integral_constant<int, 0>{});
+    };
     fetch(0);
     fetch(1);
-    wait_pieces<LA::kPieces + LB::kPieces>();
-    Frags f0, f1;
+    wait_pieces<kPieces>();
 #pragma unroll
-    for (int j = 0; j < FN; ++j) read_b(f0, 0, 0, j);
+    for (int j = 0; j < FN; ++j) read_b(f0, lds, 0, j);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) read_a(f0, 0, 0, i);
-    for (int t = 0; t < tiles; ++t) {
-      multiply(f0, f1, t & 1, 1, std::integral_constant<int, 0>{});
+    for (int i = 0; i < FM; ++i) read_a(f0, lds, 0, i);
+    multiply(f0, f1, lds, 1, nullptr, std::integral_constant<int, 0>{});
+    for (int t = 1; t < tiles; ++t) {
       wait_pieces<0>();
-      fetch(t & 1);
-      multiply(f1, f0, (t + 1) & 1, 0,
-               std::integral_constant<int, kPieces>{});
+      both(lds + (t & 1) * kStage, lds + (~t & 1) * kStage);
     }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = F::mma(f1.b[j], f1.a[i], acc[i][j]);
   } else {
     // Several blocks a CU fill each other's gaps, and a simple order leaves
-    // them the registers (dw of 65536x512x2048: 176 us, 250 us as above).
-    fetch(0);
-    for (int t = 0; t < tiles; ++t) {
-      wait_pieces<0>();
-      if (t + 1 < tiles) fetch((t + 1) & 1);
+    // them the registers (524288x128x128 bf16: dx 52 us, 56 us as above).
+    auto multiply = [&](const char* __restrict__ from, char* __restrict__ to,
+                        bool more) {
+      if (more) {
+        load_a.fetch(to);
+        load_b.fetch(to + OA::kBytes);
+      }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         Frags f;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) read_b(f, t & 1, s, j);
+        for (int j = 0; j < FN; ++j) read_b(f, from, s, j);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) read_a(f, t & 1, s, i);
+        for (int i = 0; i < FM; ++i) read_a(f, from, s, i);
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int j = 0; j < FN; ++j)
             acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
       }
+    };
+    fetch(0);
+    for (int t = 0; t < tiles; ++t) {
+      wait_pieces<0>();
+      multiply(lds + (t & 1) * kStage, lds + (~t & 1) * kStage,
+               t + 1 < tiles);
     }
   }
   wait_pieces<0>();  // the epilogue writes where the pieces go
@@ -798,12 +835,10 @@ GFA_DEV void small_block(char* lds, int block, const GemmArgs& g,
       load_a.fetch(lds + stage * kStage);
       load_b.fetch(lds + stage * kStage + kHalf);
     };
-#pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) fetch(t);
-    for (int t = 0; t < tiles; ++t) {
-      wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
-      fetch((t + STAGES - 1) % STAGES);
-      const char* pa = lds + t % STAGES * kStage + tile_of;
+    auto multiply = [&](const char* __restrict__ from, char* __restrict__ to) {
+      load_a.fetch(to);
+      load_b.fetch(to + kHalf);
+      const char* pa = from + tile_of;
       const char* pb = pa + kHalf;
       typename F::Type fa[2], fb[2];
 #pragma unroll
@@ -816,6 +851,13 @@ GFA_DEV void small_block(char* lds, int block, const GemmArgs& g,
 #pragma unroll
         for (int j = 0; j < 2; ++j)
           acc[i][j] = F::mma(fb[j], fa[i], acc[i][j]);
+    };
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) fetch(t);
+    for (int t = 0; t < tiles; ++t) {
+      wait_pieces<(STAGES - 2) * (LA::kPieces + LB::kPieces)>();
+      multiply(lds + t % STAGES * kStage,
+               lds + (t + STAGES - 1) % STAGES * kStage);
     }
     wait_pieces<0>();  // the next operand, or the sums, go where pieces went
   }
@@ -984,7 +1026,7 @@ namespace {
 
 // Microseconds that a CU spends on one k-tile of a block, alone on it or with
 // others, and on the rest of a block's work. Measured: 8192x4096x4096 bf16
-// takes 242, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 940,
+// takes 234, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 940,
 // 1021 and 1089 us; 524288x128x128 bf16, half of whose tiles of 256 would be
 // padding, 120 us with those and 48 us with 128. Of 21 shapes and up to 40
 // ways to cut each, in both types, what the figures choose is within 5% of
@@ -995,7 +1037,7 @@ struct TileCost {
 };
 const TileCost kTileCosts[2][5] = {
     // bf16
-    {{256, 1.9, 1.9, 8}, {128, 0.95, 0.61, 2}, {64, 0.40, 0.214, 1},
+    {{256, 1.7, 1.7, 8}, {128, 0.77, 0.57, 2}, {64, 0.40, 0.214, 1},
      {32, 0.2, 0.12, 0.5}, {16, 0.06, 0.05, 0.5}},
     // float
     {{256, 7.4, 7.4, 8}, {128, 2.15, 2.0, 2}, {64, 0.65, 0.53, 1},
@@ -1060,7 +1102,6 @@ LinearPlan linear_plan(long M, long N, long K, bool f32, LinearKind kind) {
       const long rounds = (blocks * s + 255) / 256;
       double cost = rounds == 1 ? each * t.alone + t.rest
                                 : rounds * (each * t.shared + t.rest);
-      if (kind == kWeights && t.side == 256 && !f32) cost *= 1.15;
       if (s > 1) cost += 3 + 2e-6 * s * M * N;
       if (cost < least) {
         least = cost;
