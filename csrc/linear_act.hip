@@ -211,6 +211,11 @@ GFA_DEV void wait_pieces() {
                : "memory");
 }
 
+// waits for the block's waves to be done with LDS
+GFA_DEV void wait_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 GFA_DEV auto buffer_at(const void* p, long bytes) {
   const long most = 0x7ffffff0;
   return __builtin_amdgcn_make_buffer_rsrc(
@@ -237,6 +242,7 @@ struct Loader {
   int offset[kEach];
 
   // x0: first row (column) of the tile, X: all of them; kb, kn: part of k
+  Loader() = default;
   GFA_DEV Loader(const T* p, long stride, long x0, long X, long kb, int kn,
                  int wave_, int lane_)
       : left(kn), wave(wave_), lane(lane_) {
@@ -298,167 +304,21 @@ GFA_DEV void order(std::integer_sequence<int, I...>) {
    ...);
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool ACOLS, bool BCOLS,
-          int EPI>
-__global__ __launch_bounds__(WM * WN * 64)
-void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
-                 const T* __restrict__ a, const T* __restrict__ b) {
-  using OA = Operand<T, BM, ACOLS>;
-  using OB = Operand<T, BN, BCOLS>;
-  using F = Frag<T>;
-  constexpr int BK = OA::BK, WAVES = WM * WN;
-  constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  constexpr int kStage = OA::kBytes + OB::kBytes;
-  // the epilogue turns so many rows of a wave at a time in LDS
-  constexpr int ROWS = 32;
-  constexpr int EROW = TN * 4 + 16;
-  constexpr int kEpi = WAVES * ROWS * EROW;
-  constexpr int kLds = 2 * kStage > kEpi ? 2 * kStage : kEpi;
-  __shared__ __attribute__((aligned(16))) char lds[kLds];
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-  // Work: an XCD's blocks (every eighth) take neighbouring tiles of one part
-  // of k, in groups of 4 rows of tiles, so that they share operands in its
-  // L2 (all tiles of a part, where there are few).
-  const int tm = (int)((g.M + BM - 1) / BM), tn = (int)((g.N + BN - 1) / BN);
-  const int parts = (int)((g.K + g.k_split - 1) / g.k_split);
-  const int total = tm * tn * parts, per = (total + 7) / 8;
-  const int work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || work >= total) return;
-  const int part = work / (tm * tn), tile = work - part * tm * tn;
-  const int group = tile / (4 * tn), in_group = tile - group * 4 * tn;
-  const int rows = min(4, tm - group * 4);
-  const int mt = group * 4 + in_group % rows;
+constexpr int kEpilogueRows = 32;
+// Block's results, that of work m0, n0 (row mt of tiles) and part
+template <typename T, int BM, int BN, int WM, int WN, int EPI>
+GFA_DEV void tile_epilogue(const f32x4 (&acc)[BM / WM / 16][BN / WN / 16],
+                           char* lds, int wave, int lane, int mt, long n0,
+                           int part, const GemmArgs& g,
+                           const EpilogueArgs<T>& e, T* c) {
+  constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN, FN = TN / 16;
   const long m0 = (long)mt * BM;
-  const long n0 = (long)(in_group / rows) * BN;
-  const long kb = part * g.k_split;
-  const int kn = (int)min(g.K - kb, g.k_split);
-
-  using LA = Loader<T, BM, ACOLS, WAVES, 1>;
-  using LB = Loader<T, BN, BCOLS, WAVES, 1>;
-  LA load_a(a, g.lda, m0, g.M, kb, kn, wave, lane);
-  LB load_b(b, g.ldb, n0, g.N, kb, kn, wave, lane);
-  auto fetch = [&](int stage) {
-    load_a.fetch(lds + stage * kStage);
-    load_b.fetch(lds + stage * kStage + OA::kBytes);
-  };
-
-  auto piece = [&](char* to, int p) {
-    if (p < LA::kEach)
-      load_a.piece(to, p);
-    else
-      load_b.piece(to + OA::kBytes, p - LA::kEach);
-  };
-
   const int wm = wave / WN * TM, wn = wave % WN * TN;
-  f32x4 acc[FM][FN] = {};
-  const int tiles = (kn + BK - 1) / BK;
-  // n along the rows of the result, so that a lane holds four neighbours:
-  // b is the left operand.
-  struct Frags {
-    typename F::Type a[FM], b[FN];
-  };
-  auto read_a = [&](Frags& f, const char* from, int step, int i) {
-    f.a[i] = F::template read<BM, ACOLS>(from, wm + i * 16, step, lane);
-  };
-  auto read_b = [&](Frags& f, const char* from, int step, int j) {
-    f.b[j] = F::template read<BN, BCOLS>(from + OA::kBytes, wn + j * 16, step,
-                                         lane);
-  };
-  if constexpr (BM == 256) {
-    // One block a CU: while one of a k-tile's two steps is multiplied, the
-    // fragments of the next are read, a row's as soon as the row before it is
-    // done with, and the k-tile after next is fetched into the half that was
-    // read last (8192x4096x4096 bf16: 234 us, 263 us as below).
-    constexpr int kPieces = LA::kPieces + LB::kPieces;
-    Frags f0, f1;
-    // next: the step's fragments in `from`; pieces go to `to`
-    auto multiply = [&](const Frags& f, Frags& next, const char* from,
-                        int step, char* to, auto pieces) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
-#pragma unroll
-        for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
-          read_b(next, from, step, j);
-        read_a(next, from, step, i);
-        if (pieces())
-#pragma unroll
-          for (int p = i * kPieces / FM; p < (i + 1) * kPieces / FM; ++p)
-            piece(to, p);
-      }
-      order<FM, FN, F::kMfmas, ACOLS ? F::kColReads : 1,
-            BCOLS ? F::kColReads : 1, pieces()>(
-          std::make_integer_sequence<int, FM>{});
-    };
-    // A k-tile's second step and the next one's first. Where the compiler
-    // cannot tell that no piece goes to where fragments are read, it lets
-    // transposed reads wait for all pieces under way (8192x4096x4096 bf16: dx
-    // 235 us, 267 us so; dw 216 us, 245 us so).
-    auto both = [&](const char* __restrict__ from, char* __restrict__ to) {
-      multiply(f1, f0, from, 0, to, std::integral_constant<int, kPieces>{});
-      load_a.advance();
-      load_b.advance();
-      multiply(f0, f1, from, 1, nullptr, std::integral_constant<int, 0>{});
-    };
-    fetch(0);
-    fetch(1);
-    wait_pieces<kPieces>();
-#pragma unroll
-    for (int j = 0; j < FN; ++j) read_b(f0, lds, 0, j);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) read_a(f0, lds, 0, i);
-    multiply(f0, f1, lds, 1, nullptr, std::integral_constant<int, 0>{});
-    for (int t = 1; t < tiles; ++t) {
-      wait_pieces<0>();
-      both(lds + (t & 1) * kStage, lds + (~t & 1) * kStage);
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-        acc[i][j] = F::mma(f1.b[j], f1.a[i], acc[i][j]);
-  } else {
-    // Several blocks a CU fill each other's gaps, and a simple order leaves
-    // them the registers (524288x128x128 bf16: dx 52 us, 56 us as above).
-    auto multiply = [&](const char* __restrict__ from, char* __restrict__ to,
-                        bool more) {
-      if (more) {
-        load_a.fetch(to);
-        load_b.fetch(to + OA::kBytes);
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        Frags f;
-#pragma unroll
-        for (int j = 0; j < FN; ++j) read_b(f, from, s, j);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) read_a(f, from, s, i);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-            acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
-      }
-    };
-    fetch(0);
-    for (int t = 0; t < tiles; ++t) {
-      wait_pieces<0>();
-      multiply(lds + (t & 1) * kStage, lds + (~t & 1) * kStage,
-               t + 1 < tiles);
-    }
-  }
-  wait_pieces<0>();  // the epilogue writes where the pieces go
-
-  // ---- epilogue ----
   // Each wave passes ROWS rows at a time through LDS of its own, from the
   // matrix cores' layout to eight neighbouring n a lane: full lines to and
   // from memory, and a loop for the activation, whose code unrolled over all
   // accumulators would not stay in the instruction cache.
+  constexpr int ROWS = kEpilogueRows, EROW = TN * 4 + 16;
   constexpr int LPR = TN / 8, RPI = 64 / LPR, ITER = ROWS / RPI;
   char* mine = lds + wave * ROWS * EROW;
   const long n = n0 + wn + (lane % LPR) * 8;
@@ -579,6 +439,195 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       for (int w = 0; w < WM; ++w) v += s[w * BN + i];
       if (n0 + i < g.N) e.partial[(long)mt * g.N + n0 + i] = v;
     }
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool ACOLS, bool BCOLS,
+          int EPI>
+__global__ __launch_bounds__(WM * WN * 64)
+void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
+                 const T* __restrict__ a, const T* __restrict__ b) {
+  using OA = Operand<T, BM, ACOLS>;
+  using OB = Operand<T, BN, BCOLS>;
+  using F = Frag<T>;
+  constexpr int BK = OA::BK, WAVES = WM * WN;
+  constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  constexpr int kStage = OA::kBytes + OB::kBytes;
+  constexpr int kEpi = WAVES * kEpilogueRows * (TN * 4 + 16);
+  // tiles of 256: the next one's first pieces come in during the epilogue
+  constexpr bool AHEAD = BM == 256;
+  constexpr int kEpiAt = AHEAD ? kStage : 0;
+  constexpr int kLds =
+      2 * kStage > kEpiAt + kEpi ? 2 * kStage : kEpiAt + kEpi;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // Work: an XCD's blocks (every eighth) take neighbouring tiles of one part
+  // of k, in groups of 4 rows of tiles, so that they share operands in its
+  // L2 (all tiles of a part, where there are few).
+  const int tm = (int)((g.M + BM - 1) / BM), tn = (int)((g.N + BN - 1) / BN);
+  const int parts = (int)((g.K + g.k_split - 1) / g.k_split);
+  const int total = tm * tn * parts, per = (total + 7) / 8;
+  const int end = min(total, ((int)(blockIdx.x & 7) + 1) * per);
+  int work = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (work >= end) return;
+  int part, mt;
+  long n0;
+  using LA = Loader<T, BM, ACOLS, WAVES, 1>;
+  using LB = Loader<T, BN, BCOLS, WAVES, 1>;
+  LA load_a;
+  LB load_b;
+  auto place = [&] {
+    part = work / (tm * tn);
+    const int tile = work - part * tm * tn;
+    const int group = tile / (4 * tn), in_group = tile - group * 4 * tn;
+    const int rows = min(4, tm - group * 4);
+    mt = group * 4 + in_group % rows;
+    n0 = (long)(in_group / rows) * BN;
+    const long kb = part * g.k_split;
+    const int kn = (int)min(g.K - kb, g.k_split);
+    load_a = LA(a, g.lda, (long)mt * BM, g.M, kb, kn, wave, lane);
+    load_b = LB(b, g.ldb, n0, g.N, kb, kn, wave, lane);
+    return (kn + BK - 1) / BK;
+  };
+  int tiles = place();
+  auto fetch = [&](int stage) {
+    load_a.fetch(lds + stage * kStage);
+    load_b.fetch(lds + stage * kStage + OA::kBytes);
+  };
+
+  auto piece = [&](char* to, int p) {
+    if (p < LA::kEach)
+      load_a.piece(to, p);
+    else
+      load_b.piece(to + OA::kBytes, p - LA::kEach);
+  };
+
+  const int wm = wave / WN * TM, wn = wave % WN * TN;
+  f32x4 acc[FM][FN];
+  auto clear = [&] {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{};
+  };
+  // n along the rows of the result, so that a lane holds four neighbours:
+  // b is the left operand.
+  struct Frags {
+    typename F::Type a[FM], b[FN];
+  };
+  auto read_a = [&](Frags& f, const char* from, int step, int i) {
+    f.a[i] = F::template read<BM, ACOLS>(from, wm + i * 16, step, lane);
+  };
+  auto read_b = [&](Frags& f, const char* from, int step, int j) {
+    f.b[j] = F::template read<BN, BCOLS>(from + OA::kBytes, wn + j * 16, step,
+                                         lane);
+  };
+  if constexpr (BM == 256) {
+    // One block a CU: while one of a k-tile's two steps is multiplied, the
+    // fragments of the next are read, a row's as soon as the row before it is
+    // done with, and the k-tile after next is fetched into the half that was
+    // read last (8192x4096x4096 bf16: 234 us, 263 us as below).
+    constexpr int kPieces = LA::kPieces + LB::kPieces;
+    Frags f0, f1;
+    // next: the step's fragments in `from`; pieces go to `to`
+    auto multiply = [&](const Frags& f, Frags& next, const char* from,
+                        int step, char* to, auto pieces) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
+#pragma unroll
+        for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
+          read_b(next, from, step, j);
+        read_a(next, from, step, i);
+        if (pieces())
+#pragma unroll
+          for (int p = i * kPieces / FM; p < (i + 1) * kPieces / FM; ++p)
+            piece(to, p);
+      }
+      order<FM, FN, F::kMfmas, ACOLS ? F::kColReads : 1,
+            BCOLS ? F::kColReads : 1, pieces()>(
+          std::make_integer_sequence<int, FM>{});
+    };
+    // A k-tile's second step and the next one's first. Where the compiler
+    // cannot tell that no piece goes to where fragments are read, it lets
+    // transposed reads wait for all pieces under way (8192x4096x4096 bf16: dx
+    // 235 us, 267 us so; dw 216 us, 245 us so).
+    auto both = [&](const char* __restrict__ from, char* __restrict__ to) {
+      multiply(f1, f0, from, 0, to, std::integral_constant<int, kPieces>{});
+      load_a.advance();
+      load_b.advance();
+      multiply(f0, f1, from, 1, nullptr, std::integral_constant<int, 0>{});
+    };
+    fetch(0);
+    for (;;) {
+      clear();
+      fetch(1);
+      wait_pieces<kPieces>();
+#pragma unroll
+      for (int j = 0; j < FN; ++j) read_b(f0, lds, 0, j);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) read_a(f0, lds, 0, i);
+      multiply(f0, f1, lds, 1, nullptr, std::integral_constant<int, 0>{});
+      for (int t = 1; t < tiles; ++t) {
+        wait_pieces<0>();
+        both(lds + (t & 1) * kStage, lds + (~t & 1) * kStage);
+      }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = F::mma(f1.b[j], f1.a[i], acc[i][j]);
+      wait_pieces<0>();  // the epilogue writes where the pieces go
+      const int row = mt, p = part;
+      const long col = n0;
+      work += gridDim.x / 8;
+      if (work < end) {
+        tiles = place();
+        fetch(0);
+      }
+      tile_epilogue<T, BM, BN, WM, WN, EPI>(acc, lds + kEpiAt, wave, lane,
+                                            row, col, p, g, e, c);
+      if (work >= end) return;
+      wait_lds();
+    }
+  } else {
+    // Several blocks a CU fill each other's gaps, and a simple order leaves
+    // them the registers (524288x128x128 bf16: dx 52 us, 56 us as above).
+    auto multiply = [&](const char* __restrict__ from, char* __restrict__ to,
+                        bool more) {
+      if (more) {
+        load_a.fetch(to);
+        load_b.fetch(to + OA::kBytes);
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        Frags f;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) read_b(f, from, s, j);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) read_a(f, from, s, i);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = F::mma(f.b[j], f.a[i], acc[i][j]);
+      }
+    };
+    clear();
+    fetch(0);
+    for (int t = 0; t < tiles; ++t) {
+      wait_pieces<0>();
+      multiply(lds + (t & 1) * kStage, lds + (~t & 1) * kStage,
+               t + 1 < tiles);
+    }
+    wait_pieces<0>();  // the epilogue writes where the pieces go
+    tile_epilogue<T, BM, BN, WM, WN, EPI>(acc, lds + kEpiAt, wave, lane, mt,
+                                          n0, part, g, e, c);
   }
 }
 
@@ -1059,7 +1108,9 @@ void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
     }
   }
   const long tiles = ceil_div(g.M, tile) * (long)ceil_div(g.N, tile);
-  const dim3 grid((unsigned)((tiles * splits + 7) / 8 * 8));
+  // tiles of 256 fill a CU, whose block takes one after the other
+  const long blocks = (tiles * splits + 7) / 8 * 8;
+  const dim3 grid((unsigned)(tile == 256 ? std::min(blocks, 256l) : blocks));
 #define LAUNCH(B, WM, WN)                                                     \
   hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, ACOLS, BCOLS, EPI>),       \
                      grid, dim3(WM * WN * 64), 0, s, g, e, c, a, b)
