@@ -454,8 +454,11 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr int kStage = OA::kBytes + OB::kBytes;
   constexpr int kEpi = WAVES * kEpilogueRows * (TN * 4 + 16);
-  // tiles of 256: the next one's first pieces come in during the epilogue
-  constexpr bool AHEAD = BM == 256;
+  // Tiles of 256 in bf16: a block takes one after the other, and the next
+  // one's first pieces come in during the epilogue (65536x512x2048: 185 us,
+  // 199 us with a block a tile). Products of floats take five times as long,
+  // and what the next tile needs would not stay in registers beside them.
+  constexpr bool AHEAD = BM == 256 && sizeof(T) == 2;
   constexpr int kEpiAt = AHEAD ? kStage : 0;
   constexpr int kLds =
       2 * kStage > kEpiAt + kEpi ? 2 * kStage : kEpiAt + kEpi;
@@ -585,7 +588,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       wait_pieces<0>();  // the epilogue writes where the pieces go
       const int row = mt, p = part;
       const long col = n0;
-      work += gridDim.x / 8;
+      work = AHEAD ? work + gridDim.x / 8 : end;
       if (work < end) {
         tiles = place();
         fetch(0);
@@ -1108,9 +1111,11 @@ void launch_tile(int tile, T* c, const T* a, const T* b, const GemmArgs& g,
     }
   }
   const long tiles = ceil_div(g.M, tile) * (long)ceil_div(g.N, tile);
-  // tiles of 256 fill a CU, whose block takes one after the other
+  // one block a CU for bf16 tiles of 256
   const long blocks = (tiles * splits + 7) / 8 * 8;
-  const dim3 grid((unsigned)(tile == 256 ? std::min(blocks, 256l) : blocks));
+  const dim3 grid((unsigned)(tile == 256 && sizeof(T) == 2
+                                 ? std::min(blocks, 256l)
+                                 : blocks));
 #define LAUNCH(B, WM, WN)                                                     \
   hipLaunchKernelGGL((linear_tile<T, B, B, WM, WN, ACOLS, BCOLS, EPI>),       \
                      grid, dim3(WM * WN * 64), 0, s, g, e, c, a, b)
