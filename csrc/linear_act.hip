@@ -407,6 +407,10 @@ GFA_DEV void tile_epilogue(const f32x4 (&acc)[BM / WM / 16][BN / WN / 16],
         if (EPI == kForward && op) z[j] += other[q][j];
         if (EPI == kSlope) z[j] *= other[q][j];
       }
+      // 0 behind the last column, where an infinite x makes z no number
+      if (EPI == kSlope && !whole)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = j < left ? z[j] : 0.f;
       if (m >= g.M) continue;
       if constexpr (EPI == kSlope) {
 #pragma unroll

@@ -598,6 +598,21 @@ def test_linear_act_bad_values_stay_alone(dev, dtype, m, k, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [9, 300, 6000])
+def test_linear_act_flat_where_x_is_infinite(dev, dtype, m):
+    """Where x is infinite tanh is flat and dx 0, for widths whose rows are
+    padded too: no infinity times a weight behind the last one."""
+    x, w, b, _ = linear_inputs(dev, m, 64, 515, dtype)
+    w = torch.where(w == 0, 1.0, w)
+    x[3, 7] = math.inf
+    x.requires_grad_()
+    y = linear_act(x, w, b, "tanh", weight_gain=0.05)
+    dx, = torch.autograd.grad(y, x, randn(m, 515, device=dev, dtype=dtype))
+    assert torch.isfinite(dx).all() and not dx[3].any() and dx[2].any()
+
+
+@pytest.mark.gpu
 def test_linear_act_far_rows(dev):
     """Offsets past 32 bits: over 2^31 elements of x."""
     k, n, rows = 512, 16, (1 << 22) + 70
