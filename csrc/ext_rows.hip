@@ -520,10 +520,11 @@ variable_list composed_grads(const variable_list& in,
     views.push_back(in[i].defined() ? in[i].view_as(in[i]) : Tensor());
     if (need[i]) wanted.push_back(views.back());
   }
+  variable_list out(in.size());
+  if (wanted.empty()) return out;
   const variable_list got = torch::autograd::grad(
       {f(views)}, wanted, {dy}, /*retain_graph=*/std::nullopt,
       /*create_graph=*/true);
-  variable_list out(in.size());
   size_t k = 0;
   for (size_t i = 0; i < in.size(); ++i)
     if (need[i]) out[i] = got[k++];
@@ -575,6 +576,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b,
   return std::get<0>(layer_norm_fwd(x, w, b, eps, false));
 }
 
+// without the residual
 Tensor composed_linear_act(const variable_list& in, const LinearParams& p) {
   Tensor z = torch::matmul(in[0].to(torch::kFloat32),
                            in[1].to(torch::kFloat32).t()) * p.weight_gain;
@@ -590,7 +592,6 @@ Tensor composed_linear_act(const variable_list& in, const LinearParams& p) {
   }
   y = y * p.gain;
   if (!std::isinf(p.clamp)) y = y.clamp(-p.clamp, p.clamp);
-  if (in[3].defined()) y = y + in[3];
   return y.to(in[0].scalar_type());
 }
 
@@ -599,8 +600,10 @@ Tensor composed_linear_act(const variable_list& in, const LinearParams& p) {
 // moves 8 bytes an element and a pass over dz; computing it again costs k
 // multiplications an element and happens where dz is made. The two meet at
 // about 1500 (bf16) and 128 (float) multiplications.
-bool keeps_z(const Tensor& x, const LinearParams& p) {
+bool keeps_z(const Tensor& x, const Tensor& w, const OptTensor& bias,
+             const LinearParams& p) {
   return p.curved() &&
+         (x.requires_grad() || w.requires_grad() || wants_grad(bias)) &&
          x.size(-1) > (x.scalar_type() == torch::kFloat32 ? 128 : 1536);
 }
 
@@ -608,8 +611,11 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w,
                         const OptTensor& bias, const OptTensor& residual,
                         const LinearParams& p) {
-    auto [y, z] = linear_act_fwd(x, w, bias, residual, p, keeps_z(x, p));
-    ctx->save_for_backward({x, w, plain(bias), plain(residual), plain(z)});
+    auto [y, z] =
+        linear_act_fwd(x, w, bias, residual, p, keeps_z(x, w, bias, p));
+    // the residual, whose gradient is dy, is not needed again
+    ctx->save_for_backward({x, w, plain(bias), plain(z)});
+    ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["params"] =
         std::vector<double>{(double)p.act, p.alpha,       p.gain,
                             p.clamp,       p.weight_gain, p.bias_gain};
@@ -619,20 +625,24 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const auto s = ctx->get_saved_variables();
     const auto d = ctx->saved_data["params"].toDoubleVector();
     const LinearParams p{(int64_t)d[0], d[1], d[2], d[3], d[4], d[5]};
-    const variable_list in{s[0], s[1], s[2], s[3]};
+    const variable_list in{s[0], s[1], s[2]};
     const auto need = needed(ctx, in);
+    const Tensor dres = ctx->saved_data["residual"].toBool() &&
+                                ctx->needs_input_grad(s[2].defined() ? 3 : 2)
+                            ? dy[0]
+                            : Tensor();
     if (torch::GradMode::is_enabled()) {
       auto out = composed_grads(in, need, dy[0], [&](const variable_list& v) {
         return composed_linear_act(v, p);
       });
+      out.push_back(dres);
       out.emplace_back();
       return out;
     }
     const auto [dx, dw, db] =
-        linear_act_bwd(dy[0], opt(s[4]), s[0], s[1], opt(s[2]), p, need[0],
+        linear_act_bwd(dy[0], opt(s[3]), s[0], s[1], opt(s[2]), p, need[0],
                        need[1], need[2]);
-    return {plain(dx), plain(dw), plain(db), need[3] ? dy[0] : Tensor(),
-            Tensor()};
+    return {plain(dx), plain(dw), plain(db), dres, Tensor()};
   }
 };
 

@@ -564,6 +564,31 @@ def test_linear_act_single_gradients(dev, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("again", [False, True])
+def test_linear_act_does_not_keep_the_residual(dev, again):
+    """Its gradient is dy, so it may change before the backward pass."""
+    x, w, b, res = linear_inputs(dev, 40, 48, 64, F32)
+    leaf = res.clone().requires_grad_()
+    dy = randn(40, 64, device=dev, seed=6, grad=again)
+    for others in (False, True):
+        leaves = [leaf] + [t.detach().clone().requires_grad_()
+                           for t in (x, w, b) if others]
+        args = leaves[1:] or (x, w, b)
+        got = []
+        for change in (False, True):
+            r = leaf * 1
+            y = linear_act(args[0], args[1], args[2], "silu", r)
+            if change:
+                r.zero_()
+            got.append(torch.autograd.grad(y, leaves, dy, create_graph=again))
+        assert torch.equal(got[0][0], dy)
+        for a, c in zip(*got):
+            assert torch.equal(a, c)
+    if again:
+        assert got[0][0].requires_grad
+
+
+@pytest.mark.gpu
 def test_linear_act_empty(dev):
     x = randn(0, 3, 8, device=dev, grad=True)
     w, b = randn(5, 8, device=dev, grad=True), randn(5, device=dev, grad=True)
