@@ -360,9 +360,8 @@ class MappingNetwork(nn.Module):
             for layer in self.layers:
                 x = layer(x)
         else:
-            x = self.layers[0](x)
-            for norm, layer in zip(self.norms, self.layers[1:]):
-                x = layer(norm(x), residual=x)
+            for i, layer in enumerate(self.layers):
+                x = layer(self.norms[i - 1](x), residual=x) if i else layer(x)
         if update_w_avg:
             with torch.no_grad():
                 self.w_avg.copy_(

@@ -842,6 +842,13 @@ def test_residual_mapping_is_the_formula():
     assert torch.allclose(net(z)[:, 0], x, rtol=1e-4, atol=1e-4)
 
 
+@pytest.mark.parametrize("layers", [0, 1])
+def test_residual_mapping_of_few_layers_is_plain(layers):
+    plain, net = mapping(False, layers), mapping(True, layers)
+    z = randn(3, 5, 64, seed=7)
+    assert torch.equal(net(z), plain(z))
+
+
 def test_plain_mapping_has_no_norms():
     keys = set(mapping(False).state_dict())
     assert not any("norm" in k for k in keys)
