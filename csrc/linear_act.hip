@@ -1094,7 +1094,7 @@ struct TileCost {
 const TileCost kTileCosts[2][5] = {
     // bf16
     {{256, 1.7, 1.7, 8}, {128, 0.77, 0.57, 2}, {64, 0.40, 0.214, 1},
-     {32, 0.2, 0.12, 0.5}, {16, 0.06, 0.05, 0.5}},
+     {32, 0.2, 0.16, 0.5}, {16, 0.06, 0.05, 0.5}},
     // float
     {{256, 7.4, 7.4, 8}, {128, 2.15, 2.0, 2}, {64, 0.65, 0.53, 1},
      {32, 0.24, 0.21, 0.5}, {16, 0.165, 0.15, 0.5}}};
