@@ -29,14 +29,15 @@ using LdsPtr = __attribute__((address_space(3))) void*;
 // 16-byte aligned.
 //
 // What bounds it: float the matrix cores (busy 94% of the time at 4096^3, 146
-// TFLOP/s); bf16 8192x4096x4096 keeps them busy 61% (1136 TFLOP/s; a copy of
-// the operands and the result would take 32 us); a short k leaves a tile's
-// 128 KB of results, 9 us of its 23 us at k = 512.
+// TFLOP/s); bf16 8192x4096x4096 keeps them busy 68% (1175 TFLOP/s; dx 75%, dw
+// 79%; a copy of the operands and the result would take 32 us); a short k
+// leaves a tile's 128 KB of results, half of its 23 us at k = 512.
 //
 // LDS layout. Rows: [m][128 bytes], 16-byte granule g of row r at g ^ (r/2
 // mod 8), so that the 16 rows a fragment read touches spread over all 64
-// banks (conflicts: 2% of the LDS's busy cycles). Columns: [k][BX], granules of row k exchanged likewise; bf16
-// fragments come out of it through the transposing LDS read.
+// banks (conflicts: 2% of the LDS's busy cycles). Columns: [k][BX], granules
+// of row k exchanged likewise; bf16 fragments come out of it through the
+// transposing LDS read.
 template <typename T, int BX, bool COLS>
 struct Operand {
   static constexpr int ES = sizeof(T);
@@ -1084,9 +1085,9 @@ namespace {
 // others, and on the rest of a block's work. Measured: 8192x4096x4096 bf16
 // takes 234, 314 and 439 us with tiles of 256, 128 and 64, 4096^3 float 940,
 // 1021 and 1089 us; 524288x128x128 bf16, half of whose tiles of 256 would be
-// padding, 120 us with those and 48 us with 128. Of 21 shapes and up to 40
-// ways to cut each, in both types, what the figures choose is within 5% of
-// the quickest in 37 cases and within 20% in the others.
+// padding, 120 us with those and 48 us with 128. Fitted to 21 shapes in both
+// types, each cut in up to 40 ways, and put right where a choice lost since
+// (2048x4096x2048 bf16: 50 us with 128, 53 us with 64).
 struct TileCost {
   int side;
   double alone, shared, rest;
