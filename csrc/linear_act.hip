@@ -699,10 +699,14 @@ struct Finish4 {
     for (int j = 0; j < 4; ++j) {
       if (j >= left) o[j] = 0.f;
       if (j < end) {
-        const auto raw = round_raw<T>(o[j]);
+        auto raw = round_raw<T>(o[j]);
+        if constexpr (EPI == kSlope && sizeof(T) == 2)
+          if (e.dz_low) {
+            float rest;
+            split(o[j], raw, rest);
+            put(e.dz_low + m * g.ldc + n + j, rest);
+          }
         *reinterpret_cast<typename Raw<T>::type*>(c + m * g.ldc + n + j) = raw;
-        if (EPI == kSlope && e.dz_low)
-          put(e.dz_low + m * g.ldc + n + j, o[j] - raw_to_f32(raw));
       }
     }
   }
@@ -1293,14 +1297,18 @@ void linear_dz_kernel(T* __restrict__ dz, T* __restrict__ low,
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= s[j];
         // padded rows, zero behind the last element
-        store8(dz + (r + u * step) * dz_stride + i, v, 8);
-        if (low) {
-          float rest[8];
+        float first[8], rest[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            rest[j] = v[j] - raw_to_f32(round_raw<T>(v[j]));
-          store8(low + (r + u * step) * dz_stride + i, rest, 8);
+        for (int j = 0; j < 8; ++j) {
+          first[j] = v[j];
+          if (sizeof(T) == 2 && low) {
+            u16 high;
+            split(v[j], high, rest[j]);
+            first[j] = raw_to_f32(high);
+          }
         }
+        store8(dz + (r + u * step) * dz_stride + i, first, 8);
+        if (low) store8(low + (r + u * step) * dz_stride + i, rest, 8);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] += v[j];  // before their rounding

@@ -16,6 +16,20 @@ template <typename T> GFA_DEV void put(T* p, float v) {
   *reinterpret_cast<typename Raw<T>::type*>(p) = round_raw<T>(v);
 }
 
+// v in two bf16 numbers whose sum is v up to 2^-15 of it: what is left of it
+// toward zero, and the rest. Both have v's sign and, unless v is 0, neither is
+// 0: a product with an infinity stays that infinity, where rests of the other
+// sign or 0 would make the sum of both products no number. So does an infinite
+// v, which has no rest. (A NaN that a product made has its first bit below
+// the exponent set: it stays one.)
+GFA_DEV void split(float v, u16& high, float& rest) {
+  constexpr float kLeast = 1.17549435e-38f;  // smallest normal number
+  high = (u16)(__float_as_uint(v) >> 16);
+  rest = v - raw_to_f32(high);
+  if (!(fabsf(rest) >= kLeast && fabsf(rest) < INFINITY))
+    rest = v == 0.f ? 0.f : copysignf(kLeast, v);
+}
+
 // activation codes of gansformer_amd/ops/linear_act.py
 enum Act { kLinear = 0, kRelu, kLrelu, kTanh, kSigmoid, kGelu, kSilu };
 
@@ -204,7 +218,7 @@ struct EpilogueArgs {
   const T* residual;  // forward: [M, N] with rows of res_stride, or null
   long res_stride;
   float* z;     // forward: [M, N] or null
-  T* dz_low;    // slope: what rounding took from dz, or null
+  T* dz_low;    // slope: the rest of dz (split), or null
   const T* dy;  // slope: [M, N] with rows of dy_stride
   long dy_stride;
   // slope: sums over the rows of each row of tiles, or null; with k in
@@ -247,8 +261,8 @@ struct SmallBackward {
   T *dw_out, *dx_out;
   void* db_out;
   bool db_f32;
-  // dz and, unless null, what rounding took from it: the rounding errors of
-  // a few rows do not average out
+  // dz and, unless null, the rest of it: the rounding errors of a few rows do
+  // not average out
   const T *dz, *dz_low;
   const T *x, *w;
   // db: db_scale times the sums of the groups of partial, or of dz's rows
@@ -273,8 +287,8 @@ struct PadArgs {
 template <typename T>
 void launch_pad_rows(const PadArgs<T>& p0, const PadArgs<T>& p1, hipStream_t);
 
-// dz = dy * slope(z) (z and dz null: dz = dy), low (or null) what rounding
-// took from it, and, unless partial is null,
+// dz = dy * slope(z) (z and dz null: dz = dy), low (or null) the rest of it
+// (split), and, unless partial is null,
 // partial[g][n] = sums of dz over the rows of group g
 int linear_dz_groups(long rows, int n);
 template <typename T>

@@ -816,6 +816,30 @@ def test_captured_and_replayed(dev, m):
                 assert torch.equal(a, b)
 
 
+# ---------------- every digit of dz ----------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("gain", [1.0, 1.3])
+@pytest.mark.parametrize("m,k,n", [(5, 72, 40), (64, 72, 40), (30, 1600, 33),
+                                   (2500, 136, 264), (2100, 1700, 40)])
+def test_linear_act_infinite_gradient(dev, m, k, n, gain):
+    """An infinite dy, weight or x makes infinities of the gradients that it
+    belongs to, in bf16 whose dz comes in two parts too, and no others."""
+    x, w, _, _ = linear_inputs(dev, m, k, n, BF16)
+    x, w = x.abs() + 1, w.abs() + 1
+    for where in ("dy", "x", "w"):
+        dy = torch.ones(m, n, device=dev, dtype=BF16)
+        leaves = [x.clone(), w.clone()]
+        {"dy": dy, "x": leaves[0], "w": leaves[1]}[where][3, 7] = math.inf
+        dx, dw = torch.autograd.grad(
+            linear_act(*[t.requires_grad_() for t in leaves], act="relu",
+                       gain=gain), leaves, dy)
+        for got, i in {"dy": ((dx, 3), (dw, 7)), "x": ((dw.t(), 7),),
+                       "w": ((dx.t(), 7),)}[where]:
+            assert (got[i] == math.inf).all(), where
+            got[i] = 0
+        assert torch.isfinite(dx).all() and torch.isfinite(dw).all(), where
+
+
 # ---------------- in the mapping network ----------------
 def mapping(residual, layers=4, dim=64):
     from gansformer_amd.models.networks import MappingNetwork
