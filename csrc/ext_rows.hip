@@ -398,10 +398,9 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     int groups = 0;
     if (curved) {
       const int64_t width = (n + 7) / 8 * 8;  // zeros behind n
-      // few rows: also what rounding dz to bf16 took
-      const bool low = !is_f32 && any && small;
-      scalar_t* dz = dz_room.get<scalar_t>(m * width * (low ? 2 : 1));
-      if (low) e.dz_low = dz + m * width;
+      // a bf16 dz in two parts
+      scalar_t* dz = dz_room.get<scalar_t>(m * width * (is_f32 ? 1 : 2));
+      if (!is_f32) e.dz_low = dz + m * width;
       const auto plan = gfa::linear_plan(m, n, k, is_f32, gfa::kSlopes);
       groups = again ? gfa::linear_row_tiles(plan, m)
                      : gfa::linear_dz_groups(m, (int)n);
@@ -441,6 +440,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     const bool db_f32 = need_db && bias->scalar_type() == torch::kFloat32;
     const gfa::GemmArgs gx{m, k, n, dr.stride, wr.stride, k, scale, n};
     const gfa::GemmArgs gw{n, k, m, dr.stride, xr.stride, k, scale, m};
+    const int passes = e.dz_low ? 2 : 1;
     if (small) {
       gfa::SmallBackward<scalar_t> s{};
       s.dw = gw;
@@ -467,18 +467,22 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
                                           partial, groups, (int)n, db_scale,
                                           cur_stream());
       if (need_dx) {
-        const auto plan = gfa::linear_plan(m, k, n, is_f32, gfa::kInputs);
+        const auto plan =
+            gfa::linear_plan(m, k, n * passes, is_f32, gfa::kInputs);
         gfa::launch_linear_dx<scalar_t>(
             mptr<scalar_t>(dx),
             dx_parts.get<float>(plan.splits > 1 ? plan.splits * m * k : 0),
-            rptr<scalar_t>(dr), rptr<scalar_t>(wr), gx, plan, cur_stream());
+            rptr<scalar_t>(dr), e.dz_low, rptr<scalar_t>(wr), gx, plan,
+            cur_stream());
       }
       if (need_dw) {
-        const auto plan = gfa::linear_plan(n, k, m, is_f32, gfa::kWeights);
+        const auto plan =
+            gfa::linear_plan(n, k, m * passes, is_f32, gfa::kWeights);
         gfa::launch_linear_dw<scalar_t>(
             mptr<scalar_t>(dw),
             dw_parts.get<float>(plan.splits > 1 ? plan.splits * n * k : 0),
-            rptr<scalar_t>(dr), rptr<scalar_t>(xr), gw, plan, cur_stream());
+            rptr<scalar_t>(dr), e.dz_low, rptr<scalar_t>(xr), gw, plan,
+            cur_stream());
       }
     }
   });

@@ -5,6 +5,10 @@
 //   y  = clamp(act(z) * gain) + residual
 //   dz = dy * slope(z);  dx = dz W;  dW = dz^T x;  db = sum_rows dz
 //
+// A bf16 dz is kept as two bf16 numbers, and dx and dW are the sums of the
+// products of both: rounded to one, dz would put as much error into dx and dW
+// as their own rounding does.
+//
 // Every product is one C[m, n] = sum_k A[m, k] B[n, k] over operands that are
 // contiguous along k ("rows") or along m or n ("columns"). Sums in float on
 // the matrix cores; what leaves a kernel is rounded to T once.
@@ -203,6 +207,16 @@ GFA_DEV void store8(bf16* p, const float* v, int left) {
   }
 }
 
+// v becomes the first of split's two numbers, rest the second
+GFA_DEV void split8(float (&v)[8], float (&rest)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    u16 high;
+    split(v[j], high, rest[j]);
+    v[j] = raw_to_f32(high);
+  }
+}
+
 // waits until at most N of the wave's pieces are under way and its LDS reads
 // are done, then for the block's other waves
 template <int N>
@@ -256,6 +270,14 @@ struct Loader {
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       offset[i] = O::source((i * WAVES + wave) * 64 + lane, (int)stride);
+  }
+
+  // back over so many k-tiles, in an operand of the same shape `apart` bytes
+  // from this one
+  GFA_DEV void rewind(int ktiles, long apart) {
+    at += apart - ktiles * step;
+    bytes += ktiles * step;
+    left += ktiles * BK;
   }
 
   // A piece of the next k-tile, the i-th of this wave. Past the end nothing is
@@ -417,7 +439,14 @@ GFA_DEV void tile_epilogue(const f32x4 (&acc)[BM / WM / 16][BN / WN / 16],
 #pragma unroll
         for (int j = 0; j < 8; ++j) sums[j] += z[j];
         // dz has padded rows, zero behind the last element
-        if (left) store8(c + m * g.ldc + n, z, 8);
+        if (left) {
+          if constexpr (sizeof(T) == 2) {
+            float rest[8];
+            split8(z, rest);
+            store8(e.dz_low + m * g.ldc + n, rest, 8);
+          }
+          store8(c + m * g.ldc + n, z, 8);
+        }
       } else if constexpr (EPI == kPartial) {
         store8(e.partial + (part * g.M + m) * g.N + n, z, left);
       } else {
@@ -487,6 +516,9 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
   using LB = Loader<T, BN, BCOLS, WAVES, 1>;
   LA load_a;
   LB load_b;
+  // dx and dw of bf16: the product goes over k again with the rest of dz
+  constexpr bool TWICE = BCOLS && sizeof(T) == 2;
+  bool again = false;
   auto place = [&] {
     part = work / (tm * tn);
     const int tile = work - part * tm * tn;
@@ -498,19 +530,31 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     const int kn = (int)min(g.K - kb, g.k_split);
     load_a = LA(a, g.lda, (long)mt * BM, g.M, kb, kn, wave, lane);
     load_b = LB(b, g.ldb, n0, g.N, kb, kn, wave, lane);
-    return (kn + BK - 1) / BK;
+    if (TWICE) again = e.a_low;
+    return (kn + BK - 1) / BK * (again ? 2 : 1);
   };
   int tiles = place();
-  auto fetch = [&](int stage) {
-    load_a.fetch(lds + stage * kStage);
-    load_b.fetch(lds + stage * kStage + OA::kBytes);
-  };
-
+  constexpr int kPieces = LA::kPieces + LB::kPieces;
   auto piece = [&](char* to, int p) {
     if (p < LA::kEach)
       load_a.piece(to, p);
     else
       load_b.piece(to + OA::kBytes, p - LA::kEach);
+  };
+  auto advance = [&] {
+    load_a.advance();
+    load_b.advance();
+    if (TWICE && again && load_a.left <= 0) {
+      load_a.rewind(tiles / 2, (e.a_low - a) * (long)sizeof(T));
+      load_b.rewind(tiles / 2, 0);
+      again = false;
+    }
+  };
+  // the next k-tile
+  auto fetch = [&](char* to) {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) piece(to, p);
+    advance();
   };
 
   const int wm = wave / WN * TM, wn = wave % WN * TN;
@@ -538,7 +582,6 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     // fragments of the next are read, a row's as soon as the row before it is
     // done with, and the k-tile after next is fetched into the half that was
     // read last (8192x4096x4096 bf16: 234 us, 263 us as below).
-    constexpr int kPieces = LA::kPieces + LB::kPieces;
     Frags f0, f1;
     // next: the step's fragments in `from`; pieces go to `to`
     auto multiply = [&](const Frags& f, Frags& next, const char* from,
@@ -567,14 +610,13 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     // 235 us, 267 us so; dw 216 us, 245 us so).
     auto both = [&](const char* __restrict__ from, char* __restrict__ to) {
       multiply(f1, f0, from, 0, to, std::integral_constant<int, kPieces>{});
-      load_a.advance();
-      load_b.advance();
       multiply(f0, f1, from, 1, nullptr, std::integral_constant<int, 0>{});
+      advance();
     };
-    fetch(0);
+    fetch(lds);
     for (;;) {
       clear();
-      fetch(1);
+      fetch(lds + kStage);
       wait_pieces<kPieces>();
 #pragma unroll
       for (int j = 0; j < FN; ++j) read_b(f0, lds, 0, j);
@@ -596,7 +638,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       work = AHEAD ? work + gridDim.x / 8 : end;
       if (work < end) {
         tiles = place();
-        fetch(0);
+        fetch(lds);
       }
       tile_epilogue<T, BM, BN, WM, WN, EPI>(acc, lds + kEpiAt, wave, lane,
                                             row, col, p, g, e, c);
@@ -608,10 +650,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
     // them the registers (524288x128x128 bf16: dx 52 us, 56 us as above).
     auto multiply = [&](const char* __restrict__ from, char* __restrict__ to,
                         bool more) {
-      if (more) {
-        load_a.fetch(to);
-        load_b.fetch(to + OA::kBytes);
-      }
+      if (more) fetch(to);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         Frags f;
@@ -627,7 +666,7 @@ void linear_tile(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
       }
     };
     clear();
-    fetch(0);
+    fetch(lds);
     for (int t = 0; t < tiles; ++t) {
       wait_pieces<0>();
       multiply(lds + (t & 1) * kStage, lds + (~t & 1) * kStage,
@@ -700,12 +739,11 @@ struct Finish4 {
       if (j >= left) o[j] = 0.f;
       if (j < end) {
         auto raw = round_raw<T>(o[j]);
-        if constexpr (EPI == kSlope && sizeof(T) == 2)
-          if (e.dz_low) {
-            float rest;
-            split(o[j], raw, rest);
-            put(e.dz_low + m * g.ldc + n + j, rest);
-          }
+        if constexpr (EPI == kSlope && sizeof(T) == 2) {
+          float rest;
+          split(o[j], raw, rest);
+          put(e.dz_low + m * g.ldc + n + j, rest);
+        }
         *reinterpret_cast<typename Raw<T>::type*>(c + m * g.ldc + n + j) = raw;
       }
     }
@@ -930,7 +968,9 @@ __global__ __launch_bounds__(256)
 void linear_small(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
                   const T* __restrict__ a, const T* __restrict__ b) {
   __shared__ __attribute__((aligned(16))) char lds[kSmallLds];
-  small_block<T, ACOLS, BCOLS, EPI>(lds, blockIdx.x, g, e, c, a, b);
+  small_block<T, ACOLS, BCOLS, EPI>(
+      lds, blockIdx.x, g, e, c, a, b,
+      BCOLS && sizeof(T) == 2 ? e.a_low : nullptr);
 }
 
 // out[i] = scale * sum_r src[r][i] for eight columns from n0 on
@@ -1232,18 +1272,22 @@ void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
 }
 
 template <typename T>
-void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
-                      const GemmArgs& g, const LinearPlan& p, hipStream_t s) {
+void launch_linear_dx(T* dx, float* partial, const T* dz, const T* dz_low,
+                      const T* w, const GemmArgs& g, const LinearPlan& p,
+                      hipStream_t s) {
   EpilogueArgs<T> e{};
   e.partial = partial;
+  e.a_low = dz_low;
   launch_split<T, false, true, kPlain>(dx, dz, w, g, e, p, s);
 }
 
 template <typename T>
-void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
-                      const GemmArgs& g, const LinearPlan& p, hipStream_t s) {
+void launch_linear_dw(T* dw, float* partial, const T* dz, const T* dz_low,
+                      const T* x, const GemmArgs& g, const LinearPlan& p,
+                      hipStream_t s) {
   EpilogueArgs<T> e{};
   e.partial = partial;
+  e.a_low = dz_low;
   launch_split<T, true, true, kPlain>(dw, dz, x, g, e, p, s);
 }
 
@@ -1296,22 +1340,18 @@ void linear_dz_kernel(T* __restrict__ dz, T* __restrict__ low,
         act_slopes(s, act);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= s[j];
-        // padded rows, zero behind the last element
-        float first[8], rest[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          first[j] = v[j];
-          if (sizeof(T) == 2 && low) {
-            u16 high;
-            split(v[j], high, rest[j]);
-            first[j] = raw_to_f32(high);
-          }
-        }
-        store8(dz + (r + u * step) * dz_stride + i, first, 8);
-        if (low) store8(low + (r + u * step) * dz_stride + i, rest, 8);
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] += v[j];  // before their rounding
+      if (!z) continue;
+      // padded rows, zero behind the last element
+      const long at = (r + u * step) * dz_stride + i;
+      if constexpr (sizeof(T) == 2) {
+        float rest[8];
+        split8(v, rest);
+        store8(low + at, rest, 8);
+      }
+      store8(dz + at, v, 8);
     }
   }
   if (!partial) return;
@@ -1359,13 +1399,13 @@ void launch_linear_dz(T* dz, T* low, long dz_stride, float* partial,
 // One launch where both products' tiles of 32 fit the card a few times over
 // and neither k is long (both gradients of 1500x512x512: bf16 14.9 us, float
 // 26 us; in launches of their own 18 and 37 us, and two launches more for the
-// host). A few rows of bf16 go there from further off, for
-// the part of dz that rounding takes.
+// host). With a dz in two parts, dz included: 544x512x512 bf16 20.5 against
+// 24.1 us, 1500x512x512 31.6 against 35.8, near the rule's edge (512x1024x1024)
+// 37.5 against 33.6.
 bool linear_backward_is_small(long m, long n, long k, bool f32) {
   auto tiles = [](long a, long b) {
     return (long)ceil_div(a, 32) * ceil_div(b, 32);
   };
-  if (!f32 && linear_reads_any_rows(m)) return n <= 4096 && tiles(n, k) <= 4096;
   return m <= 2048 && n <= 2048 && tiles(m, k) <= 768 && tiles(n, k) <= 1024;
 }
 
@@ -1394,11 +1434,11 @@ void launch_linear_backward_small(SmallBackward<T> p, hipStream_t s) {
                                        const EpilogueArgs<T>&,               \
                                        const LinearPlan&, hipStream_t);      \
   template void launch_linear_dx<T>(T*, float*, const T*, const T*,          \
-                                    const GemmArgs&, const LinearPlan&,      \
-                                    hipStream_t);                            \
+                                    const T*, const GemmArgs&,               \
+                                    const LinearPlan&, hipStream_t);         \
   template void launch_linear_dw<T>(T*, float*, const T*, const T*,          \
-                                    const GemmArgs&, const LinearPlan&,      \
-                                    hipStream_t);                            \
+                                    const T*, const GemmArgs&,               \
+                                    const LinearPlan&, hipStream_t);         \
   template void launch_pad_rows<T>(const PadArgs<T>&, const PadArgs<T>&,     \
                                    hipStream_t);                             \
   template void launch_linear_dz<T>(T*, T*, long, float*, const T*, long,    \

@@ -218,7 +218,8 @@ struct EpilogueArgs {
   const T* residual;  // forward: [M, N] with rows of res_stride, or null
   long res_stride;
   float* z;     // forward: [M, N] or null
-  T* dz_low;    // slope: the rest of dz (split), or null
+  T* dz_low;    // slope: the rest of a bf16 dz (split)
+  const T* a_low;  // dx, dw: that rest, the left operand a second time, or null
   const T* dy;  // slope: [M, N] with rows of dy_stride
   long dy_stride;
   // slope: sums over the rows of each row of tiles, or null; with k in
@@ -246,14 +247,17 @@ template <typename T>
 void launch_linear_slope(T* dz, const T* x, const T* w, const GemmArgs& g,
                          const EpilogueArgs<T>& e, const LinearPlan&,
                          hipStream_t);
-// dx[M, N] = alpha dz[M, K] W[K, N]
+// dx[M, N] = alpha dz[M, K] W[K, N]; dz_low: the rest of dz, or null. The plan
+// is that of a K twice as long where there is a rest.
 template <typename T>
-void launch_linear_dx(T* dx, float* partial, const T* dz, const T* w,
-                      const GemmArgs& g, const LinearPlan&, hipStream_t);
-// dw[M, N] = alpha dz[K, M]^T x[K, N]
+void launch_linear_dx(T* dx, float* partial, const T* dz, const T* dz_low,
+                      const T* w, const GemmArgs& g, const LinearPlan&,
+                      hipStream_t);
+// dw[M, N] = alpha dz[K, M]^T x[K, N], likewise
 template <typename T>
-void launch_linear_dw(T* dw, float* partial, const T* dz, const T* x,
-                      const GemmArgs& g, const LinearPlan&, hipStream_t);
+void launch_linear_dw(T* dw, float* partial, const T* dz, const T* dz_low,
+                      const T* x, const GemmArgs& g, const LinearPlan&,
+                      hipStream_t);
 // dw, dx and db (each null if not wanted) of a small layer in one launch
 template <typename T>
 struct SmallBackward {
@@ -261,9 +265,7 @@ struct SmallBackward {
   T *dw_out, *dx_out;
   void* db_out;
   bool db_f32;
-  // dz and, unless null, the rest of it: the rounding errors of a few rows do
-  // not average out
-  const T *dz, *dz_low;
+  const T *dz, *dz_low;  // dz_low: the rest of dz, or null
   const T *x, *w;
   // db: db_scale times the sums of the groups of partial, or of dz's rows
   const float* partial;
@@ -287,8 +289,8 @@ struct PadArgs {
 template <typename T>
 void launch_pad_rows(const PadArgs<T>& p0, const PadArgs<T>& p1, hipStream_t);
 
-// dz = dy * slope(z) (z and dz null: dz = dy), low (or null) the rest of it
-// (split), and, unless partial is null,
+// dz = dy * slope(z) (z and dz null: dz = dy), low the rest of it if it is
+// bf16 (split), and, unless partial is null,
 // partial[g][n] = sums of dz over the rows of group g
 int linear_dz_groups(long rows, int n);
 template <typename T>

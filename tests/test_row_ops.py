@@ -817,6 +817,60 @@ def test_captured_and_replayed(dev, m):
 
 
 # ---------------- every digit of dz ----------------
+class LinearDigits(Linear):
+    """The same call with the tolerances of a backward that keeps z and dz
+    in 32 bits: z and the slope's own operations are off by float roundings,
+    db sums dz before any rounding, and the two products read a bf16 dz as
+    the bf16 towards zero (a step off, 2 h) and the rest rounded to bf16 (h of
+    that)."""
+
+    def check_backward(self, dy, dx=None, dw=None, db=None):
+        h = HALF[self.x.dtype]
+        x2, wd = self.x.double().reshape(-1, self.x.shape[-1]), self.w.double()
+        d = dy.double().reshape(self.z.shape)
+        dz = d * self.slope
+        e_s = abs(self.gain) * (CURVE[self.act] * self.e_z
+                                + 12 * U * (1 + self.z.abs()))
+        if self.act == "linear":
+            e_s = 0 * e_s
+        e_sum = d.abs() * e_s + 2 * U * dz.abs()
+        e_dz = e_sum + 2 * h * h * dz.abs()
+        m, n, wg = dz.shape[0], dz.shape[1], abs(self.wg)
+        # sums of 2 n and 2 m products, of both parts of dz
+        for got, want, tol, what in (
+                (dx, self.wg * (dz @ wd), e_dz @ wd.abs() + (2 * n + 4) * U
+                 * ((dz.abs() + e_dz) @ wd.abs()), "dx"),
+                (dw, self.wg * (dz.t() @ x2), e_dz.t() @ x2.abs()
+                 + (2 * m + 4) * U * ((dz.abs() + e_dz).t() @ x2.abs()),
+                 "dw")):
+            if got is not None:
+                tol = wg * tol
+                within(got.reshape(want.shape), want,
+                       tol + h * (want.abs() + tol) + 1e-30, what)
+        if db is not None:
+            want = self.bg * dz.sum(0)
+            tol = abs(self.bg) * (e_sum.sum(0) + (m + 4) * U
+                                  * (dz.abs() + e_sum).sum(0))
+            within(db, want, tol + HALF[db.dtype] * (want.abs() + tol)
+                   + 1e-30, "db")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [a for a in ACTS if a != "linear"])
+@pytest.mark.parametrize("m,k,n", [
+    (1, 64, 72), (20, 515, 130), (2, 1024, 8200), (33, 64, 40), (300, 72, 520),
+    (1037, 515, 771), (40, 1600, 33), (2100, 1700, 200), (5000, 256, 264),
+    (20000, 136, 520)])
+def test_linear_act_rounds_its_gradients_once(dev, act, m, k, n):
+    """bf16 gradients are those of a dz in 32 bits, rounded at the end: few
+    rows and many, z kept and z from the product again, every tile."""
+    x, w, b, res = linear_inputs(dev, m, k, n, BF16)
+    linear_grads(LinearDigits(x, w, b, res, act, wg=1 / math.sqrt(k)), dev,
+                 poisoned=True)
+    linear_grads(LinearDigits(x, w, None, None, act, clamp=0.6, gain=1.7,
+                              wg=1 / math.sqrt(k)), dev)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("gain", [1.0, 1.3])
 @pytest.mark.parametrize("m,k,n", [(5, 72, 40), (64, 72, 40), (30, 1600, 33),
