@@ -273,16 +273,19 @@ std::vector<int64_t> out_shape(const Tensor& x, int64_t n) {
 }
 
 // The tiles read rows of 16-byte granules: rows elsewhere, or of another
-// width, are copied to padded ones (zeros behind the last element). up to two
-// tensors in one launch.
+// width, are copied to padded ones (zeros behind the last element). So are rows
+// that repeat or overlap where a product sums over them (`summed`): the last
+// tile's end is found by the operand's, which has to lie before the row after
+// the last. Up to two tensors in one launch.
 template <typename T>
 struct TileRows {
   Room room;
   gfa::PadArgs<T> pad{};
 
-  void add(Rows& r, int64_t n) {
+  void add(Rows& r, int64_t n, bool summed = false) {
     const int64_t v = 16 / sizeof(T);
     if (n % v == 0 && r.stride % v == 0 && r.stride < (1 << 20) &&
+        (!summed || r.stride >= n) &&
         reinterpret_cast<uintptr_t>(r.at) % 16 == 0)
       return;
     const int64_t width = (n + 7) / 8 * 8;
@@ -389,8 +392,8 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
     Rows xr = rows_of(x), wr = rows_of(w), dr = rows_of(dy);
     TileRows<scalar_t> px, pw, pd;
     const bool any = gfa::linear_reads_any_rows(m);
-    if (need_dw || (again && !any)) px.add(xr, k);
-    if (need_dx || (again && !any)) pw.add(wr, k);
+    if (need_dw || (again && !any)) px.add(xr, k, need_dw);
+    if (need_dx || (again && !any)) pw.add(wr, k, need_dx);
     pad(px, pw);
     auto e = epilogue<scalar_t>(bc, p);
     Room dz_room, partial_room, dx_parts, dw_parts;
@@ -431,7 +434,7 @@ std::tuple<OptTensor, OptTensor, OptTensor> linear_act_bwd(
                                         e.act, m, (int)n, cur_stream());
       }
       if (need_dx || need_dw) {
-        pd.add(dr, n);
+        pd.add(dr, n, need_dw);
         pad(pd);
       }
     }

@@ -250,7 +250,8 @@ struct Loader {
   static constexpr int kEach = kTile / WAVES;  // a wave's of a k-tile
   const char* at;  // the corner of the next k-tile
   long bytes;      // from there to the operand's end, whose rows end with a
-                   // whole granule
+                   // whole granule; of columns, rows behind the last k lie
+                   // outside, since none begins before the last one's end
   long step;       // from one k-tile to the next
   int left;        // k from there on
   int wave, lane;

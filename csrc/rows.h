@@ -201,7 +201,8 @@ void launch_sum_groups(P* out0, P* out1, const float* partial, int groups,
                        int n, float scale, hipStream_t);
 
 // C[m, n] = epilogue(alpha * sum_k A[m, k] B[n, k]). lda, ldb: strides of
-// the operands' rows (or columns), multiples of 16 bytes below 2^20.
+// the operands' rows (or columns), multiples of 16 bytes below 2^20; of
+// columns, no shorter than M or N.
 struct GemmArgs {
   long M, N, K;
   long lda, ldb, ldc;

@@ -894,6 +894,37 @@ def test_linear_act_infinite_gradient(dev, m, k, n, gain):
         assert torch.isfinite(dx).all() and torch.isfinite(dw).all(), where
 
 
+# ---------------- rows that repeat or overlap ----------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m", [2, 4, 80, 90, 600, 2100, 5000])
+def test_linear_act_repeated_rows(dev, dtype, m):
+    """Rows of x, of dy (the gradient of a sum over rows) and of the weight
+    that are one row, and windows that overlap: as copies of them."""
+    k, n = 72, 40
+    flat = randn(8 * m + k + n, device=dev, dtype=dtype)
+    one_w = randn(1, k, device=dev, dtype=dtype, seed=1)
+    w = randn(n, k, device=dev, dtype=dtype, seed=2)
+    xs = flat[:k].expand(m, k), flat.unfold(0, k, 8)[:m]
+    dys = flat[8:8 + n].expand(m, n), flat.unfold(0, n, 8)[:m]
+    for x in xs:
+        for weight in (w, one_w.expand(n, k)):
+            c = LinearDigits(x, weight, None, None, "linear", wg=0.1)
+            for dy in dys:
+                leaves = [x.detach().requires_grad_(),
+                          weight.detach().requires_grad_()]
+                y = linear_act(*leaves, weight_gain=0.1)
+                assert leaves[0].stride() == x.stride()
+                dx, dw = torch.autograd.grad(y, leaves, dy)
+                c.check_backward(dy, dx, dw)
+    # as a program meets it
+    v = randn(n, device=dev, dtype=dtype, seed=3)
+    w.requires_grad_()
+    linear_act(xs[0], w, weight_gain=0.1).sum(0).backward(v)
+    LinearDigits(xs[0], w.detach(), None, None, "linear", wg=0.1) \
+        .check_backward(v.expand(m, n), dw=w.grad)
+
+
 # ---------------- in the mapping network ----------------
 def mapping(residual, layers=4, dim=64):
     from gansformer_amd.models.networks import MappingNetwork
