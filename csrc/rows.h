@@ -99,10 +99,12 @@ GFA_DEV void act_values(float (&z)[N], const ActParams& p) {
     case kTanh: each([&](float z) { return tanh_of(z, unused); }); break;
     case kSigmoid: each([](float z) { return sigmoid(z); }); break;
     case kGelu:
-      // z Phi(z), without a difference of nearly equal numbers on either side
+      // z Phi(z), without a difference of nearly equal numbers on either side;
+      // past 16 the tail is 0, and z, which may be infinite, does not meet it.
+      // fmaxf and fminf drop a NaN, the tail keeps it.
       each([&](float z) {
         const float q = normal_tail(z, unused);
-        return (z <= 0.f ? 0.f : z) - fabsf(z) * q;
+        return fmaxf(z, 0.f) - fabsf(fminf(z, 16.f)) * q;
       });
       break;
     case kSilu: each([](float z) { return z * sigmoid(z); }); break;

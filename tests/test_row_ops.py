@@ -925,6 +925,35 @@ def test_linear_act_repeated_rows(dev, dtype, m):
         .check_backward(v.expand(m, n), dw=w.grad)
 
 
+# ---------------- infinite values of z ----------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("clamp", [None, 3.0])
+@pytest.mark.parametrize("m", [12, 600, 5000])
+def test_linear_act_at_infinity(dev, dtype, act, clamp, m):
+    """y where z is infinite, the type's largest value or no number, as the
+    composition has it: gelu and silu are infinite at infinity."""
+    big = torch.finfo(dtype).max
+    x = randn(m, 1, device=dev, dtype=dtype)
+    x[:8, 0] = torch.tensor([math.inf, -math.inf, math.nan, big, -big, 60.0,
+                             -60.0, 0.0], device=dev)
+    w = torch.ones(5, 1, device=dev, dtype=dtype)
+    got = linear_act(x, w, act=act, gain=1.0, clamp=clamp)
+    want = linear_act(x.cpu(), w.cpu(), act=act, gain=1.0, clamp=clamp)
+    odd = ~torch.isfinite(want)
+    assert torch.equal(got.cpu()[odd].isnan(), want[odd].isnan())
+    assert torch.equal(got.cpu()[odd].nan_to_num(1.0),
+                       want[odd].nan_to_num(1.0))
+    if clamp is None and act in ("gelu", "silu", "relu", "lrelu", "linear"):
+        assert (got[0] == math.inf).all()
+    # 8 U (1 + |z|) is the activation's own arithmetic, on either side
+    z = x.double().cpu()
+    tol = 16 * U * (1 + z.abs()) + 2 * HALF[dtype] * want.double().abs()
+    off = (got.cpu().double() - want.double()).abs()
+    assert (off <= tol)[~odd].all()
+
+
 # ---------------- in the mapping network ----------------
 def mapping(residual, layers=4, dim=64):
     from gansformer_amd.models.networks import MappingNetwork
