@@ -5,6 +5,8 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "rows.h"
 
@@ -514,14 +516,22 @@ std::vector<bool> needed(AutogradContext* ctx, const variable_list& in) {
   return need;
 }
 
-// Differentiable gradients of f(inputs) in those that need one, for a
-// backward that is itself differentiated. Through a view of each input: one
-// may come from another (a residual and what was made from it), and this
-// operator's gradient must not run on into that history.
+// Whether a backward is itself differentiated, in reverse or forward mode
+bool differentiated(const Tensor& dy) {
+  return torch::GradMode::is_enabled() || torch::autograd::isFwGradDefined(dy);
+}
+
+// Differentiable gradients of f(inputs) in those that need one, for such a
+// backward: of the inputs without the residual, whose gradient is dy. Through
+// a view of each input: one may come from another (a residual and what was
+// made from it), and this operator's gradient must not run on into that
+// history.
 template <typename F>
 variable_list composed_grads(const variable_list& in,
                              const std::vector<bool>& need, const Tensor& dy,
                              F&& f) {
+  const bool again = torch::GradMode::is_enabled();
+  torch::AutoGradMode graph(true);
   variable_list views, wanted;
   for (size_t i = 0; i < in.size(); ++i) {
     views.push_back(in[i].defined() ? in[i].view_as(in[i]) : Tensor());
@@ -531,11 +541,21 @@ variable_list composed_grads(const variable_list& in,
   if (wanted.empty()) return out;
   const variable_list got = torch::autograd::grad(
       {f(views)}, wanted, {dy}, /*retain_graph=*/std::nullopt,
-      /*create_graph=*/true);
+      /*create_graph=*/again);
   size_t k = 0;
   for (size_t i = 0; i < in.size(); ++i)
     if (need[i]) out[i] = got[k++];
   return out;
+}
+
+// Whether a call has to consist of torch's own operations: one of its tensors
+// carries a forward-mode tangent, which the kernels would drop, or the call is
+// traced, and a trace would hold their results as constants.
+bool takes_composition(const Tensor& x, const OptTensor& a, const OptTensor& b,
+                       const OptTensor& c = {}) {
+  using torch::autograd::isFwGradDefined;
+  return torch::jit::tracer::isTracing() || isFwGradDefined(x) ||
+         isFwGradDefined(a) || isFwGradDefined(b) || isFwGradDefined(c);
 }
 
 Tensor composed_layer_norm(const variable_list& in, double eps) {
@@ -559,7 +579,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto s = ctx->get_saved_variables();
     const variable_list in{s[0], s[1], s[2]};
     const auto need = needed(ctx, in);
-    if (torch::GradMode::is_enabled()) {
+    if (differentiated(dy[0])) {
       const double eps = ctx->saved_data["eps"].toDouble();
       auto out = composed_grads(in, need, dy[0], [&](const variable_list& v) {
         return composed_layer_norm(v, eps);
@@ -577,14 +597,16 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b,
                   double eps) {
   check_layer_norm(x, w, b);
+  if (takes_composition(x, w, b))
+    return composed_layer_norm({x, plain(w), plain(b)}, eps);
   if (torch::GradMode::is_enabled() &&
       (x.requires_grad() || wants_grad(w) || wants_grad(b)))
     return LayerNorm::apply(x, w, b, eps);
   return std::get<0>(layer_norm_fwd(x, w, b, eps, false));
 }
 
-// without the residual
-Tensor composed_linear_act(const variable_list& in, const LinearParams& p) {
+Tensor composed_linear_act(const variable_list& in, const LinearParams& p,
+                           const OptTensor& residual = {}) {
   Tensor z = torch::matmul(in[0].to(torch::kFloat32),
                            in[1].to(torch::kFloat32).t()) * p.weight_gain;
   if (in[2].defined()) z = z + in[2].to(torch::kFloat32) * p.bias_gain;
@@ -599,6 +621,7 @@ Tensor composed_linear_act(const variable_list& in, const LinearParams& p) {
   }
   y = y * p.gain;
   if (!std::isinf(p.clamp)) y = y.clamp(-p.clamp, p.clamp);
+  if (residual) y = y + *residual;
   return y.to(in[0].scalar_type());
 }
 
@@ -638,7 +661,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
                                 ctx->needs_input_grad(s[2].defined() ? 3 : 2)
                             ? dy[0]
                             : Tensor();
-    if (torch::GradMode::is_enabled()) {
+    if (differentiated(dy[0])) {
       auto out = composed_grads(in, need, dy[0], [&](const variable_list& v) {
         return composed_linear_act(v, p);
       });
@@ -660,6 +683,8 @@ Tensor linear_act(const Tensor& x, const Tensor& w, const OptTensor& bias,
   check_linear(x, w, bias, residual);
   CHECK_ARG(act >= 0 && act <= gfa::kSilu, "linear_act: activation ", act);
   const LinearParams p{act, alpha, gain, clamp, weight_gain, bias_gain};
+  if (takes_composition(x, w, bias, residual))
+    return composed_linear_act({x, w, plain(bias)}, p, residual);
   if (torch::GradMode::is_enabled() &&
       (x.requires_grad() || w.requires_grad() || wants_grad(bias) ||
        wants_grad(residual)))

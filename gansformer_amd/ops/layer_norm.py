@@ -9,7 +9,8 @@ a scale and shift per element) as the normalization of a TOKEN over its
 channels. The HIP kernels (csrc/layer_norm.hip) run forward and first-order
 backward, the sums over the rows for the parameters' gradients included;
 their autograd function (csrc/ext_rows.hip) sends a create_graph backward
-through a differentiable composition.
+through a differentiable composition, and so goes a call with forward-mode
+tangents or under torch.jit.trace.
 """
 
 from __future__ import annotations

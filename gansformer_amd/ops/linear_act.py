@@ -13,7 +13,8 @@ weight, a library product, a bias/activation pass and an addition. Backward:
 All products run on the kernels of csrc/linear_act.hip. A backward that
 needs z takes it from the product again, or from 32 bits kept by the forward
 where that is quicker. The autograd function (csrc/ext_rows.hip) sends a
-create_graph backward through a differentiable composition.
+create_graph backward through a differentiable composition, and so goes a call
+with forward-mode tangents or under torch.jit.trace.
 """
 
 from __future__ import annotations

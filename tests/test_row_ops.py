@@ -954,6 +954,105 @@ def test_linear_act_at_infinity(dev, dtype, act, clamp, m):
     assert (off <= tol)[~odd].all()
 
 
+# ---------------- forward mode and tracing ----------------
+def tangents(x, w, b, r, lw, lb, t):
+    """values and tangents of the two operators, of a tangent in each input"""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        d = [forward_ad.make_dual(p, q) for p, q in
+             zip((x, w, b, r, lw, lb), t)]
+        outs = [linear_act(d[0], d[1], d[2], "gelu", d[3], clamp=2.0,
+                           weight_gain=0.2),
+                layer_norm(d[0], d[4], d[5]),
+                linear_act(x, w, b, "silu", d[3]),
+                layer_norm(x, lw, d[5])]
+        pairs = [forward_ad.unpack_dual(y) for y in outs]
+        return [v.detach().clone() if v is not None else None
+                for pair in pairs for v in pair]
+
+
+def tangent_inputs(dev, dtype, grad=False):
+    x, w, b, r = linear_inputs(dev, 9, 24, 16, dtype)
+    ins = [x, w, b, r, randn(24, device=dev, seed=4),
+           randn(24, device=dev, seed=5)]
+    t = [randn(*p.shape, device=dev, dtype=p.dtype, seed=20 + i)
+         for i, p in enumerate(ins)]
+    return [p.requires_grad_(grad) for p in ins], t
+
+
+def test_tangents_cpu():
+    ins, t = tangent_inputs("cpu", torch.float64)
+    ins, t = [p.double() for p in ins], [p.double() for p in t]
+    got = tangents(*ins, t)
+    h = 1e-6
+    from torch.func import jvp
+    _, want = jvp(lambda *a: layer_norm(a[0], a[1], a[2]),
+                  (ins[0], ins[4], ins[5]), (t[0], t[4], t[5]))
+    assert torch.allclose(got[3], want)
+    up, down = ([p + s * h * q for p, q in zip(ins, t)] for s in (1, -1))
+    diff = (layer_norm(up[0], up[4], up[5])
+            - layer_norm(down[0], down[4], down[5])) / (2 * h)
+    # central differences: h^2 times a third derivative, and 1e-16 / h
+    assert torch.allclose(got[3], diff, atol=1e-6)
+    assert all(v is not None for v in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_gpu(dev, dtype, grad):
+    """A tangent in any input reaches the output, whether or not gradients
+    are wanted as well: the same composition as on the CPU, in 32 bits, of
+    sums of up to 24 terms and a handful of operations, rounded once."""
+    ins, t = tangent_inputs(dev, dtype, grad)
+    got = tangents(*ins, t)
+    want = tangents(*[p.detach().cpu() for p in ins], [p.cpu() for p in t])
+    for g, r in zip(got, want):
+        assert g is not None
+        r = r.double()
+        assert (g.double().cpu() - r).norm() <= \
+            (2 * HALF[dtype] + 128 * U) * r.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_tangent_of_the_gradient(dev, dtype):
+    """The backward pass is linear in dy: the gradients' tangents are the
+    gradients of dy's tangent, rounded once on either side."""
+    from torch.autograd import forward_ad
+    x, w, b, res = linear_inputs(dev, 9, 24, 16, dtype)
+    lw, lb = randn(24, device=dev, seed=4), randn(24, device=dev, seed=5)
+    for leaves, f in (((x, w, b, res),
+                       lambda x, w, b, r: linear_act(x, w, b, "silu", r)),
+                      ((x, lw, lb), layer_norm)):
+        leaves = [t.detach().requires_grad_() for t in leaves]
+        y = f(*leaves)
+        dy, t = (randn(*y.shape, device=dev, dtype=dtype, seed=s)
+                 for s in (6, 7))
+        want = torch.autograd.grad(y, leaves, t, retain_graph=True)
+        with forward_ad.dual_level():
+            got = torch.autograd.grad(y, leaves, forward_ad.make_dual(dy, t))
+            got = [forward_ad.unpack_dual(g).tangent for g in got]
+        for g, r in zip(got, want):
+            assert g is not None
+            assert (g.double() - r.double()).norm() <= \
+                (2 * HALF[r.dtype] + 128 * U) * r.double().norm()
+
+
+@pytest.mark.gpu
+def test_traced(dev):
+    """A trace holds the operators, not one call's results."""
+    w, b = randn(16, 24, device=dev, seed=1), randn(16, device=dev, seed=2)
+
+    def f(x):
+        h = layer_norm(x, w[0], w[1])
+        return linear_act(h, w, b, "gelu", weight_gain=0.2)
+    traced = torch.jit.trace(f, (randn(9, 24, device=dev),))
+    x = randn(9, 24, device=dev, seed=7)
+    want = f(x)
+    assert (traced(x) - want).norm() <= 256 * U * want.norm()
+
+
 # ---------------- in the mapping network ----------------
 def mapping(residual, layers=4, dim=64):
     from gansformer_amd.models.networks import MappingNetwork
