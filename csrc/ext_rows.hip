@@ -620,7 +620,11 @@ Tensor composed_linear_act(const variable_list& in, const LinearParams& p,
     case gfa::kSilu: y = z * torch::sigmoid(z); break;
   }
   y = y * p.gain;
-  if (!std::isinf(p.clamp)) y = y.clamp(-p.clamp, p.clamp);
+  // clamp's own gradient would pass where y just reaches it; the kernels' and
+  // bias_act's is 0 there
+  if (!std::isinf(p.clamp))
+    y = torch::where(y.abs() >= p.clamp, y.detach().clamp(-p.clamp, p.clamp),
+                     y);
   if (residual) y = y + *residual;
   return y.to(in[0].scalar_type());
 }

@@ -6,7 +6,7 @@
 One kernel where `linear_nobias` and `bias_act` take a scaled copy of the
 weight, a library product, a bias/activation pass and an addition. Backward:
 
-    dz = dy * gain * act'(z), zero where the clamp holds
+    dz = dy * gain * act'(z), zero where |gain * act(z)| >= clamp
     dx = weight_gain * dz @ weight      dweight = weight_gain * dz^T @ x
     dbias = bias_gain * sum_rows dz     dresidual = dy
 
@@ -52,7 +52,9 @@ def _eager_linear_act(x, weight, bias, residual, act, alpha, gain, clamp,
         z = z + bias.to(ft) * bias_gain
     y = _act(z, act, alpha) * gain
     if clamp is not None:
-        y = y.clamp(-clamp, clamp)
+        # clamp's own gradient would pass where y just reaches it; the
+        # kernels' and bias_act's is 0 there
+        y = torch.where(y.abs() >= clamp, y.detach().clamp(-clamp, clamp), y)
     if residual is not None:
         y = y + residual.to(ft)
     return y.to(x.dtype)

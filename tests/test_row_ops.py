@@ -1053,6 +1053,36 @@ def test_traced(dev):
     assert (traced(x) - want).norm() <= 256 * U * want.norm()
 
 
+# ---------------- at the clamp ----------------
+def clamp_border(dev, dtype):
+    """act(z) gain is exactly the clamp in the first two rows"""
+    x = torch.tensor([[0.5], [-0.5], [0.25], [1.0]], device=dev, dtype=dtype,
+                     requires_grad=True)
+    w = torch.ones(3, 1, device=dev, dtype=dtype)
+    y = linear_act(x, w, act="linear", gain=2.0, clamp=1.0)
+    assert torch.equal(y[:, 0], x.new_tensor([1.0, -1.0, 0.5, 1.0]))
+    want = x.new_tensor([[0.0], [0.0], [6.0], [0.0]])
+    for again in (True, False):
+        (dx,) = torch.autograd.grad(y.sum(), x, create_graph=again)
+        assert torch.equal(dx, want), again
+    x2 = torch.tensor([[math.nan]], device=dev, dtype=dtype,
+                      requires_grad=True)
+    assert linear_act(x2, w, clamp=1.0).isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, torch.float64])
+def test_clamp_border_cpu(dtype):
+    clamp_border("cpu", dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_clamp_border_gpu(dev, dtype):
+    """The gradient is 0 where the clamp is just reached, as `bias_act` has
+    it, in every way to compute it."""
+    clamp_border(dev, dtype)
+
+
 # ---------------- in the mapping network ----------------
 def mapping(residual, layers=4, dim=64):
     from gansformer_amd.models.networks import MappingNetwork
