@@ -144,6 +144,12 @@ def build_from_state(state: dict) -> torch.nn.Module:
 def load_variables(module: torch.nn.Module, variables, strict=True):
     sd = module.state_dict()
     variables = list(variables)
+    # A plain mapping's weights compute something else between residuals.
+    given = {n for n, _ in variables}
+    norms = [n for n in sd if n.startswith("mapping.norms.")]
+    if strict and not given.issuperset(norms):
+        raise KeyError("the pkl's mapping network is not a residual one "
+                       "(mapping_residual), the module's is")
     # Reference pickles carry TF graph-scoped names (G_synthesis/8x8/...)
     # with TF shape conventions; route those through the best-effort name
     # map (tf_name_map.py) instead of failing on every variable.

@@ -215,3 +215,27 @@ def test_tf_name_map_remaining_leaves():
     # dlatent_avg broadcasts over all k+1 latents
     assert torch.allclose(sd2["mapping.w_avg"],
                           torch.full_like(sd["mapping.w_avg"], 0.25))
+
+
+def test_plain_mapping_does_not_resume_a_residual_one(tmp_path):
+    """Its weights would be used between residuals, with norms that were
+    never trained; the other way round the norms have no place."""
+    from gansformer_amd.training.snapshot import load_resume
+    kw = dict(z_dim=32, w_dim=32, img_resolution=16, num_components=2,
+              channel_base=512, channel_max=64, bf16_res_count=0,
+              mapping_layers=2)
+    _, D = tiny_nets()
+    path = str(tmp_path / "network-snapshot-000000.pkl")
+    for residual in (False, True):
+        G = Generator(mapping_residual=residual, **kw)
+        with torch.no_grad():
+            for p in G.mapping.parameters():
+                p.normal_()
+        pkl_compat.save_network_pkl(path, G, D, G)
+        same, other = (Generator(mapping_residual=r, **kw)
+                       for r in (residual, not residual))
+        load_resume(path, same, D, same)
+        z = G.sample_z(2)
+        assert torch.equal(same.mapping(z), G.mapping(z))
+        with pytest.raises(KeyError):
+            load_resume(path, other, D, other)
