@@ -14,6 +14,11 @@ from .loss import (PathLengthRegularizer, d_logistic_loss,
 from .loop_utils import ema_update, lazy_adam
 
 
+# Per GPU, from 256x256 on: the discriminator's backward has faulted the GPU
+# at 64 images for a cause that is not known; up to 56 run clean.
+MAX_BATCH_256 = 56
+
+
 class GANTrainer:
     def __init__(self, G, D, Gs, device, batch_gpu, batch_size,
                  g_lr=0.002, d_lr=0.002, beta1=0.0, beta2=0.99, eps=1e-8,
@@ -21,6 +26,14 @@ class GANTrainer:
                  pl_weight=2.0, pl_decay=0.01, ema_kimg=10.0,
                  ema_rampup=0.05, rounds=1, bucket_mb=25.0, r1_fp32=False,
                  label_fn=None):
+        res = getattr(D, "img_resolution", 0)
+        if (torch.device(device).type == "cuda" and res >= 256
+                and batch_gpu > MAX_BATCH_256):
+            raise ValueError(
+                f"batch of {batch_gpu} per GPU at {res}x{res}: at most "
+                f"{MAX_BATCH_256} from 256x256 on, where 64 have faulted the "
+                f"GPU in the discriminator's backward; use several rounds "
+                f"(a batch size above gpus * batch per GPU) instead")
         self.G, self.D, self.Gs = G, D, Gs
         self.device = device
         self.batch_gpu = batch_gpu

@@ -94,3 +94,23 @@ def test_training_loop_conditional(tmp_path):
         dataset_args=dict(dataset="synthetic", resolution=32,
                           synthetic_size=64, label_dim=5)))
     assert out["steps"] >= 1
+
+
+def test_trainer_refuses_batches_that_fault():
+    """Refused before anything runs on the GPU: the device is only named."""
+    from gansformer_amd.models.networks import Discriminator, Generator
+    from gansformer_amd.training.trainer import GANTrainer
+    kw = dict(img_resolution=16, channel_base=256, channel_max=32,
+              bf16_res_count=0)
+    G = Generator(z_dim=32, w_dim=32, num_components=2, mapping_layers=1, **kw)
+    D = Discriminator(**kw)
+
+    def trainer(res, batch, device="cuda"):
+        D.img_resolution = res
+        return GANTrainer(G, D, G, device, batch, batch)
+    for res, batch in ((256, 57), (256, 64), (1024, 64)):
+        with pytest.raises(ValueError, match="rounds"):
+            trainer(res, batch)
+        trainer(res, batch, "cpu")
+    for res, batch in ((256, 56), (1024, 4), (128, 128)):
+        trainer(res, batch)
