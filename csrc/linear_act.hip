@@ -902,7 +902,10 @@ void linear_direct(GemmArgs g, EpilogueArgs<T> e, T* __restrict__ c,
 // all 32x32), so a block's operands pass through LDS once and its time falls
 // with k alone; their sums meet in LDS. Where that still leaves CUs idle, k
 // is split over blocks too (kPartial). 544x512x512: 5.8 us bf16, 10.2 us
-// float, which the matrix cores bound (tiles of 64: 6.7 and 14.8 us).
+// float (tiles of 64: 6.7 and 14.8 us). The product itself is 1.9 us of the
+// whole card's float rate; 272 blocks put two on some of the 256 CUs, which is
+// 3.4 us there, and the rest is the latency of eight short stages one after
+// the other and of the launch.
 constexpr int kSmallLds = 4 * 2 * 2 * 32 * 128;  // stages, operands, depth
 template <typename T, bool ACOLS, bool BCOLS, int EPI>
 GFA_DEV void small_block(char* lds, int block, const GemmArgs& g,

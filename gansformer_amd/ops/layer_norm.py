@@ -51,8 +51,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     weight, bias: [N] in x's dtype or float32 (both in the same one), or
     None for a scale of 1 and a shift of 0. Returns x's shape and dtype;
     the statistics are held in 32 bits. On the GPU x is float32 or
-    bfloat16. Rows may be strided (a slice of a wider tensor is read in
-    place as long as its last dimension is contiguous).
+    bfloat16 and N below 2^30. Rows may be strided (a slice of a wider
+    tensor is read in place as long as its last dimension is contiguous).
     """
     if x.is_cuda:  # checks its arguments likewise
         return native.require_ext().layer_norm(x, weight, bias, eps)

@@ -10,11 +10,13 @@ weight, a library product, a bias/activation pass and an addition. Backward:
     dx = weight_gain * dz @ weight      dweight = weight_gain * dz^T @ x
     dbias = bias_gain * sum_rows dz     dresidual = dy
 
-All products run on the kernels of csrc/linear_act.hip. A backward that
-needs z takes it from the product again, or from 32 bits kept by the forward
-where that is quicker. The autograd function (csrc/ext_rows.hip) sends a
-create_graph backward through a differentiable composition, and so goes a call
-with forward-mode tangents or under torch.jit.trace.
+Sums, z and dz are held in 32 bits (a bf16 dz enters its two products as two
+bf16 numbers), and every result is rounded once. All products run on the kernels
+of csrc/linear_act.hip. A backward that needs z takes it from the product
+again, or from 32 bits kept by the forward where that is quicker. The autograd
+function (csrc/ext_rows.hip) sends a create_graph backward through a
+differentiable composition, and so goes a call with forward-mode tangents or
+under torch.jit.trace.
 """
 
 from __future__ import annotations
@@ -69,8 +71,10 @@ def linear_act(x, weight, bias=None, act="linear", residual=None, alpha=None,
     float32; residual: [..., N] in x's dtype, added after the clamp. act is
     one of `linear_activations`, with `bias_act`'s default alpha and gain.
     clamp: None or negative for none. Returns [..., N] in x's dtype, rounded
-    once from 32 bits. On the GPU x is float32 or bfloat16; x, weight and
-    residual may have strided rows.
+    once from 32 bits. On the GPU x is float32 or bfloat16, the weight below
+    2^20 a side and the rows of x fewer than 2^30; x, weight and residual may
+    have strided rows, and rows that repeat or overlap (for the gradients of
+    a weight those of x and of the incoming gradient are then copied).
     """
     spec = linear_activations.get(act)
     if spec is None:
