@@ -33,8 +33,8 @@ using LdsPtr = __attribute__((address_space(3))) void*;
 // 16-byte aligned.
 //
 // What bounds it: float the matrix cores (busy 94% of the time at 4096^3, 146
-// TFLOP/s); bf16 8192x4096x4096 keeps them busy 68% (1175 TFLOP/s; dx 75%, dw
-// 79%; a copy of the operands and the result would take 32 us); a short k
+// TFLOP/s); bf16 8192x4096x4096 keeps them busy 67% (1175 TFLOP/s; dx 74%, dw
+// 78%; a copy of the operands and the result would take 32 us); a short k
 // leaves a tile's 128 KB of results, half of its 23 us at k = 512.
 //
 // LDS layout. Rows: [m][128 bytes], 16-byte granule g of row r at g ^ (r/2

@@ -872,6 +872,15 @@ def test_linear_act_rounds_its_gradients_once(dev, act, m, k, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(33000, 512, 1032), (40000, 1024, 520),
+                                   (9000, 1544, 1000)])
+def test_linear_act_rounds_large_gradients_once(dev, m, k, n):
+    """Tiles of 256, several a block, and parts of a long sum over rows."""
+    x, w, b, _ = linear_inputs(dev, m, k, n, BF16)
+    linear_grads(LinearDigits(x, w, b, None, "gelu", wg=1 / math.sqrt(k)), dev)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("gain", [1.0, 1.3])
 @pytest.mark.parametrize("m,k,n", [(5, 72, 40), (64, 72, 40), (30, 1600, 33),
                                    (2500, 136, 264), (2100, 1700, 40)])
