@@ -16,6 +16,24 @@ import torch
 import torch.distributed as dist
 
 
+# The store of this process's runs and how many it has served: a run after
+# another in the same processes takes a prefix of its own in the same store.
+# Opened anew at the same port, a rank that is done first would join the store
+# that rank 0 has not closed yet, and rank 0 would wait for it in the new one.
+_stores = {}
+
+
+def _next_store(rank, world_size, timeout):
+    addr = os.environ["MASTER_ADDR"], int(os.environ["MASTER_PORT"])
+    key = (*addr, rank, world_size)
+    if key not in _stores:
+        _stores[key] = [dist.TCPStore(*addr, world_size, is_master=rank == 0,
+                                      timeout=timeout), 0]
+    _stores[key][1] += 1
+    store, run = _stores[key]
+    return dist.PrefixStore(f"run{run}", store)
+
+
 def setup_distributed(backend=None, timeout_sec=1800):
     """Initialise from torchrun-style env vars; no-op if WORLD_SIZE<=1.
 
@@ -50,9 +68,12 @@ def setup_distributed(backend=None, timeout_sec=1800):
             backend = "nccl" if use_gpu else "gloo"
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         os.environ.setdefault("MASTER_PORT", "29571")
+        timeout = datetime.timedelta(seconds=timeout_sec)
+        # a launcher's agent keeps a store of its own (env://)
+        agent = os.environ.get("TORCHELASTIC_USE_AGENT_STORE") == "True"
         dist.init_process_group(
-            backend=backend, rank=rank, world_size=world_size,
-            timeout=datetime.timedelta(seconds=timeout_sec))
+            backend=backend, rank=rank, world_size=world_size, timeout=timeout,
+            store=None if agent else _next_store(rank, world_size, timeout))
     return rank, world_size, device
 
 

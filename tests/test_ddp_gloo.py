@@ -545,3 +545,44 @@ def test_world2_resume(tmp_path_factory):
         p.join(timeout=30)
     assert res[0][0] == res[1][0] >= 16
     assert res[0][1] >= 1
+
+
+# ---------------------------------------------------------------------------
+# One run after another in the same processes: a rank that is done first
+# must not meet the store of the run before, which rank 0 still holds.
+# ---------------------------------------------------------------------------
+
+def _worker_again(rank, world, port, q):
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world),
+                      LOCAL_RANK=str(rank), MASTER_ADDR="127.0.0.1",
+                      MASTER_PORT=str(port))
+    torch.set_num_threads(1)
+    import time
+    import torch.distributed as dist
+    from gansformer_amd.parallel.dist import cleanup, setup_distributed
+    got = []
+    for i in range(3):
+        setup_distributed(timeout_sec=20)
+        t = torch.tensor([float(rank + 10 * i)])
+        dist.all_reduce(t)
+        got.append(t.item())
+        dist.barrier()
+        if rank == 0:
+            time.sleep(1.0)
+        cleanup()
+    q.put((rank, got))
+
+
+@pytest.mark.timeout(120)
+def test_setup_again_after_cleanup():
+    world = 2
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_worker_again, args=(r, world, 29773, q),
+                         daemon=True) for r in range(world)]
+    for p in procs:
+        p.start()
+    res = dict(q.get(timeout=100) for _ in range(world))
+    for p in procs:
+        p.join(timeout=30)
+    assert res[0] == res[1] == [1.0, 21.0, 41.0]
